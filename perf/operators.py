@@ -10,7 +10,7 @@ zero point (0 ... 15, otherwise 8) per row and group of consecutive K values:
     W[n, k] = round_T((code[n, k] - zero[k // group, n]) * scale[k // group, n])
 
 ``scales`` and ``zeros`` are [K / group, N].  ``packed`` is [ceil(N / 16), ceil(K / 64), 512] bytes: tiles of 16 rows
-and 64 columns, in which the byte at (((g * 4 + t) * 4 + s) * 2 + e) * 2 + q holds column 16 s + 8 q + 2 t + e of row g
+and 64 columns, in which the byte at (((t * 8 + g) * 4 + s) * 2 + e) * 2 + q holds column 16 t + 4 s + 2 q + e of row g
 (low four bits) and of row g + 8 (high four bits).  Experts add a leading dimension to all three.
 """
 import math
@@ -119,8 +119,8 @@ def _pack(codes):
     *lead, n, k = codes.shape
     codes = torch.nn.functional.pad(codes, (0, -k % 64, 0, -n % 16))
     n16, k64 = codes.shape[-2] // 16, codes.shape[-1] // 64
-    c = codes.reshape(-1, n16, 2, 8, k64, 4, 2, 4, 2)                   # row half h, row g, tile, s, q, t, e
-    c = c.permute(2, 0, 1, 4, 3, 7, 5, 8, 6)                            # h first, then tile and byte order
+    c = codes.reshape(-1, n16, 2, 8, k64, 4, 4, 2, 2)                   # row half h, row g, tile, t, s, q, e
+    c = c.permute(2, 0, 1, 4, 5, 3, 6, 8, 7)                            # h first, then tile and byte order
     return (c[0] | (c[1] << 4)).reshape(*lead, n16, k64, 512).contiguous()
 
 
@@ -202,9 +202,9 @@ def _run_own(st):
 def _codes(packed, n, k):
     """The codes [..., n, k] of a packed weight, as fp32."""
     *lead, n16, k64, _ = packed.shape
-    b = packed.reshape(-1, n16, k64, 8, 4, 4, 2, 2)                      # g, t, s, e, q
+    b = packed.reshape(-1, n16, k64, 4, 8, 4, 2, 2)                      # t, g, s, e, q
     c = torch.stack((b & 15, b >> 4))                                   # row half first
-    c = c.permute(1, 2, 0, 4, 3, 6, 8, 5, 7)                            # tile row, h, g, tile column, s, q, t, e
+    c = c.permute(1, 2, 0, 5, 3, 4, 6, 8, 7)                            # tile row, h, g, tile column, t, s, q, e
     return c.reshape(*lead, n16 * 16, k64 * 64)[..., :n, :k].float()
 
 
@@ -328,8 +328,8 @@ def _exact_weight(packed, scales, zeros, n, k):
     dev = packed.device
     r, c = torch.arange(n, device=dev)[:, None], torch.arange(k, device=dev)[None, :]
     col = c % 64
-    s, q, t, e = col // 16, col // 8 % 2, col // 2 % 4, col % 2
-    address = ((r // 16) * packed.shape[-2] + c // 64) * 512 + (r % 8) * 64 + t * 16 + s * 4 + e * 2 + q
+    t, s, q, e = col // 16, col // 4 % 4, col // 2 % 2, col % 2
+    address = ((r // 16) * packed.shape[-2] + c // 64) * 512 + t * 128 + (r % 8) * 16 + s * 4 + e * 2 + q
     code = (packed.reshape(-1)[address].long() >> (4 * (r // 8 % 2))) & 15
     g = (c // (k // scales.shape[0])).expand(n, k)
     r = r.expand(n, k)
