@@ -304,6 +304,58 @@ VQG_API int vqg_quantize_update(const void* w, const void* idx, void* codebook_i
 VQG_API int vqg_pack12(const void* idx_u16, void* packed_out, long long values, void* stream);
 VQG_API int vqg_unpack12(const void* packed, void* idx_u16_out, long long values, void* stream);
 
+/* ---- 4-bit weights with group scales (no counterpart in the reference) ---------------------------
+ * For the layers that one or two bits per weight do not serve.  T = fp16 or bf16 (`dtype` 0 or 1) is the type
+ * of activations, scales and results:
+ *     W[n, k] = round_T((code[n, k] - zero[k / group, n]) * scale[k / group, n]),      code, zero in 0 ... 15,
+ * zero = 8 everywhere where no zero points are given.  `group` consecutive columns share a scale: 32, a
+ * multiple of 64, or K; K is a multiple of 32 and of `group`, N is any number.
+ *   packed  [ceil(N/16)][ceil(K/64)][512] bytes, 16-byte aligned: tiles of 16 rows x 64 columns; the byte at
+ *           (((t*8 + g)*4 + s)*2 + e)*2 + q of a tile holds column 16t + 4s + 2q + e of row g (low four bits) and
+ *           of row g + 8 (high four bits).  What fills up the last tiles is not used.
+ *   scales  [K/group][N] of type T;   zeros  [K/group][N] bytes or NULL
+ * Experts put a leading dimension [E] before all three.
+ *
+ * vqg_int4_gemm: Y[M, N] = X[M, K] * W^T, fp32 accumulation, one rounding to T.  Workspace of
+ *   vqg_int4_workspace_bytes() bytes (0: none is needed), 1024-byte aligned, its first
+ *   vqg_workspace_counter_bytes() zeroed once, one per stream.
+ * vqg_int4_dequant: W [E, N, K] of type T, the bits that the products multiply.
+ * vqg_int4_quantize: the format from dense weights [E, N, K] of type T.  Per group, every operation rounded to
+ *   fp32, rint to even: symmetric (zeros_out NULL) scale = round_T(max|w| / 7), code = clamp(rint(w / scale) + 8,
+ *   0, 15); with zero points lo = min(w, 0), hi = max(w, 0), scale = round_T((hi - lo) / 15), zero =
+ *   clamp(rint(-lo / scale), 0, 15), code = clamp(rint(w / scale) + zero, 0, 15).  Weights are finite.
+ * Ordering: as for vqg_gemm, weights are taken to be constant (vqg_int4_quantize is taken care of). */
+VQG_API size_t vqg_int4_workspace_bytes(int M, int N, int K);
+VQG_API int vqg_int4_gemm(const void* x, const void* packed, const void* scales, const void* zeros, void* y, int M, int N, int K,
+                          int group, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+VQG_API int vqg_int4_dequant(const void* packed, const void* scales, const void* zeros, void* w_out, int experts, int N,
+                             int K, int group, int dtype, void* stream);
+VQG_API int vqg_int4_quantize(const void* w, void* packed_out, void* scales_out, void* zeros_out, int experts, int N, int K,
+                              int group, int dtype, void* stream);
+
+/* ---- Mixture of experts (no counterpart in the reference) ----------------------------------------
+ * vqg_route_experts: which experts a token goes to.  logits [T, E] (logits_dtype 0 fp16, 1 bf16, 2 fp32);
+ *   p = softmax (scoring 0) or sigmoid (1) of the logits; choice = p + bias (fp32 [E] or NULL).  With groups > 1
+ *   the experts form `groups` equal runs; a run's score is the sum of its two largest choices (group_score 0) or
+ *   its largest (1), and only the top_groups best runs take part.  The top_k largest choices give experts_out
+ *   [T, top_k] int32 in falling order and weights_out [T, top_k] fp32 = p, divided by their sum if renormalize,
+ *   times scale.  Equal choices and equal scores go to the lower index; they are compared in 64 bits, so the
+ *   answer is that of exact arithmetic.  An expert whose logit is -inf or NaN is never chosen and takes no part in
+ *   the softmax; a slot for which nothing is left gets expert -1 and weight 0.  E <= 512, top_k <= 32, groups <= 32.
+ * vqg_int4_experts: y[t] = sum over j of weights[t, j] * down_e(SiLU(gate_e(x_t)) * up_e(x_t)), e = experts[t, j].
+ *   up_* [E, 2 * inner, hidden]: (gate, up) row pairs as in vqg_gemm_swiglu; down_* [E, hidden, inner]; both in the
+ *   4-bit format.  A slot whose expert is outside 0 ... E-1 adds nothing (a token with no expert gets zeros); the
+ *   same expert twice adds twice.  The gated product is rounded to T, all sums are fp32.  E <= 512.  Workspace of
+ *   vqg_int4_experts_workspace_bytes() bytes, 256-byte aligned, contents arbitrary. */
+VQG_API int vqg_route_experts(const void* logits, const void* bias, void* weights_out, void* experts_out, int T, int E,
+                              int top_k, int scoring, int groups, int top_groups, int group_score, int renormalize,
+                              float scale, int logits_dtype, void* stream);
+VQG_API size_t vqg_int4_experts_workspace_bytes(int T, int top_k, int E, int hidden, int inner);
+VQG_API int vqg_int4_experts(const void* x, const void* experts, const void* weights, const void* up_packed,
+                             const void* up_scales, const void* up_zeros, const void* down_packed, const void* down_scales,
+                             const void* down_zeros, void* y, int T, int top_k, int E, int hidden, int inner, int up_group,
+                             int down_group, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Failure-path self-test (no counterpart in the reference, whose kernels wait without bound,
  * e.g. the cuda::barrier waits of strategy_3/wasp/src.cu:262-319): launches one small kernel that
  * waits on an mbarrier nobody signals, with the same bounded-wait routine the pipelined kernels use

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_longlong, c_size_t, c_uint, c_ulonglong, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_uint, c_ulonglong, c_void_p, POINTER
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libvqg_b200.so")
@@ -52,6 +52,13 @@ SIGNATURES = {
     "vqg_pack12": (c_int, [c_void_p, c_void_p, c_longlong, c_void_p]),
     "vqg_unpack12": (c_int, [c_void_p, c_void_p, c_longlong, c_void_p]),
     "vqg_gemm_small_batch_noalloc": (c_int, [c_void_p] * 4 + [c_int] * 7 + [c_void_p]),
+    "vqg_int4_workspace_bytes": (c_size_t, [c_int] * 3),
+    "vqg_int4_gemm": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    "vqg_int4_dequant": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "vqg_int4_quantize": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "vqg_route_experts": (c_int, [c_void_p] * 4 + [c_int] * 8 + [c_float, c_int, c_void_p]),
+    "vqg_int4_experts_workspace_bytes": (c_size_t, [c_int] * 5),
+    "vqg_int4_experts": (c_int, [c_void_p] * 10 + [c_int] * 8 + [c_void_p, c_size_t, c_void_p]),
     "vqg_device_status": (c_int, [POINTER(c_int)]),
     "vqg_launch_count": (c_ulonglong, []),
 }

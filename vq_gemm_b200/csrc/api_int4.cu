@@ -1,0 +1,167 @@
+// extern "C" entry points of the 4-bit products, their quantiser and the experts' layer: argument checks, routes, scratch.
+#include "int4.cuh"
+
+using namespace vqg;
+
+namespace {
+
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// A group is 32 columns, a multiple of 64, or the whole row; a row is a whole number of groups.
+bool group_ok(int K, int group) { return K % 32 == 0 && group > 0 && K % group == 0 && (group == 32 || group % 64 == 0 || group == K); }
+
+int check_weight(const void* packed, const void* scales, const void* zeros, int experts, int N, int K, int group, int dtype) {
+  if (experts < 0 || N < 0 || K < 0 || (dtype != 0 && dtype != 1)) return VQG_ERR_BAD_ARG;
+  if (experts == 0 || N == 0 || K == 0) return VQG_OK;
+  if (!group_ok(K, group)) return VQG_ERR_UNSUPPORTED;
+  if (!packed || !scales || !aligned(packed, 16) || !aligned(scales, 2)) return VQG_ERR_BAD_ARG;
+  (void)zeros;   // bytes: any address
+  return VQG_OK;
+}
+
+Int4Weight weight(const void* packed, const void* scales, const void* zeros, int N, int K, int group) {
+  Int4Weight w{};
+  w.packed = static_cast<const uint8_t*>(packed);
+  w.scales = scales;
+  w.zeros = static_cast<const uint8_t*>(zeros);
+  w.N = N; w.K = K; w.group = group;
+  return w;
+}
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+// Slots up to which a batch is worked on slot by slot, without ordering it by expert.
+constexpr int kDirectSlots = 32;
+
+struct ExpertScratch {
+  size_t h, part, row_slot, chunks, n_chunks, total;
+};
+ExpertScratch expert_scratch(int T, int top_k, int E, int hidden, int inner) {
+  ExpertScratch a{};
+  const size_t slots = static_cast<size_t>(T) * top_k;
+  a.h = 0;
+  a.part = a.h + up(slots * inner * 2);
+  a.row_slot = a.part + (slots > kDirectSlots ? up(slots * hidden * 4) : 0);
+  a.chunks = a.row_slot + up(slots * 4);
+  a.n_chunks = a.chunks + up(static_cast<size_t>(expert_max_chunks(static_cast<int>(slots), E, kInt4SmallRows)) * sizeof(int4));
+  a.total = a.n_chunks + 256;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vqg_int4_workspace_bytes(int M, int N, int K) {
+  (void)M; (void)N; (void)K;
+  return 0;
+}
+
+int vqg_int4_gemm(const void* x, const void* packed, const void* scales, const void* zeros, void* y, int M, int N, int K,
+                  int group, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  (void)workspace; (void)workspace_bytes;
+  if (M < 0) return VQG_ERR_BAD_ARG;
+  const int st = check_weight(packed, scales, zeros, 1, N, K, group, dtype);
+  if (st != VQG_OK) return st;
+  if (M == 0 || N == 0) return VQG_OK;
+  if (!y || !aligned(y, 16)) return VQG_ERR_BAD_ARG;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (K == 0) return cuda_status(cudaMemsetAsync(y, 0, static_cast<size_t>(M) * N * 2, s));
+  if (!x || !aligned(x, 16)) return VQG_ERR_BAD_ARG;
+  if (ensure_status_word() != cudaSuccess) return VQG_ERR_NO_DEVICE;
+  return launch_int4_small(weight(packed, scales, zeros, N, K, group), x, y, M, dtype == 1, s);
+}
+
+int vqg_int4_dequant(const void* packed, const void* scales, const void* zeros, void* w_out, int experts, int N, int K,
+                     int group, int dtype, void* stream) {
+  const int st = check_weight(packed, scales, zeros, experts, N, K, group, dtype);
+  if (st != VQG_OK) return st;
+  if (experts == 0 || N == 0 || K == 0) return VQG_OK;
+  if (experts > 65535) return VQG_ERR_UNSUPPORTED;
+  if (!w_out || !aligned(w_out, 16)) return VQG_ERR_BAD_ARG;
+  if (ensure_status_word() != cudaSuccess) return VQG_ERR_NO_DEVICE;
+  return launch_int4_dequant(weight(packed, scales, zeros, N, K, group), w_out, experts, dtype == 1, static_cast<cudaStream_t>(stream));
+}
+
+int vqg_int4_quantize(const void* w, void* packed_out, void* scales_out, void* zeros_out, int experts, int N, int K, int group,
+                      int dtype, void* stream) {
+  const int st = check_weight(packed_out, scales_out, zeros_out, experts, N, K, group, dtype);
+  if (st != VQG_OK) return st;
+  if (experts == 0 || N == 0 || K == 0) return VQG_OK;
+  if (experts > 65535) return VQG_ERR_UNSUPPORTED;
+  if (!w || !aligned(w, 16)) return VQG_ERR_BAD_ARG;
+  if (ensure_status_word() != cudaSuccess) return VQG_ERR_NO_DEVICE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  note_weights_written(s);
+  return launch_int4_quantize(w, static_cast<uint8_t*>(packed_out), scales_out, static_cast<uint8_t*>(zeros_out), experts, N, K,
+                              group, dtype == 1, s);
+}
+
+int vqg_route_experts(const void* logits, const void* bias, void* weights_out, void* experts_out, int T, int E, int top_k,
+                      int scoring, int groups, int top_groups, int group_score, int renormalize, float scale, int logits_dtype,
+                      void* stream) {
+  if (T < 0 || E < 1 || top_k < 1 || top_k > E) return VQG_ERR_BAD_ARG;
+  if (scoring < 0 || scoring > 1 || group_score < 0 || group_score > 1 || logits_dtype < 0 || logits_dtype > 2) return VQG_ERR_BAD_ARG;
+  if (groups < 1 || E % groups != 0 || top_groups < 1 || top_groups > groups) return VQG_ERR_BAD_ARG;
+  if (E > 512 || top_k > 32 || groups > 32) return VQG_ERR_UNSUPPORTED;
+  if (T == 0) return VQG_OK;
+  if (!logits || !weights_out || !experts_out || !aligned(logits, logits_dtype == 2 ? 4 : 2) || !aligned(bias, 4) ||
+      !aligned(weights_out, 4) || !aligned(experts_out, 4))
+    return VQG_ERR_BAD_ARG;
+  if (ensure_status_word() != cudaSuccess) return VQG_ERR_NO_DEVICE;
+  return launch_route_experts(logits, logits_dtype, static_cast<const float*>(bias), static_cast<float*>(weights_out),
+                              static_cast<int*>(experts_out), T, E, top_k, scoring, groups, top_groups, group_score,
+                              renormalize != 0, scale, static_cast<cudaStream_t>(stream));
+}
+
+size_t vqg_int4_experts_workspace_bytes(int T, int top_k, int E, int hidden, int inner) {
+  if (T <= 0 || top_k <= 0 || E <= 0 || hidden <= 0 || inner <= 0) return 0;
+  return expert_scratch(T, top_k, E, hidden, inner).total;
+}
+
+int vqg_int4_experts(const void* x, const void* experts, const void* weights, const void* up_packed, const void* up_scales,
+                     const void* up_zeros, const void* down_packed, const void* down_scales, const void* down_zeros, void* y,
+                     int T, int top_k, int E, int hidden, int inner, int up_group, int down_group, int dtype, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (T < 0 || top_k < 1 || E < 1 || hidden < 1 || inner < 1 || inner > 0x3fffffff) return VQG_ERR_BAD_ARG;
+  int st = check_weight(up_packed, up_scales, up_zeros, E, 2 * inner, hidden, up_group, dtype);
+  if (st == VQG_OK) st = check_weight(down_packed, down_scales, down_zeros, E, hidden, inner, down_group, dtype);
+  if (st != VQG_OK) return st;
+  if (T == 0) return VQG_OK;
+  if (E > 512 || static_cast<long long>(T) * top_k > 0x3fffffffLL) return VQG_ERR_UNSUPPORTED;
+  if (!x || !experts || !weights || !y || !aligned(x, 16) || !aligned(y, 16) || !aligned(experts, 4) || !aligned(weights, 4))
+    return VQG_ERR_BAD_ARG;
+  const ExpertScratch at = expert_scratch(T, top_k, E, hidden, inner);
+  if (!workspace || workspace_bytes < at.total || !aligned(workspace, 256)) return VQG_ERR_WORKSPACE;
+  if (ensure_status_word() != cudaSuccess) return VQG_ERR_NO_DEVICE;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = dtype == 1;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  const Int4Weight gu = weight(up_packed, up_scales, up_zeros, 2 * inner, hidden, up_group);
+  const Int4Weight dn = weight(down_packed, down_scales, down_zeros, hidden, inner, down_group);
+  ExpertRows rows{};
+  rows.ids = static_cast<const int*>(experts);
+  rows.weights = static_cast<const float*>(weights);
+  rows.E = E; rows.top_k = top_k; rows.slots = T * top_k;
+  void* h = ws + at.h;
+  if (rows.slots <= kDirectSlots) {
+    st = launch_int4_small_gated(gu, x, h, rows, 0, bf16, s);
+    if (st != VQG_OK) return st;
+    return launch_int4_small_down_direct(dn, h, y, rows, T, bf16, s);
+  }
+  float* part = reinterpret_cast<float*>(ws + at.part);
+  int* row_slot = reinterpret_cast<int*>(ws + at.row_slot);
+  int4* chunks = reinterpret_cast<int4*>(ws + at.chunks);
+  int* n_chunks = reinterpret_cast<int*>(ws + at.n_chunks);
+  st = launch_expert_plan(rows.ids, rows.slots, E, kInt4SmallRows, row_slot, chunks, n_chunks, s);
+  if (st != VQG_OK) return st;
+  rows.row_slot = row_slot; rows.chunks = chunks; rows.n_chunks = n_chunks;
+  const int most = expert_max_chunks(rows.slots, E, kInt4SmallRows);
+  if (most > 65535) return VQG_ERR_UNSUPPORTED;
+  st = launch_int4_small_gated(gu, x, h, rows, most, bf16, s);
+  if (st == VQG_OK) st = launch_int4_small_down(dn, h, part, rows, most, bf16, s);
+  if (st == VQG_OK) st = launch_expert_combine(part, rows, y, T, hidden, bf16, s);
+  return st;
+}
+
+}  // extern "C"

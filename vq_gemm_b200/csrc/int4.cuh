@@ -1,0 +1,111 @@
+// 4-bit weights with group scales: the format, the problem descriptors and the decoding of a packed word.
+//
+//   W[n, k] = round_T((code[n, k] - zero[k / group, n]) * scale[k / group, n])        T = fp16 or bf16
+//
+// code and zero are 0 ... 15 (zero is 8 where there are no zero points), scale is of type T.  The difference is a whole
+// number of at most five bits and therefore exact in T, so W is the exact product rounded once: every kernel here
+// multiplies the same bits that the dequantisation writes.
+//
+// Storage: tiles of 16 rows x 64 columns, 512 bytes each, [ceil(N/16)][ceil(K/64)] of them.  The byte at
+// (((t*8 + g)*4 + s)*2 + e)*2 + q holds column 16t + 4s + 2q + e of row g (low four bits) and of row g + 8 (high four
+// bits).  The order is the one the hardware wants: lane t*8 + g of a warp reads its 16 bytes with one load (the warp 512
+// contiguous ones); word s of them is the A fragment of one 16x8x16 matrix instruction whose 16 columns are, for thread t
+// of a quad, 16t + 4s ... +3 -- a permutation of the tile's columns under which that thread's B fragments are 16
+// consecutive values of X; and bits i and i + 16 of a word are neighbouring columns, which one AND turns into a pair.
+// Rows and columns that fill up the last tiles hold anything; the kernels do not let them reach a result.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace vqg {
+
+struct Int4Weight {
+  const uint8_t* packed;   // [E][ceil(N/16)][ceil(K/64)][512]
+  const void* scales;      // [E][K/group][N] of type T
+  const uint8_t* zeros;    // the same shape, or null
+  int N, K, group;
+  __host__ __device__ int row_tiles() const { return (N + 15) / 16; }
+  __host__ __device__ int k_tiles() const { return (K + 63) / 64; }
+  __host__ __device__ long long expert_bytes() const { return static_cast<long long>(row_tiles()) * k_tiles() * 512; }
+  __host__ __device__ long long expert_scales() const { return static_cast<long long>(K / group) * N; }
+};
+
+// Rows of a mixture-of-experts batch.  A slot is one (token, choice) pair, slot = token * top_k + choice.  In planned form
+// the slots are ordered by expert: `row_slot[r]` is the slot of row r, and chunk c covers rows [chunk.y, chunk.y + chunk.z)
+// of expert chunk.x.  In direct form (few slots) row r is slot r and there is no plan.
+struct ExpertRows {
+  const int* ids;        // [slots] chosen expert of each slot; outside 0 ... E-1: the slot is dropped
+  const float* weights;  // [slots]
+  const int* row_slot;   // planned form: [slots]
+  const int4* chunks;    // planned form
+  const int* n_chunks;   // planned form: one number
+  int E, top_k, slots;
+};
+
+int launch_int4_small(const Int4Weight& w, const void* x, void* y, int M, bool bf16, cudaStream_t s);
+// H[r, N/2] = SiLU(gate) * up for the rows of a plan (or for every slot in direct form)
+int launch_int4_small_gated(const Int4Weight& w, const void* x, void* h, const ExpertRows& rows, int max_chunks, bool bf16,
+                            cudaStream_t s);
+// part[slot, N] fp32 = H[r] * W_e^T for the rows of a plan
+int launch_int4_small_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int max_chunks, bool bf16,
+                           cudaStream_t s);
+// y[token, N] = sum over the token's choices of weight * H[slot] W_e^T, direct form
+int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, const ExpertRows& rows, int tokens, bool bf16,
+                                  cudaStream_t s);
+constexpr int kInt4SmallRows = 32;   // rows of a chunk of the planned form
+
+int launch_int4_dequant(const Int4Weight& w, void* out, int experts, bool bf16, cudaStream_t s);
+int launch_int4_quantize(const void* w, uint8_t* packed, void* scales, uint8_t* zeros, int experts, int N, int K, int group,
+                         bool bf16, cudaStream_t s);
+
+int launch_route_experts(const void* logits, int logits_type, const float* bias, float* weights, int* ids, int T, int E,
+                         int top_k, int scoring, int groups, int top_groups, int group_score, bool renormalize, float scale,
+                         cudaStream_t s);
+// Orders the slots by expert.  row_slot [slots], chunks [max_chunks], n_chunks [1].
+int launch_expert_plan(const int* ids, int slots, int E, int chunk_rows, int* row_slot, int4* chunks, int* n_chunks,
+                       cudaStream_t s);
+inline int expert_max_chunks(int slots, int E, int chunk_rows) { return slots / chunk_rows + (slots < E ? slots : E); }
+// y[t] = sum over j of weights[t, j] * part[t * top_k + j], slots that were dropped left out
+int launch_expert_combine(const float* part, const ExpertRows& rows, void* y, int tokens, int cols, bool bf16, cudaStream_t s);
+
+#ifdef __CUDACC__
+template <bool BF16>
+struct Int4Type;
+template <>
+struct Int4Type<false> {
+  using T = __half;
+  static constexpr uint32_t kMagic = 0x64006400u;   // 1024: a code in the low mantissa bits adds its value
+  __device__ static uint32_t sub(uint32_t a, uint32_t b) { uint32_t r; asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  __device__ static uint32_t mul(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  __device__ static uint32_t offset(int zero) { return (0x6400u + static_cast<uint32_t>(zero)) * 0x10001u; }   // 1024 + zero, twice
+  __device__ static float to_float(T v) { return __half2float(v); }
+  __device__ static T from_float(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Int4Type<true> {
+  using T = __nv_bfloat16;
+  static constexpr uint32_t kMagic = 0x43004300u;   // 128
+  __device__ static uint32_t sub(uint32_t a, uint32_t b) { uint32_t r; asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  __device__ static uint32_t mul(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  __device__ static uint32_t offset(int zero) { return (0x4300u + static_cast<uint32_t>(zero)) * 0x10001u; }
+  __device__ static float to_float(T v) { return __bfloat162float(v); }
+  __device__ static T from_float(float v) { return __float2bfloat16_rn(v); }
+};
+
+// The pair of columns (2q, 2q + 1) of word `w` for row half h: (code - zero) * scale in both halves of the result.
+// `off` = Int4Type::offset(zero), `s2` = the scale twice.
+template <bool BF16, int H, int Q>
+__device__ __forceinline__ uint32_t int4_pair(uint32_t w, uint32_t off, uint32_t s2) {
+  using I = Int4Type<BF16>;
+  const uint32_t v = ((w >> (8 * Q + 4 * H)) & 0x000f000fu) | I::kMagic;
+  return I::mul(I::sub(v, off), s2);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t int4_scale2(const void* scales, long long i) {
+  return static_cast<uint32_t>(__ldg(static_cast<const unsigned short*>(scales) + i)) * 0x10001u;
+}
+#endif
+
+}  // namespace vqg

@@ -10,7 +10,7 @@ Inference only: no autograd formula is registered.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 from torch import nn
@@ -76,6 +76,53 @@ def _(x, indices, codebook, rows_per_codebook):
     if indices.shape[1] * codebook.shape[2] != x.shape[1]:
         raise RuntimeError("indices [2*N_out, K/v] and codebook [G, C, v] do not match x [M, K]")
     return x.new_empty((x.shape[0], indices.shape[0] // 2))
+
+
+@torch.library.custom_op("vq_gemm_b200::int4_linear", mutates_args=(), device_types="cuda")
+def int4_linear(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor]) -> torch.Tensor:
+    """x [M, K], packed [ceil(N/16), ceil(K/64), 512] uint8, scales [K/group, N] (and zeros, uint8) -> [M, N] of x's type."""
+    return ops.int4_gemm(x, packed, scales, zeros)
+
+
+@int4_linear.register_fake
+def _(x, packed, scales, zeros):
+    if x.dim() != 2:
+        raise RuntimeError("int4_linear expects x [M, K]")
+    N, _ = ops._int4_weight(packed, scales, zeros, x.shape[1], False)
+    return x.new_empty((x.shape[0], N))
+
+
+@torch.library.custom_op("vq_gemm_b200::route_experts", mutates_args=(), device_types="cuda")
+def route_experts(logits: torch.Tensor, top_k: int, scoring: str, bias: Optional[torch.Tensor], groups: int, top_groups: int,
+                  group_score: str, renormalize: bool, scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """logits [T, E] -> (weights [T, top_k] float32, experts [T, top_k] int32); see ``ops.route_experts``."""
+    return ops.route_experts(logits, top_k, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups,
+                             group_score=group_score, renormalize=renormalize, scale=scale)
+
+
+@route_experts.register_fake
+def _(logits, top_k, scoring, bias, groups, top_groups, group_score, renormalize, scale):
+    if logits.dim() != 2:
+        raise RuntimeError("route_experts expects logits [T, E]")
+    shape = (logits.shape[0], top_k)
+    return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32)
+
+
+@torch.library.custom_op("vq_gemm_b200::int4_experts", mutates_args=(), device_types="cuda")
+def int4_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, up_packed: torch.Tensor,
+                 up_scales: torch.Tensor, up_zeros: Optional[torch.Tensor], down_packed: torch.Tensor,
+                 down_scales: torch.Tensor, down_zeros: Optional[torch.Tensor]) -> torch.Tensor:
+    """x [T, hidden] through its chosen experts; see ``ops.int4_experts``."""
+    return ops.int4_experts(x, experts, weights, (up_packed, up_scales, up_zeros), (down_packed, down_scales, down_zeros))
+
+
+@int4_experts.register_fake
+def _(x, experts, weights, up_packed, up_scales, up_zeros, down_packed, down_scales, down_zeros):
+    if x.dim() != 2 or experts.dim() != 2 or experts.shape[0] != x.shape[0]:
+        raise RuntimeError("int4_experts expects x [T, hidden], experts and weights [T, top_k]")
+    rows, _ = ops._int4_weight(up_packed, up_scales, up_zeros, x.shape[1], True)
+    ops._int4_weight(down_packed, down_scales, down_zeros, rows // 2, True)
+    return torch.empty_like(x)
 
 
 class VQLinear(nn.Module):
@@ -219,3 +266,107 @@ class VQGatedUp(nn.Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, v={self.v}, "
                 f"entries={self.codebook.shape[1]}, rows_per_codebook={self.rows_per_codebook}")
+
+
+class Int4Linear(nn.Module):
+    """``y = x @ W^T (+ bias)`` with 4-bit weights and group scales, for the layers that one or two bits do not serve.
+
+    ``packed`` [ceil(out/16), ceil(in/64), 512] uint8, ``scales`` [in/group, out] float16 or bfloat16 -- the layer's type --
+    and optionally ``zeros`` [in/group, out] uint8, as ``quantize.int4_quantize`` makes them; ``in_features`` where it is
+    not a multiple of 64.  All are buffers.  Accepts inputs of any leading shape and casts them to the layer's type."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                 bias: Optional[torch.Tensor] = None, in_features: Optional[int] = None):
+        super().__init__()
+        self.in_features = packed.shape[-2] * 64 if in_features is None else int(in_features)
+        try:
+            self.out_features, self.group = ops._int4_weight(packed, scales, zeros, self.in_features, False)
+        except RuntimeError as e:
+            raise ValueError(str(e)) from None
+        self.register_buffer("packed", packed.contiguous())
+        self.register_buffer("scales", scales.contiguous())
+        self.register_buffer("zeros", None if zeros is None else zeros.contiguous())
+        if bias is not None and bias.shape != (self.out_features,):
+            raise ValueError("bias must be [out_features]")
+        self.register_buffer("bias", None if bias is None else bias.to(scales.dtype).contiguous())
+
+    @classmethod
+    def from_weight(cls, weight: torch.Tensor, *, group: int = 128, symmetric: bool = True,
+                    bias: Optional[torch.Tensor] = None) -> "Int4Linear":
+        """Quantises a dense [out_features, in_features] fp16 or bf16 weight on its CUDA device."""
+        from .quantize import int4_quantize
+        return cls(*int4_quantize(weight, group=group, symmetric=symmetric), bias, weight.shape[1])
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.in_features:
+            raise RuntimeError(f"last dimension {x.shape[-1]} != in_features {self.in_features}")
+        x2 = x.reshape(-1, self.in_features).to(self.scales.dtype)
+        y = torch.ops.vq_gemm_b200.int4_linear(x2.contiguous(), self.packed, self.scales, self.zeros)
+        if self.bias is not None:
+            y = y + self.bias
+        return y.reshape(*x.shape[:-1], self.out_features)
+
+    def dequantized_weight(self) -> torch.Tensor:
+        """The dense [out_features, in_features] weight this layer stands for, bit for bit."""
+        return ops.int4_dequant(self.packed, self.scales, self.zeros, in_features=self.in_features)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, "
+                f"zeros={self.zeros is not None}, bias={self.bias is not None}")
+
+
+class Int4Experts(nn.Module):
+    """Mixture-of-experts MLP with 4-bit experts: ``router`` (a module that gives logits [..., E], e.g. an ``Int4Linear``, a
+    ``VQLinear`` or an ``nn.Linear``), then ``route_experts``, then the gated products of the chosen experts.
+
+    ``gate_up`` and ``down`` are (packed, scales, zeros or None) of [E, 2 * inner, hidden] and [E, hidden, inner] weights;
+    ``in_features`` is hidden.  ``bias`` [E] float32 is the router's balance bias."""
+
+    def __init__(self, router: nn.Module, gate_up, down, *, top_k: int, in_features: int, scoring: str = "softmax",
+                 bias: Optional[torch.Tensor] = None, groups: int = 1, top_groups: Optional[int] = None,
+                 group_score: str = "top2", renormalize: bool = True, scale: float = 1.0):
+        super().__init__()
+        try:
+            rows, _ = ops._int4_weight(*gate_up, in_features, True)
+            hidden, _ = ops._int4_weight(*down, rows // 2, True)
+        except RuntimeError as e:
+            raise ValueError(str(e)) from None
+        if rows % 2 or hidden != in_features or down[0].shape[0] != gate_up[0].shape[0]:
+            raise ValueError("gate_up must be [E, 2 * inner, hidden] and down [E, hidden, inner]")
+        self.router = router
+        self.in_features, self.inner, self.experts = in_features, rows // 2, gate_up[0].shape[0]
+        if not 1 <= top_k <= self.experts:
+            raise ValueError(f"cannot choose {top_k} of {self.experts} experts")
+        self.top_k, self.scoring, self.groups = top_k, scoring, groups
+        self.top_groups = groups if top_groups is None else top_groups
+        self.group_score, self.renormalize, self.scale = group_score, renormalize, scale
+        for name, weight in (("gate_up", gate_up), ("down", down)):
+            for part, t in zip(("packed", "scales", "zeros"), weight):
+                self.register_buffer(f"{name}_{part}", None if t is None else t.contiguous())
+        self.register_buffer("bias", None if bias is None else bias.to(torch.float32).contiguous())
+
+    @classmethod
+    def from_weights(cls, router: nn.Module, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *, group: int = 128,
+                     symmetric: bool = True, **routing) -> "Int4Experts":
+        """Quantises dense gate, up [E, inner, hidden] and down [E, hidden, inner] weights on their CUDA device."""
+        from .quantize import int4_quantize
+        pairs = torch.stack((gate, up), dim=2).flatten(1, 2).contiguous()      # row pairs: gate row i, up row i
+        return cls(router, int4_quantize(pairs, group=group, symmetric=symmetric),
+                   int4_quantize(down, group=group, symmetric=symmetric), in_features=gate.shape[2], **routing)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.in_features:
+            raise RuntimeError(f"last dimension {x.shape[-1]} != in_features {self.in_features}")
+        x2 = x.reshape(-1, self.in_features)
+        logits = self.router(x2).contiguous()
+        weights, chosen = torch.ops.vq_gemm_b200.route_experts(
+            logits, self.top_k, self.scoring, self.bias, self.groups, self.top_groups, self.group_score, self.renormalize,
+            self.scale)
+        y = torch.ops.vq_gemm_b200.int4_experts(
+            x2.to(self.gate_up_scales.dtype).contiguous(), chosen, weights, self.gate_up_packed, self.gate_up_scales,
+            self.gate_up_zeros, self.down_packed, self.down_scales, self.down_zeros)
+        return y.reshape(x.shape)
+
+    def extra_repr(self) -> str:
+        return (f"hidden={self.in_features}, inner={self.inner}, experts={self.experts}, top_k={self.top_k}, "
+                f"scoring={self.scoring}, groups={self.groups}, top_groups={self.top_groups}")

@@ -6,6 +6,9 @@
     vq_gemm_swiglu(x, indices, codebook)   gated product SiLU(X g) * (X u) over (gate, up) row pairs
     vq_gemm_residual(x, indices, codebook) residual (multi-codebook) weights: indices [S, N, K/v], codebook [S, G, C, v]
     dequant(indices, codebook, ...)        bit-exact dequantised weights
+    int4_gemm(x, packed, scales, zeros)    4-bit weights with group scales; int4_dequant gives the weights
+    route_experts(logits, top_k, ...)      the experts each token goes to, and their weights
+    int4_experts(x, experts, weights, ...) the gated products of the chosen experts, 4-bit weights
 
 All tensors must be CUDA tensors on one device; the output is allocated by the callee on that
 device (the reference hard-codes device 0, strategy_1/src.cu:343) and the launch goes to torch's
@@ -14,7 +17,7 @@ current stream (the reference uses the legacy default stream).  Errors raise ``R
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -308,6 +311,151 @@ def dequant(indices: torch.Tensor, codebook: torch.Tensor, *, rows_per_codebook:
     with torch.cuda.device(dev):
         st = lib.vqg_dequant(indices.data_ptr(), codebook.data_ptr(), out.data_ptr(), *args, _stream_ptr(dev))
     _lib.check(st, "dequant")
+    return out
+
+
+_INT4_TYPES = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _int4_weight(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], K: int, experts: bool):
+    """(N, group) of a 4-bit weight with K input features, after checking that its tensors fit one another."""
+    if packed.dtype != torch.uint8 or scales.dtype not in _INT4_TYPES:
+        raise RuntimeError("4-bit weights need packed uint8 and scales float16 or bfloat16")
+    lead = 1 if experts else 0
+    if packed.dim() != 3 + lead or scales.dim() != 2 + lead or packed.shape[-1] != 512:
+        raise RuntimeError("4-bit weights need packed [ceil(N/16), ceil(K/64), 512] and scales [K/group, N]"
+                           + (", each with a leading dimension of experts" if experts else ""))
+    G, N = scales.shape[-2:]
+    if G < 1 or K < 1 or K % G or packed.shape[-3] != -(-N // 16) or packed.shape[-2] != -(-K // 64) or (
+            experts and packed.shape[0] != scales.shape[0]):
+        raise RuntimeError(f"packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not match K={K}")
+    group = K // G
+    if K % 32 or not (group == 32 or group % 64 == 0 or G == 1):
+        raise RuntimeError(f"K={K} in groups of {group}: K must be a multiple of 32 and a group 32, a multiple of 64, or K")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise RuntimeError("zeros must be uint8 and of the shape of scales")
+    return N, group
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def int4_gemm(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Y[M, N] = X[M, K] @ W^T for a 4-bit weight with group scales (``quantize.int4_quantize``), fp32 accumulation.
+    x, scales and Y are of one type, float16 or bfloat16; group = K // scales.shape[0]."""
+    lib = _lib.load()
+    dev = _require_cuda(x, packed, scales, *(() if zeros is None else (zeros,)))
+    if x.dim() != 2 or x.dtype != scales.dtype:
+        raise RuntimeError("x must be [M, K] and of the type of scales")
+    M, K = x.shape
+    N, group = _int4_weight(packed, scales, zeros, K, False)
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=dev)
+    elif tuple(out.shape) != (M, N) or out.dtype != x.dtype or not out.is_contiguous() or out.device != dev:
+        raise RuntimeError("out must be a contiguous [M, N] tensor of x's type on the inputs' device")
+    with torch.cuda.device(dev):
+        ws = _ws(dev, lib.vqg_int4_workspace_bytes(M, N, K))
+        st = lib.vqg_int4_gemm(x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), M, N, K, group,
+                               _INT4_TYPES[x.dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream_ptr(dev))
+    _lib.check(st, "int4_gemm")
+    return out
+
+
+def int4_dequant(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
+                 in_features: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The dense [N, K] (or [E, N, K]) weights that the 4-bit products multiply, bit for bit.  ``in_features`` is K
+    where it is not a multiple of 64."""
+    lib = _lib.load()
+    dev = _require_cuda(packed, scales, *(() if zeros is None else (zeros,)))
+    experts = packed.dim() == 4
+    K = packed.shape[-2] * 64 if in_features is None else int(in_features)
+    N, group = _int4_weight(packed, scales, zeros, K, experts)
+    E = packed.shape[0] if experts else 1
+    shape = (E, N, K) if experts else (N, K)
+    if out is None:
+        out = torch.empty(shape, dtype=scales.dtype, device=dev)
+    elif tuple(out.shape) != shape or out.dtype != scales.dtype or out.device != dev or not out.is_contiguous():
+        raise RuntimeError(f"out must be a contiguous tensor of shape {shape} and of the type of scales on {dev}")
+    with torch.cuda.device(dev):
+        st = lib.vqg_int4_dequant(packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), E, N, K, group,
+                                  _INT4_TYPES[scales.dtype], _stream_ptr(dev))
+    _lib.check(st, "int4_dequant")
+    return out
+
+
+_LOGIT_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
+                  groups: int = 1, top_groups: Optional[int] = None, group_score: str = "top2", renormalize: bool = False,
+                  scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(weights [T, top_k] float32, experts [T, top_k] int32) for router logits [T, E].
+
+    p = softmax or sigmoid of the logits; the choice goes by p + ``bias`` (float32 [E], for balance), within the
+    ``top_groups`` best of ``groups`` equal runs of experts (a run's score: the sum of its two largest choices, or with
+    ``group_score="max"`` its largest); weights are p of the chosen, divided by their sum with ``renormalize``, times
+    ``scale``.  In falling order of choice, equal ones to the lower index.  Experts with a logit of -inf or NaN are
+    never chosen; a slot for which none is left has expert -1 and weight 0."""
+    lib = _lib.load()
+    dev = _require_cuda(logits, *(() if bias is None else (bias,)))
+    if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES:
+        raise RuntimeError("logits must be [T, E], float16, bfloat16 or float32")
+    T, E = logits.shape
+    if scoring not in ("softmax", "sigmoid") or group_score not in ("top2", "max"):
+        raise RuntimeError("scoring must be softmax or sigmoid, group_score top2 or max")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
+        raise RuntimeError("bias must be a float32 [E] tensor")
+    top_groups = groups if top_groups is None else top_groups
+    if E < 1 or not 1 <= top_k <= E or groups < 1 or E % groups or not 1 <= top_groups <= groups:
+        raise RuntimeError(f"cannot choose {top_k} of {E} experts in {top_groups} of {groups} groups")
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    experts = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        st = lib.vqg_route_experts(logits.data_ptr(), _ptr(bias), weights.data_ptr(), experts.data_ptr(), T, E, top_k,
+                                   int(scoring == "sigmoid"), groups, top_groups, int(group_score == "max"),
+                                   int(renormalize), scale, _LOGIT_TYPES[logits.dtype], _stream_ptr(dev))
+    _lib.check(st, "route_experts")
+    return weights, experts
+
+
+def int4_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, gate_up: Sequence[Optional[torch.Tensor]],
+                 down: Sequence[Optional[torch.Tensor]], *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Y[t] = sum over j of weights[t, j] * down_e(SiLU(gate_e(x_t)) * up_e(x_t)), e = experts[t, j].
+
+    ``gate_up`` and ``down`` are (packed, scales, zeros or None) of 4-bit weights [E, 2 * inner, hidden] (row pairs as
+    :func:`interleave_gate_up` makes them) and [E, hidden, inner]; ``experts`` [T, top_k] int32 and ``weights`` [T, top_k]
+    float32 as :func:`route_experts` gives them.  Slots with an expert outside 0 ... E-1 add nothing."""
+    lib = _lib.load()
+    up_p, up_s, up_z = gate_up
+    dn_p, dn_s, dn_z = down
+    dev = _require_cuda(x, experts, weights, *(t for t in (up_p, up_s, up_z, dn_p, dn_s, dn_z) if t is not None))
+    if x.dim() != 2 or x.dtype != up_s.dtype or x.dtype != dn_s.dtype:
+        raise RuntimeError("x must be [T, hidden] and of the type of both weights' scales")
+    T, hidden = x.shape
+    if experts.dim() != 2 or experts.shape[0] != T or experts.dtype != torch.int32 or experts.shape[1] < 1:
+        raise RuntimeError("experts must be an int32 [T, top_k] tensor")
+    if weights.shape != experts.shape or weights.dtype != torch.float32:
+        raise RuntimeError("weights must be a float32 tensor of the shape of experts")
+    rows, up_group = _int4_weight(up_p, up_s, up_z, hidden, True)
+    if rows % 2 or rows < 2:
+        raise RuntimeError("gate_up needs an even number of rows (gate, up pairs)")
+    inner, E, top_k = rows // 2, up_p.shape[0], experts.shape[1]
+    dn_rows, down_group = _int4_weight(dn_p, dn_s, dn_z, inner, True)
+    if dn_rows != hidden or dn_p.shape[0] != E:
+        raise RuntimeError(f"down must be [{E}, {hidden}, {inner}] to follow gate_up")
+    if out is None:
+        out = torch.empty((T, hidden), dtype=x.dtype, device=dev)
+    elif tuple(out.shape) != (T, hidden) or out.dtype != x.dtype or not out.is_contiguous() or out.device != dev:
+        raise RuntimeError("out must be a contiguous [T, hidden] tensor of x's type on the inputs' device")
+    with torch.cuda.device(dev):
+        ws = torch.empty(lib.vqg_int4_experts_workspace_bytes(T, top_k, E, hidden, inner), dtype=torch.uint8, device=dev)
+        st = lib.vqg_int4_experts(x.data_ptr(), experts.data_ptr(), weights.data_ptr(), up_p.data_ptr(), up_s.data_ptr(),
+                                  _ptr(up_z), dn_p.data_ptr(), dn_s.data_ptr(), _ptr(dn_z), out.data_ptr(), T, top_k, E,
+                                  hidden, inner, up_group, down_group, _INT4_TYPES[x.dtype], ws.data_ptr(), ws.numel(),
+                                  _stream_ptr(dev))
+    _lib.check(st, "int4_experts")
     return out
 
 

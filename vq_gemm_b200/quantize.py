@@ -9,6 +9,8 @@ bench.py:83-85), so the rules are this library's own and are written down where 
 * ``kmeans_update``: one Lloyd step with exact, order-independent sums (``vqg_quantize_update``).
 * ``kmeans_quantize``: seeded initialisation from the data + ``iters`` x (assign, update) + assign.
 * ``pack12`` / ``unpack12``: 12-bit storage for indices into 4096-entry codebooks.
+* ``int4_quantize``: 4-bit codes with group scales (``vqg_int4_quantize``), for ``int4_gemm``; ``int4_pack`` /
+  ``int4_unpack`` move codes of any origin into and out of its tile order.
 
 Everything runs on the GPU through the C ABI; there is no CPU path here.
 """
@@ -155,3 +157,54 @@ def unpack12(packed: torch.Tensor) -> torch.Tensor:
         st = lib.vqg_unpack12(packed.data_ptr(), out.data_ptr(), out.numel(), _stream_ptr(dev))
     _lib.check(st, "unpack12")
     return out
+
+
+def int4_quantize(weight: torch.Tensor, *, group: int = 128, symmetric: bool = True
+                  ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """(packed, scales, zeros) of a dense fp16 or bf16 weight [N, K], or of experts' weights [E, N, K].
+
+    ``group`` consecutive columns share a scale: 32, a multiple of 64, or 0 for the whole row.  Symmetric: scale =
+    max|w| / 7, no zero points (``zeros`` is None); else scale = range / 15 and a zero point per group."""
+    lib = _lib.load()
+    dev = _require_cuda(weight)
+    if weight.dim() not in (2, 3) or weight.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("weight must be a float16 or bfloat16 [N, K] or [E, N, K] tensor")
+    lead = tuple(weight.shape[:-2])
+    N, K = weight.shape[-2:]
+    group = K if group == 0 else group
+    if N < 1 or K < 1 or K % 32 or group < 1 or K % group or not (group == 32 or group % 64 == 0 or group == K):
+        raise RuntimeError(f"K={K} in groups of {group}: K must be a multiple of 32 and a group 32, a multiple of 64, or K")
+    packed = torch.empty(lead + (-(-N // 16), -(-K // 64), 512), dtype=torch.uint8, device=dev)
+    scales = torch.empty(lead + (K // group, N), dtype=weight.dtype, device=dev)
+    zeros = None if symmetric else torch.empty(lead + (K // group, N), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        st = lib.vqg_int4_quantize(weight.data_ptr(), packed.data_ptr(), scales.data_ptr(),
+                                   None if zeros is None else zeros.data_ptr(), lead[0] if lead else 1, N, K, group,
+                                   int(weight.dtype == torch.bfloat16), _stream_ptr(dev))
+    _lib.check(st, "quantize.int4_quantize")
+    return packed, scales, zeros
+
+
+def int4_pack(codes: torch.Tensor) -> torch.Tensor:
+    """Codes [..., N, K] (uint8, 0 ... 15) in the tile order of the 4-bit products, [..., ceil(N/16), ceil(K/64), 512]: for
+    weights that were quantised elsewhere.  A layout change in torch operations, done once, on any device."""
+    if codes.dtype != torch.uint8 or codes.dim() < 2:
+        raise RuntimeError("codes must be a uint8 [..., N, K] tensor")
+    *lead, N, K = codes.shape
+    c = torch.nn.functional.pad(codes & 15, (0, -K % 64, 0, -N % 16))
+    n16, k64 = c.shape[-2] // 16, c.shape[-1] // 64
+    c = c.reshape(-1, n16, 2, 8, k64, 4, 4, 2, 2)          # half h and row g of 16 rows; t, s, q, e of 64 columns
+    c = c.permute(2, 0, 1, 4, 5, 3, 6, 8, 7)               # bytes in the order t, g, s, e, q
+    return (c[0] | (c[1] << 4)).reshape(*lead, n16, k64, 512).contiguous()
+
+
+def int4_unpack(packed: torch.Tensor, N: int, K: int) -> torch.Tensor:
+    """The codes [..., N, K] (uint8) of a packed 4-bit weight."""
+    if packed.dtype != torch.uint8 or packed.dim() < 3 or packed.shape[-1] != 512:
+        raise RuntimeError("packed must be a uint8 [..., ceil(N/16), ceil(K/64), 512] tensor")
+    *lead, n16, k64, _ = packed.shape
+    if n16 != -(-N // 16) or k64 != -(-K // 64):
+        raise RuntimeError(f"packed {tuple(packed.shape)} does not hold {N} x {K} codes")
+    b = packed.reshape(-1, n16, k64, 4, 8, 4, 2, 2)
+    c = torch.stack((b & 15, b >> 4)).permute(1, 2, 0, 5, 3, 4, 6, 8, 7)
+    return c.reshape(*lead, n16 * 16, k64 * 64)[..., :N, :K].contiguous()
