@@ -33,14 +33,20 @@ size_t up(size_t n) { return (n + 255) / 256 * 256; }
 // Slots up to which a batch is worked on slot by slot, without ordering it by expert.
 constexpr int kDirectSlots = 32;
 
+// Rows of X from which the dense product goes to the tensor-memory kernel.
+constexpr int kTensorRows = 33;
+// Rows per expert, on average, from which the experts' products do.
+bool experts_on_tensor(long long slots, int E) { return slots >= 16LL * E; }
+
 struct ExpertScratch {
-  size_t h, part, row_slot, chunks, n_chunks, total;
+  size_t h, rows, part, row_slot, chunks, n_chunks, total;
 };
 ExpertScratch expert_scratch(int T, int top_k, int E, int hidden, int inner) {
   ExpertScratch a{};
   const size_t slots = static_cast<size_t>(T) * top_k;
   a.h = 0;
-  a.part = a.h + up(slots * inner * 2);
+  a.rows = a.h + up(slots * inner * 2);
+  a.part = a.rows + (experts_on_tensor(slots, E) && slots > kDirectSlots ? up(slots * hidden * 2) : 0);
   a.row_slot = a.part + (slots > kDirectSlots ? up(slots * hidden * 4) : 0);
   a.chunks = a.row_slot + up(slots * 4);
   a.n_chunks = a.chunks + up(static_cast<size_t>(expert_max_chunks(static_cast<int>(slots), E, kInt4SmallRows)) * sizeof(int4));
@@ -53,13 +59,12 @@ ExpertScratch expert_scratch(int T, int top_k, int E, int hidden, int inner) {
 extern "C" {
 
 size_t vqg_int4_workspace_bytes(int M, int N, int K) {
-  (void)M; (void)N; (void)K;
-  return 0;
+  return M >= kTensorRows && N > 0 && K > 0 ? int4_tensor_workspace_bytes() : 0;
 }
 
 int vqg_int4_gemm(const void* x, const void* packed, const void* scales, const void* zeros, void* y, int M, int N, int K,
                   int group, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace; (void)workspace_bytes;
+
   if (M < 0) return VQG_ERR_BAD_ARG;
   const int st = check_weight(packed, scales, zeros, 1, N, K, group, dtype);
   if (st != VQG_OK) return st;
@@ -69,7 +74,12 @@ int vqg_int4_gemm(const void* x, const void* packed, const void* scales, const v
   if (K == 0) return cuda_status(cudaMemsetAsync(y, 0, static_cast<size_t>(M) * N * 2, s));
   if (!x || !aligned(x, 16)) return VQG_ERR_BAD_ARG;
   if (ensure_status_word() != cudaSuccess) return VQG_ERR_NO_DEVICE;
-  return launch_int4_small(weight(packed, scales, zeros, N, K, group), x, y, M, dtype == 1, s);
+  const Int4Weight w = weight(packed, scales, zeros, N, K, group);
+  if (M >= kTensorRows) {
+    if (!workspace || workspace_bytes < vqg_int4_workspace_bytes(M, N, K) || !aligned(workspace, 1024)) return VQG_ERR_WORKSPACE;
+    return launch_int4_tensor(w, x, y, M, dtype == 1, workspace, workspace_bytes, s);
+  }
+  return launch_int4_small(w, x, y, M, dtype == 1, s);
 }
 
 int vqg_int4_dequant(const void* packed, const void* scales, const void* zeros, void* w_out, int experts, int N, int K,
@@ -153,13 +163,20 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
   int* row_slot = reinterpret_cast<int*>(ws + at.row_slot);
   int4* chunks = reinterpret_cast<int4*>(ws + at.chunks);
   int* n_chunks = reinterpret_cast<int*>(ws + at.n_chunks);
-  st = launch_expert_plan(rows.ids, rows.slots, E, kInt4SmallRows, row_slot, chunks, n_chunks, s);
+  const bool tensor = experts_on_tensor(rows.slots, E);
+  const int chunk = tensor ? kInt4TensorRows : kInt4SmallRows, most = expert_max_chunks(rows.slots, E, chunk);
+  st = launch_expert_plan(rows.ids, rows.slots, E, chunk, row_slot, chunks, n_chunks, s);
   if (st != VQG_OK) return st;
   rows.row_slot = row_slot; rows.chunks = chunks; rows.n_chunks = n_chunks;
-  const int most = expert_max_chunks(rows.slots, E, kInt4SmallRows);
-  if (most > 65535) return VQG_ERR_UNSUPPORTED;
-  st = launch_int4_small_gated(gu, x, h, rows, most, bf16, s);
-  if (st == VQG_OK) st = launch_int4_small_down(dn, h, part, rows, most, bf16, s);
+  if (tensor) {
+    st = launch_gather_rows(x, rows, ws + at.rows, hidden, s);
+    if (st == VQG_OK) st = launch_int4_tensor_gated(gu, ws + at.rows, h, rows, most, bf16, s);
+    if (st == VQG_OK) st = launch_int4_tensor_down(dn, h, part, rows, most, bf16, s);
+  } else {
+    if (most > 65535) return VQG_ERR_UNSUPPORTED;
+    st = launch_int4_small_gated(gu, x, h, rows, most, bf16, s);
+    if (st == VQG_OK) st = launch_int4_small_down(dn, h, part, rows, most, bf16, s);
+  }
   if (st == VQG_OK) st = launch_expert_combine(part, rows, y, T, hidden, bf16, s);
   return st;
 }

@@ -40,7 +40,7 @@ struct ExpertRows {
   const float* weights;  // [slots]
   const int* row_slot;   // planned form: [slots]
   const int4* chunks;    // planned form
-  const int* n_chunks;   // planned form: one number
+  const int* n_chunks;   // planned form: number of chunks, number of rows
   int E, top_k, slots;
 };
 
@@ -56,6 +56,17 @@ int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, c
                                   cudaStream_t s);
 constexpr int kInt4SmallRows = 32;   // rows of a chunk of the planned form
 
+// Many rows: tcgen05 kernels (int4_tensor.cu).  The dense form deals out K loops evenly if it gets a workspace.
+size_t int4_tensor_workspace_bytes();
+int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool bf16, void* ws, size_t ws_bytes, cudaStream_t s);
+// rows of a plan with chunks of up to kInt4TensorRows; x_rows is X in the order of the plan (launch_gather_rows)
+int launch_int4_tensor_gated(const Int4Weight& w, const void* x_rows, void* h, const ExpertRows& rows, int max_chunks, bool bf16,
+                             cudaStream_t s);
+int launch_int4_tensor_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int max_chunks, bool bf16,
+                            cudaStream_t s);
+int launch_gather_rows(const void* x, const ExpertRows& rows, void* out, int cols, cudaStream_t s);
+constexpr int kInt4TensorRows = 256;
+
 int launch_int4_dequant(const Int4Weight& w, void* out, int experts, bool bf16, cudaStream_t s);
 int launch_int4_quantize(const void* w, uint8_t* packed, void* scales, uint8_t* zeros, int experts, int N, int K, int group,
                          bool bf16, cudaStream_t s);
@@ -63,7 +74,7 @@ int launch_int4_quantize(const void* w, uint8_t* packed, void* scales, uint8_t* 
 int launch_route_experts(const void* logits, int logits_type, const float* bias, float* weights, int* ids, int T, int E,
                          int top_k, int scoring, int groups, int top_groups, int group_score, bool renormalize, float scale,
                          cudaStream_t s);
-// Orders the slots by expert.  row_slot [slots], chunks [max_chunks], n_chunks [1].
+// Orders the slots by expert.  row_slot [slots], chunks [max_chunks], n_chunks [2].
 int launch_expert_plan(const int* ids, int slots, int E, int chunk_rows, int* row_slot, int4* chunks, int* n_chunks,
                        cudaStream_t s);
 inline int expert_max_chunks(int slots, int E, int chunk_rows) { return slots / chunk_rows + (slots < E ? slots : E); }

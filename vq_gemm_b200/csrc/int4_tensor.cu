@@ -1,0 +1,673 @@
+// Products of many rows with 4-bit weights (format: int4.cuh) on the tcgen05 tensor cores, with the weights decoded on their
+// way into tensor memory: the dense product Y = X W^T, and the two products of a mixture-of-experts layer over the rows
+// of each expert.
+//
+// The problem is transposed, D^T[n, m] = sum_k W[n, k] X[m, k]: the instruction's M dimension is 256 weight rows of a CTA
+// pair (cta_group::2), its N dimension up to 256 rows of X, A = W from tensor memory, B = X from shared memory.  A decoding
+// thread owns one weight row = one tensor-memory lane; 64 columns of it are 32 registers and one tcgen05.st.
+//
+// Roles per CTA (512 threads, four warpgroups):
+//   warp 0       TMA producer of X: this CTA's half of the rows, boxes of 32 rows x 64 columns, SWIZZLE_128B
+//   warp 1       pair leader: issues the MMAs and commits; other CTA: forwards "my operands are in place"
+//   warp 2       producer of packed weights: bulk copies of whole tiles into a ring of its own
+//   warps 4..7   epilogue
+//   warps 8..15  decoding; warps 8..11 the even, 12..15 the odd 64-column steps of a stage
+//
+// Rows of a tile: 256 at most, rounded up to 32 for the instruction, so a short tile costs what it needs on the tensor pipe.
+// Tensor memory: columns [0, 256) accumulator, [256 + 64 s, +64) A stage s (two 64-column steps).
+// Schedule of the dense product: as in tensor3.cu, the K loops of all tiles are dealt out evenly over the pairs and pieces
+// of tiles are summed in pair order by whoever arrives last.  Experts: whole tiles, dealt out in turn.
+// Every wait is bounded; no TMA load uses cluster multicast.
+#include "int4.cuh"
+#include "tc_ptx.cuh"
+
+namespace vqg {
+
+using namespace tc;
+
+namespace {
+
+constexpr int BM = 256;                  // rows of X per tile, at most
+constexpr int BNH = 128, BN = 256;       // weight rows per CTA and per pair
+constexpr int BK = 64, KS = 2;           // columns per step, steps per stage
+constexpr int STAGES = 4;
+constexpr int kThreads = 512;
+constexpr int kDecodeWarps = 8;
+constexpr uint32_t kXStep = 128 * BK * 2;                 // 16 KiB: 128 rows x 64 columns
+constexpr uint32_t kXStage = KS * kXStep;
+constexpr uint32_t kPStage = (BNH / 16) * KS * 512;       // 8 KiB of packed weights
+constexpr uint32_t kTmemCols = 512, kAccCols = 256, kStageCols = KS * BK / 2;
+constexpr uint32_t kPacked = STAGES * kXStage;
+constexpr uint32_t kStaging = kPacked + STAGES * kPStage; // [256 rows][128 weight rows] of 16 bits
+constexpr uint32_t kBars = kStaging + BM * BNH * 2;
+constexpr uint32_t kNumBars = 4 * STAGES + 3;             // full, empty, packed full, packed empty; accumulator full, empty; epilogue
+constexpr uint32_t kTmemSlot = kBars + kNumBars * 8;
+constexpr uint32_t kSmem = kTmemSlot + 16;
+static_assert(kSmem + 1024 <= 227 * 1024, "shared memory");
+static_assert(kAccCols + STAGES * kStageCols <= kTmemCols, "tensor memory");
+
+enum { kDense = 0, kGated = 1, kDown = 2 };
+
+struct TensorParams {
+  Int4Weight w;
+  void* y;
+  int* status;
+  int M;                     // dense: rows of X
+  int m_tiles, n_tiles;
+  int unit_stages, units_per_tile, q, r;   // see tensor3.cu
+  float* ws_partial;         // [pair][piece][rank][256][128] fp32
+  int* ws_counter;           // [tile][rank]
+  ExpertRows rows;
+};
+
+__device__ __forceinline__ int pair_begin(int b, int q, int r) { return b * q + (b < r ? b : r); }
+__device__ __forceinline__ int pair_of_unit(int u, int q, int r) {
+  const int big = r * (q + 1);
+  return u < big ? u / (q + 1) : r + (u - big) / q;
+}
+
+struct Segment {
+  int tile, kt_begin, kt_end, start;   // pipeline stages [kt_begin, kt_end) of the tile; first unit
+  bool whole;
+  int expert, row0, rows, n0;          // what the tile covers: rows of X, first weight row
+};
+
+// The pieces of a pair's share, in the order in which every role walks them.
+template <int MODE>
+struct Walk {
+  int lo, hi, step;
+  bool back_pending, front_first;
+  __device__ __forceinline__ Walk(int pair, int n_pairs, const TensorParams& p) {
+    if constexpr (MODE == kDense) {
+      lo = pair_begin(pair, p.q, p.r);
+      hi = pair_begin(pair + 1, p.q, p.r);
+      back_pending = (hi % p.units_per_tile) != 0;
+      front_first = (pair & 1) != 0 && (lo % p.units_per_tile) != 0;
+    } else {
+      lo = pair;
+      hi = *p.rows.n_chunks * p.n_tiles;
+      step = n_pairs;
+    }
+  }
+  __device__ __forceinline__ bool next(Segment& g, const TensorParams& p) {
+    if (lo >= hi) return false;
+    const int stages = (p.w.k_tiles() + KS - 1) / KS;
+    if constexpr (MODE == kDense) {
+      bool rev = false;
+      if (front_first) front_first = false;
+      else if (back_pending) { rev = true; back_pending = false; }
+      int end;
+      if (!rev) {
+        g.tile = lo / p.units_per_tile;
+        g.start = lo;
+        end = min(hi, (g.tile + 1) * p.units_per_tile);
+        lo = end;
+      } else {
+        g.tile = (hi - 1) / p.units_per_tile;
+        g.start = max(lo, g.tile * p.units_per_tile);
+        end = hi;
+        hi = g.start;
+      }
+      const int t0 = g.tile * p.units_per_tile;
+      g.kt_begin = (g.start - t0) * p.unit_stages;
+      g.kt_end = min((end - t0) * p.unit_stages, stages);
+      g.whole = g.start == t0 && end == t0 + p.units_per_tile;
+      g.expert = 0;
+      g.row0 = (g.tile % p.m_tiles) * BM;
+      g.rows = min(BM, p.M - g.row0);
+      g.n0 = (g.tile / p.m_tiles) * BN;
+    } else {
+      g.tile = g.start = lo;
+      lo += step;
+      g.kt_begin = 0; g.kt_end = stages; g.whole = true;
+      const int4 c = __ldg(p.rows.chunks + g.tile / p.n_tiles);
+      g.expert = c.x; g.row0 = c.y; g.rows = c.z;
+      g.n0 = (g.tile % p.n_tiles) * BN;
+    }
+    return true;
+  }
+};
+__device__ __forceinline__ int mma_rows(int rows) { return (rows + 31) & ~31; }
+
+__device__ __forceinline__ void mma_pair_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+template <bool BF16, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParams p) {
+  using I = Int4Type<BF16>;
+  using T = typename I::T;
+  extern __shared__ unsigned char smem_dyn[];
+  const uint32_t raw = smem_u32(smem_dyn);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_dyn + (base - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair_id = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  const Int4Weight& w = p.w;
+
+  auto bar_full = [&](int s) { return base + kBars + 8 * s; };
+  auto bar_empty = [&](int s) { return base + kBars + 8 * (STAGES + s); };
+  auto bar_pfull = [&](int s) { return base + kBars + 8 * (2 * STAGES + s); };
+  auto bar_pempty = [&](int s) { return base + kBars + 8 * (3 * STAGES + s); };
+  const uint32_t bar_acc_full = base + kBars + 8 * (4 * STAGES);
+  const uint32_t bar_acc_empty = base + kBars + 8 * (4 * STAGES + 1);
+  const uint32_t bar_epi = base + kBars + 8 * (4 * STAGES + 2);
+  const uint32_t to_peer = map_to_cta(base, rank ^ 1u) - base;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + kTmemSlot);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      // full: X has landed (one arrival and its bytes), eight decoding warps have written their columns; in the leader one
+      // more arrival says the same of the other CTA
+      mbar_init(bar_full(s), 1 + kDecodeWarps + (rank == 0 ? 1 : 0));
+      mbar_init(bar_empty(s), 1);
+      mbar_init(bar_pfull(s), 1);
+      mbar_init(bar_pempty(s), kDecodeWarps);
+    }
+    mbar_init(bar_acc_full, 1);
+    mbar_init(bar_acc_empty, 8);
+    mbar_init(bar_epi, 4);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kTmemSlot), "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // ------------------------------- X producer ---------------------------------------------
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        Walk<MODE> walk(pair_id, n_pairs, p);
+        Segment g;
+        while (ok && walk.next(g, p)) {
+          const int half = mma_rows(g.rows) / 2, boxes = (half + 31) / 32;
+          const int row = g.row0 + static_cast<int>(rank) * half;
+          for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+            if (!(ok = mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
+            mbar_expect_tx(bar_full(stage), KS * boxes * 4096);
+            for (int u = 0; u < KS; ++u)
+              for (int b = 0; b < boxes; ++b)
+                tma_load_2d(base + stage * kXStage + u * kXStep + b * 4096, &tmap_x, (kt * KS + u) * BK, row + 32 * b,
+                            bar_full(stage));
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        Walk<MODE> walk(pair_id, n_pairs, p);
+        Segment g;
+        if (rank == 0) {
+          // ------------------------------- MMA issuer -----------------------------------------
+          uint32_t acc_phase = 0;
+          while (ok && walk.next(g, p)) {
+            // A and B of type fp16 (0) or bf16 (1), D fp32, both K-major
+            const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) |
+                                   (static_cast<uint32_t>(mma_rows(g.rows) >> 3) << 17) | (static_cast<uint32_t>(BN >> 4) << 24);
+            if (!(ok = mbar_wait_cluster(bar_acc_empty, acc_phase ^ 1, p.status, DS_ACC_EMPTY_TIMEOUT))) break;
+            tc_fence_after();
+            for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+              if (!(ok = mbar_wait_cluster(bar_full(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
+              tc_fence_after();
+              const uint32_t a_t = tmem_base + kAccCols + static_cast<uint32_t>(stage) * kStageCols;
+#pragma unroll
+              for (int u = 0; u < KS; ++u) {
+                const uint64_t bd = make_desc(base + stage * kXStage + u * kXStep);
+#pragma unroll
+                for (int k = 0; k < BK / 16; ++k)
+                  mma_pair_ts(tmem_base, a_t + u * (BK / 2) + 8 * k, bd + 2 * k, idesc, ((kt - g.kt_begin) | u | k) != 0 ? 1u : 0u);
+              }
+              tc_commit_pair(bar_empty(stage));
+              tc_commit_pair(bar_empty(stage) + to_peer);
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            tc_commit_pair(bar_acc_full);
+            tc_commit_pair(bar_acc_full + to_peer);
+            acc_phase ^= 1;
+          }
+        } else {
+          // ------------------------------- forwarder ------------------------------------------
+          while (ok && walk.next(g, p)) {
+            for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+              if (!(ok = mbar_wait(bar_full(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
+              mbar_arrive_remote(bar_full(stage) + to_peer);
+              if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            }
+          }
+        }
+      }
+    } else if (warp == 2) {
+      // ------------------------------- packed-weight producer -----------------------------------
+      if (lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        Walk<MODE> walk(pair_id, n_pairs, p);
+        Segment g;
+        const int k_tiles = w.k_tiles();
+        while (ok && walk.next(g, p)) {
+          const int tile0 = (g.n0 + static_cast<int>(rank) * BNH) / 16;
+          const int tiles = max(0, min(BNH / 16, w.row_tiles() - tile0));
+          const uint8_t* src = w.packed + g.expert * w.expert_bytes() + static_cast<long long>(tile0) * k_tiles * 512;
+          for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+            if (!(ok = mbar_wait(bar_pempty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
+            const uint32_t bytes = min(KS, k_tiles - kt * KS) * 512;
+            mbar_expect_tx(bar_pfull(stage), tiles * bytes);
+            for (int i = 0; i < tiles; ++i)
+              bulk_load(base + kPacked + stage * kPStage + i * (KS * 512), src + (static_cast<long long>(i) * k_tiles + kt * KS) * 512,
+                        bytes, bar_pfull(stage));
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------- epilogue -----------------------------------------------------
+    // lane = weight row, column = row of X
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    const int quarter = warp & 3;
+    uint32_t acc_phase = 0, epi_phase = 0;
+    bool ok = true;
+    const uint32_t leader_acc_empty = bar_acc_empty + (rank == 0 ? 0u : to_peer);
+    unsigned char* stg = base_ptr + kStaging;
+    auto epi_sync = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_epi);
+      const bool done = mbar_wait(bar_epi, epi_phase, p.status, DS_EPILOGUE_SYNC_TIMEOUT);
+      epi_phase ^= 1;
+      return done;
+    };
+    auto release = [&]() {   // tensor memory has been read: the next tile may overwrite it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(leader_acc_empty);
+    };
+    volatile int* last_flag = reinterpret_cast<volatile int*>(base_ptr + kTmemSlot + 8);
+    constexpr int OUT_COLS = MODE == kGated ? BNH / 2 : BNH;   // output columns of this CTA's half tile
+    constexpr int ROW_BYTES = OUT_COLS * 2;
+    constexpr size_t kPartialFloats = static_cast<size_t>(BM) * BNH;
+    Walk<MODE> walk(pair_id, n_pairs, p);
+    Segment g;
+    while (ok && walk.next(g, p)) {
+      const int n0 = g.n0 + static_cast<int>(rank) * BNH;      // first weight row of this CTA
+      const int cols = mma_rows(g.rows);
+      if (!(ok = mbar_wait_cluster(bar_acc_full, acc_phase, p.status, DS_ACC_FULL_TIMEOUT))) break;
+      tc_fence_after();
+      acc_phase ^= 1;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+      if constexpr (MODE == kDown) {
+        // fp32 rows of the slots: 32 lanes are 32 consecutive floats, stored straight from the registers
+        float* part = static_cast<float*>(p.y) + n0 + quarter * 32 + lane;
+        const bool row_ok = n0 + quarter * 32 + lane < w.N;
+#pragma unroll 1
+        for (int c = 0; c < cols; c += 32) {
+          uint32_t r[32];
+          const int mine = c + lane < g.rows ? __ldg(p.rows.row_slot + g.row0 + c + lane) : -1;
+          tmem_ld32(t_row + c, r);
+          if (c + 32 >= cols) release();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int slot = __shfl_sync(0xffffffffu, mine, j);
+            if (slot >= 0 && row_ok) __stcs(part + static_cast<long long>(slot) * w.N, __uint_as_float(r[j]));
+          }
+        }
+        continue;
+      } else {
+        if (g.whole) {
+          if constexpr (MODE == kGated) {
+            // lanes 2i and 2i + 1 hold gate and up of output column i; one exchange finishes two columns of the tile
+            T* col = reinterpret_cast<T*>(stg) + ((quarter * 32 + lane) >> 1);
+            const bool odd = (lane & 1) != 0;
+            uint32_t ra[32];
+#pragma unroll 1
+            for (int c = 0; c < cols; c += 32) {
+              tmem_ld32(t_row + c, ra);
+              if (c + 32 >= cols) release();
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float send = odd ? __uint_as_float(ra[j]) : __uint_as_float(ra[j + 1]);
+                const float recv = __shfl_xor_sync(0xffffffffu, send, 1);
+                const float v = odd ? silu_mul(recv, __uint_as_float(ra[j + 1])) : silu_mul(__uint_as_float(ra[j]), recv);
+                col[(c + j + (odd ? 1 : 0)) * OUT_COLS] = I::from_float(v);
+              }
+            }
+          } else {
+            // the whole row is converted in registers and tensor memory handed back before the first store
+            uint32_t hp[BM / 2];
+            uint32_t qa[16], qb[16];
+            tmem_ld16_async(t_row, qa);
+#pragma unroll
+            for (int c = 0; c < BM / 16; c += 2) {
+              if (c * 16 < cols) {
+                tmem_ld_wait16(qa);
+                tmem_ld16_async(t_row + (c + 1) * 16, qb);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) hp[c * 8 + j] = pack_pair<BF16>(__uint_as_float(qa[2 * j]), __uint_as_float(qa[2 * j + 1]));
+                tmem_ld_wait16(qb);
+                if (c * 16 + 32 < cols) tmem_ld16_async(t_row + (c + 2) * 16, qa);
+                else release();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) hp[(c + 1) * 8 + j] = pack_pair<BF16>(__uint_as_float(qb[2 * j]), __uint_as_float(qb[2 * j + 1]));
+              }
+            }
+            unsigned short* col = reinterpret_cast<unsigned short*>(stg) + quarter * 32 + lane;
+#pragma unroll
+            for (int q = 0; q < BM / 2; ++q) {
+              if (2 * q < cols) {
+                col[(2 * q) * 128] = static_cast<unsigned short>(hp[q] & 0xffffu);
+                col[(2 * q + 1) * 128] = static_cast<unsigned short>(hp[q] >> 16);
+              }
+            }
+          }
+        } else {
+          const int slot = (g.start > g.tile * p.units_per_tile) ? 0 : 1;
+          float* part = p.ws_partial + ((static_cast<size_t>(pair_id) * 2 + slot) * 2 + rank) * kPartialFloats + quarter * 32 + lane;
+#pragma unroll 1
+          for (int c = 0; c < cols; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(t_row + c, r);
+            if (c + 32 >= cols) release();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) __stcg(part + static_cast<size_t>(c + j) * BNH, __uint_as_float(r[j]));
+          }
+          const int t0u = g.tile * p.units_per_tile;
+          const int b_first = pair_of_unit(t0u, p.q, p.r);
+          const int b_last = pair_of_unit(t0u + p.units_per_tile - 1, p.q, p.r);
+          __threadfence();
+          if (!(ok = epi_sync())) break;
+          if (warp == 4 && lane == 0) {
+            int* ctr = p.ws_counter + g.tile * 2 + static_cast<int>(rank);
+            const int last = atomicAdd(ctr, 1) == b_last - b_first;
+            if (last) *ctr = 0;
+            *last_flag = last;
+          }
+          if (!(ok = epi_sync())) break;
+          const int last = *last_flag;
+          if (!last) {
+            if (!(ok = epi_sync())) break;
+            continue;
+          }
+          __threadfence();
+          // a thread sums four weight rows of one row of X at a time, eight loads in flight per contributor
+          const int et = quarter * 32 + lane, row4 = (et & 31) * 4, msub = et >> 5;
+          constexpr int INFL = 8;
+#pragma unroll 1
+          for (int i0 = 0; i0 < cols / 4; i0 += INFL) {
+            float4 sum[INFL];
+#pragma unroll
+            for (int j = 0; j < INFL; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int b = b_first; b <= b_last; ++b) {
+              const int sl = (pair_begin(b, p.q, p.r) > t0u) ? 0 : 1;
+              const float* src = p.ws_partial + ((static_cast<size_t>(b) * 2 + sl) * 2 + rank) * kPartialFloats + row4;
+              float4 v[INFL];
+#pragma unroll
+              for (int j = 0; j < INFL; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(src + static_cast<size_t>(4 * (i0 + j) + msub) * BNH));
+#pragma unroll
+              for (int j = 0; j < INFL; ++j) { sum[j].x += v[j].x; sum[j].y += v[j].y; sum[j].z += v[j].z; sum[j].w += v[j].w; }
+            }
+#pragma unroll
+            for (int j = 0; j < INFL; ++j) {
+              uint2 o;
+              o.x = pack_pair<BF16>(sum[j].x, sum[j].y);
+              o.y = pack_pair<BF16>(sum[j].z, sum[j].w);
+              *reinterpret_cast<uint2*>(stg + (4 * (i0 + j) + msub) * 256 + row4 * 2) = o;
+            }
+          }
+        }
+        if (!(ok = epi_sync())) break;   // the whole tile is in shared memory
+        const int out_n = MODE == kGated ? w.N / 2 : w.N, out0 = MODE == kGated ? n0 / 2 : n0;
+        T* out = static_cast<T*>(p.y);
+        if (out_n % 8 == 0) {
+          constexpr int LPR = ROW_BYTES / 16, RPW = 32 / LPR;
+          const int rsel = lane / LPR, chunk = lane % LPR, ncol = out0 + chunk * 8;
+#pragma unroll 4
+          for (int m = quarter * RPW + rsel; m < g.rows; m += 4 * RPW)
+            if (ncol < out_n)
+              *reinterpret_cast<uint4*>(out + static_cast<long long>(g.row0 + m) * out_n + ncol) =
+                  *reinterpret_cast<const uint4*>(stg + m * ROW_BYTES + chunk * 16);
+        } else {   // rows that do not begin on 16 bytes: two bytes per lane, 32 neighbours together
+          for (int m = quarter; m < g.rows; m += 4)
+            for (int c = lane; c < OUT_COLS && out0 + c < out_n; c += 32)
+              out[static_cast<long long>(g.row0 + m) * out_n + out0 + c] = reinterpret_cast<const T*>(stg + m * ROW_BYTES)[c];
+        }
+        if (!(ok = epi_sync())) break;   // the staging tile is rewritten by the next one
+      }
+    }
+  } else {
+    // ------------------------------- decoding -----------------------------------------------------
+    const int quarter = warp & 3, sub = (warp - 8) >> 2;       // the step of a stage that this warp decodes
+    const int r = quarter * 32 + lane;                         // weight row in the CTA = tensor-memory lane
+    const uint32_t sh = (r & 8) ? 4 : 0;                       // rows 8 ... 15 of a tile sit in the high four bits
+    const uint32_t src = base + kPacked + (r / 16) * (KS * 512) + sub * 512 + (r & 7) * 16;
+    const uint32_t a_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols + sub * (BK / 2);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    Walk<MODE> walk(pair_id, n_pairs, p);
+    Segment g;
+    while (ok && walk.next(g, p)) {
+      const int n = g.n0 + static_cast<int>(rank) * BNH + r;
+      const bool row_ok = n < w.N;
+      const unsigned short* sc = static_cast<const unsigned short*>(w.scales) + g.expert * w.expert_scales() + n;
+      const uint8_t* ze = w.zeros ? w.zeros + g.expert * w.expert_scales() + n : nullptr;
+      // scale (twice) and offset of columns k ... k + 15; nothing there: a scale of zero, so that no fill reaches the sum
+      auto fetch = [&](int k, uint32_t& s2, uint32_t& off) {
+        s2 = 0; off = I::offset(8);
+        if (row_ok && k < w.K) {
+          const long long at = static_cast<long long>(k / w.group) * w.N;
+          s2 = __ldg(sc + at) * 0x10001u;
+          if (ze) off = I::offset(__ldg(ze + at) & 15);
+        }
+      };
+      uint32_t s_lo, s_hi, o_lo, o_hi;     // columns 0 ... 31 and 32 ... 63 of the step
+      fetch((g.kt_begin * KS + sub) * BK, s_lo, o_lo);
+      fetch((g.kt_begin * KS + sub) * BK + 32, s_hi, o_hi);
+      for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+        const uint32_t s2[2] = {s_lo, s_hi}, off[2] = {o_lo, o_hi};
+        if (kt + 1 < g.kt_end) {
+          fetch(((kt + 1) * KS + sub) * BK, s_lo, o_lo);
+          fetch(((kt + 1) * KS + sub) * BK + 32, s_hi, o_hi);
+        }
+        if (!(ok = mbar_wait(bar_pfull(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
+        uint32_t c[16], a[32];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(c[4 * t]), "=r"(c[4 * t + 1]), "=r"(c[4 * t + 2]), "=r"(c[4 * t + 3])
+                       : "r"(src + stage * kPStage + t * 128));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t v = c[i] >> sh;
+          a[2 * i] = I::mul(I::sub((v & 0x000f000fu) | I::kMagic, off[i >> 3]), s2[i >> 3]);
+          a[2 * i + 1] = I::mul(I::sub(((v >> 8) & 0x000f000fu) | I::kMagic, off[i >> 3]), s2[i >> 3]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_pempty(stage));
+        if (!(ok = mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
+        tc_fence_after();
+        tmem_st32(a_lane + static_cast<uint32_t>(stage) * kStageCols, a);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_full(stage));
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Rows of X in the order of the plan (one block per row).
+__global__ void __launch_bounds__(128)
+gather_rows_kernel(const uint4* __restrict__ x, const ExpertRows rows, uint4* __restrict__ out, int vecs) {
+  for (int r = blockIdx.x; r < rows.n_chunks[1]; r += gridDim.x) {
+    const uint4* src = x + static_cast<long long>(rows.row_slot[r] / rows.top_k) * vecs;
+    for (int i = threadIdx.x; i < vecs; i += blockDim.x) out[static_cast<long long>(r) * vecs + i] = __ldg(src + i);
+  }
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+// 16-bit row-major [rows, cols], box of 32 rows x 64 columns, zero fill (the columns that fill up the last step among it)
+bool make_x_map(CUtensorMap* map, const void* ptr, int rows, int cols, bool bf16) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+  const cuuint32_t box[2] = {BK, 32};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(ptr), dims,
+            strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+int sm_pairs() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms > 1 ? sms / 2 : 74;
+}
+constexpr size_t kPairPartialBytes = 2 * 2 * static_cast<size_t>(BM) * BNH * sizeof(float);
+
+template <typename Kernel>
+int launch(Kernel kernel, int pairs, const CUtensorMap& map, const TensorParams& p, cudaStream_t s) {
+  constexpr int smem = kSmem + 1024;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return VQG_ERR_LAUNCH;
+  kernel<<<2 * pairs, kThreads, smem, s>>>(map, p);
+  count_launch();
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+size_t int4_tensor_workspace_bytes() {
+  return kCounterBytes + static_cast<size_t>(sm_pairs()) * kPairPartialBytes;
+}
+
+int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool bf16, void* ws, size_t ws_bytes, cudaStream_t s) {
+  CUtensorMap map;
+  if (!make_x_map(&map, x, M, w.K, bf16)) return VQG_ERR_LAUNCH;
+  TensorParams p{};
+  p.w = w; p.y = y; p.M = M;
+  p.status = device_status_ptr();
+  p.m_tiles = (M + BM - 1) / BM;
+  p.n_tiles = (w.N + BN - 1) / BN;
+  const int max_pairs = sm_pairs(), stages = (w.k_tiles() + KS - 1) / KS;
+  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
+  if (tiles > 0x7fffffffLL / (stages + 1)) return VQG_ERR_UNSUPPORTED;
+  const bool split = ws && reinterpret_cast<uintptr_t>(ws) % 256 == 0 &&
+                     ws_bytes >= kCounterBytes + static_cast<size_t>(max_pairs) * kPairPartialBytes && stages > 1 &&
+                     tiles % max_pairs != 0 && tiles * 2 * sizeof(int) <= kCounterBytes;
+  p.unit_stages = split ? (stages >= 8 ? 2 : 1) : stages;
+  p.units_per_tile = (stages + p.unit_stages - 1) / p.unit_stages;
+  const long long units = tiles * p.units_per_tile;
+  const int pairs = units < max_pairs ? static_cast<int>(units) : max_pairs;
+  p.q = static_cast<int>(units / pairs);
+  p.r = static_cast<int>(units % pairs);
+  p.ws_counter = split ? static_cast<int*>(ws) : nullptr;
+  p.ws_partial = split ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes) : nullptr;
+  return bf16 ? launch(int4_tensor_kernel<true, kDense>, pairs, map, p, s) : launch(int4_tensor_kernel<false, kDense>, pairs, map, p, s);
+}
+
+namespace {
+int launch_experts(const Int4Weight& w, const void* x, void* y, const ExpertRows& rows, int max_chunks, bool bf16, bool gated,
+                   cudaStream_t s) {
+  CUtensorMap map;
+  if (!make_x_map(&map, x, rows.slots, w.K, bf16)) return VQG_ERR_LAUNCH;
+  TensorParams p{};
+  p.w = w; p.y = y; p.rows = rows;
+  p.status = device_status_ptr();
+  p.n_tiles = (w.N + BN - 1) / BN;
+  const long long most = static_cast<long long>(max_chunks) * p.n_tiles;
+  if (most > 0x7fffffffLL) return VQG_ERR_UNSUPPORTED;
+  const int pairs = most < sm_pairs() ? static_cast<int>(most) : sm_pairs();
+  if (gated) return bf16 ? launch(int4_tensor_kernel<true, kGated>, pairs, map, p, s) : launch(int4_tensor_kernel<false, kGated>, pairs, map, p, s);
+  return bf16 ? launch(int4_tensor_kernel<true, kDown>, pairs, map, p, s) : launch(int4_tensor_kernel<false, kDown>, pairs, map, p, s);
+}
+}  // namespace
+
+int launch_int4_tensor_gated(const Int4Weight& w, const void* x_rows, void* h, const ExpertRows& rows, int max_chunks, bool bf16,
+                             cudaStream_t s) {
+  return launch_experts(w, x_rows, h, rows, max_chunks, bf16, true, s);
+}
+int launch_int4_tensor_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int max_chunks, bool bf16,
+                            cudaStream_t s) {
+  return launch_experts(w, h, part, rows, max_chunks, bf16, false, s);
+}
+
+int launch_gather_rows(const void* x, const ExpertRows& rows, void* out, int cols, cudaStream_t s) {
+  const int blocks = rows.slots < 148 * 16 ? rows.slots : 148 * 16;
+  gather_rows_kernel<<<blocks, 128, 0, s>>>(static_cast<const uint4*>(x), rows, static_cast<uint4*>(out), cols / 8);
+  count_launch();
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace vqg

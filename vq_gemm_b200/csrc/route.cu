@@ -152,7 +152,8 @@ expert_plan_kernel(const int* __restrict__ ids, int slots, int E, int chunk_rows
       row0[e] = r; chunk0[e] = c;
       r += count[e]; c += (count[e] + chunk_rows - 1) / chunk_rows;
     }
-    *n_chunks = c;
+    n_chunks[0] = c;
+    n_chunks[1] = r;
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kPlanThreads)
