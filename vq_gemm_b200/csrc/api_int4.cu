@@ -13,7 +13,7 @@ bool group_ok(int K, int group) { return K % 32 == 0 && group > 0 && K % group =
 int check_weight(const void* packed, const void* scales, const void* zeros, int experts, int N, int K, int group, int dtype) {
   if (experts < 0 || N < 0 || K < 0 || (dtype != 0 && dtype != 1)) return VQG_ERR_BAD_ARG;
   if (experts == 0 || N == 0 || K == 0) return VQG_OK;
-  if (!group_ok(K, group)) return VQG_ERR_UNSUPPORTED;
+  if (!group_ok(K, group) || K > kInt4MaxK) return VQG_ERR_UNSUPPORTED;
   if (!packed || !scales || !aligned(packed, 16) || !aligned(scales, 2)) return VQG_ERR_BAD_ARG;
   (void)zeros;   // bytes: any address
   return VQG_OK;
@@ -25,6 +25,7 @@ Int4Weight weight(const void* packed, const void* scales, const void* zeros, int
   w.scales = scales;
   w.zeros = static_cast<const uint8_t*>(zeros);
   w.N = N; w.K = K; w.group = group;
+  w.group_magic = static_cast<uint32_t>(((1ULL << 32) + group / 16 - 1) / (group / 16));
   return w;
 }
 
@@ -37,6 +38,11 @@ constexpr int kDirectSlots = 32;
 constexpr int kTensorRows = 33;
 // Rows per expert, on average, from which the experts' products do.
 bool experts_on_tensor(long long slots, int E) { return slots >= 16LL * E; }
+// Rows of a chunk of an expert's rows: what most experts have, so that few read their weights twice.
+int expert_chunk_rows(long long slots, int E) {
+  if (experts_on_tensor(slots, E)) return kInt4TensorRows;
+  return slots <= 5LL * E ? 8 : slots <= 11LL * E ? 16 : 32;
+}
 
 struct ExpertScratch {
   size_t h, rows, part, row_slot, chunks, n_chunks, total;
@@ -49,7 +55,7 @@ ExpertScratch expert_scratch(int T, int top_k, int E, int hidden, int inner) {
   a.part = a.rows + (experts_on_tensor(slots, E) && slots > kDirectSlots ? up(slots * hidden * 2) : 0);
   a.row_slot = a.part + (slots > kDirectSlots ? up(slots * hidden * 4) : 0);
   a.chunks = a.row_slot + up(slots * 4);
-  a.n_chunks = a.chunks + up(static_cast<size_t>(expert_max_chunks(static_cast<int>(slots), E, kInt4SmallRows)) * sizeof(int4));
+  a.n_chunks = a.chunks + up(static_cast<size_t>(expert_max_chunks(static_cast<int>(slots), E, expert_chunk_rows(slots, E))) * sizeof(int4));
   a.total = a.n_chunks + 256;
   return a;
 }
@@ -155,7 +161,7 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
   rows.E = E; rows.top_k = top_k; rows.slots = T * top_k;
   void* h = ws + at.h;
   if (rows.slots <= kDirectSlots) {
-    st = launch_int4_small_gated(gu, x, h, rows, 0, bf16, s);
+    st = launch_int4_small_gated(gu, x, h, rows, 1, 0, bf16, s);
     if (st != VQG_OK) return st;
     return launch_int4_small_down_direct(dn, h, y, rows, T, bf16, s);
   }
@@ -164,7 +170,7 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
   int4* chunks = reinterpret_cast<int4*>(ws + at.chunks);
   int* n_chunks = reinterpret_cast<int*>(ws + at.n_chunks);
   const bool tensor = experts_on_tensor(rows.slots, E);
-  const int chunk = tensor ? kInt4TensorRows : kInt4SmallRows, most = expert_max_chunks(rows.slots, E, chunk);
+  const int chunk = expert_chunk_rows(rows.slots, E), most = expert_max_chunks(rows.slots, E, chunk);
   st = launch_expert_plan(rows.ids, rows.slots, E, chunk, row_slot, chunks, n_chunks, s);
   if (st != VQG_OK) return st;
   rows.row_slot = row_slot; rows.chunks = chunks; rows.n_chunks = n_chunks;
@@ -174,8 +180,8 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
     if (st == VQG_OK) st = launch_int4_tensor_down(dn, h, part, rows, most, bf16, s);
   } else {
     if (most > 65535) return VQG_ERR_UNSUPPORTED;
-    st = launch_int4_small_gated(gu, x, h, rows, most, bf16, s);
-    if (st == VQG_OK) st = launch_int4_small_down(dn, h, part, rows, most, bf16, s);
+    st = launch_int4_small_gated(gu, x, h, rows, chunk, most, bf16, s);
+    if (st == VQG_OK) st = launch_int4_small_down(dn, h, part, rows, chunk, most, bf16, s);
   }
   if (st == VQG_OK) st = launch_expert_combine(part, rows, y, T, hidden, bf16, s);
   return st;

@@ -38,8 +38,8 @@ int4_dequant_kernel(const Int4Weight w, void* __restrict__ out) {
     if (k >= w.K) continue;
     const uint4 c = __ldg(reinterpret_cast<const uint4*>(packed + tile * 512) + lane);
     const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-    const long long at = static_cast<long long>(k / w.group) * w.N + static_cast<long long>(e) * w.expert_scales();
-    const long long atz = static_cast<long long>(k / w.group) * w.N;
+    const long long at = static_cast<long long>(int4_group_of(w, k)) * w.N + static_cast<long long>(e) * w.expert_scales();
+    const long long atz = static_cast<long long>(int4_group_of(w, k)) * w.N;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = tr * 16 + h * 8 + g;

@@ -26,6 +26,7 @@ struct Int4Weight {
   const void* scales;      // [E][K/group][N] of type T
   const uint8_t* zeros;    // the same shape, or null
   int N, K, group;
+  uint32_t group_magic;    // ceil(2^32 / (group / 16)): see group_of()
   __host__ __device__ int row_tiles() const { return (N + 15) / 16; }
   __host__ __device__ int k_tiles() const { return (K + 63) / 64; }
   __host__ __device__ long long expert_bytes() const { return static_cast<long long>(row_tiles()) * k_tiles() * 512; }
@@ -46,15 +47,15 @@ struct ExpertRows {
 
 int launch_int4_small(const Int4Weight& w, const void* x, void* y, int M, bool bf16, cudaStream_t s);
 // H[r, N/2] = SiLU(gate) * up for the rows of a plan (or for every slot in direct form)
-int launch_int4_small_gated(const Int4Weight& w, const void* x, void* h, const ExpertRows& rows, int max_chunks, bool bf16,
-                            cudaStream_t s);
+int launch_int4_small_gated(const Int4Weight& w, const void* x, void* h, const ExpertRows& rows, int chunk_rows, int max_chunks,
+                            bool bf16, cudaStream_t s);
 // part[slot, N] fp32 = H[r] * W_e^T for the rows of a plan
-int launch_int4_small_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int max_chunks, bool bf16,
-                           cudaStream_t s);
+int launch_int4_small_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int chunk_rows, int max_chunks,
+                           bool bf16, cudaStream_t s);
 // y[token, N] = sum over the token's choices of weight * H[slot] W_e^T, direct form
 int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, const ExpertRows& rows, int tokens, bool bf16,
                                   cudaStream_t s);
-constexpr int kInt4SmallRows = 32;   // rows of a chunk of the planned form
+constexpr int kInt4SmallRows = 32;   // rows of a chunk of the planned form, at most (8, 16 or 32)
 
 // Many rows: tcgen05 kernels (int4_tensor.cu).  The dense form deals out K loops evenly if it gets a workspace.
 size_t int4_tensor_workspace_bytes();
@@ -81,7 +82,16 @@ inline int expert_max_chunks(int slots, int E, int chunk_rows) { return slots / 
 // y[t] = sum over j of weights[t, j] * part[t * top_k + j], slots that were dropped left out
 int launch_expert_combine(const float* part, const ExpertRows& rows, void* y, int tokens, int cols, bool bf16, cudaStream_t s);
 
+// K up to which 16-column runs are divided by groups with one multiplication: n / d = n * ceil(2^32 / d) >> 32 is exact while
+// n * d < 2^32, n and d at most K / 16.
+constexpr int kInt4MaxK = 1 << 19;
+
 #ifdef __CUDACC__
+// group of columns k ... k + 15 (k a multiple of 16)
+__device__ __forceinline__ int int4_group_of(const Int4Weight& w, int k) {
+  return static_cast<int>(__umulhi(static_cast<uint32_t>(k) >> 4, w.group_magic));
+}
+
 template <bool BF16>
 struct Int4Type;
 template <>
@@ -90,6 +100,7 @@ struct Int4Type<false> {
   static constexpr uint32_t kMagic = 0x64006400u;   // 1024: a code in the low mantissa bits adds its value
   __device__ static uint32_t sub(uint32_t a, uint32_t b) { uint32_t r; asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
   __device__ static uint32_t mul(uint32_t a, uint32_t b) { uint32_t r; asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+  __device__ static uint32_t fma(uint32_t a, uint32_t b, uint32_t c) { uint32_t r; asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c)); return r; }
   __device__ static uint32_t offset(int zero) { return (0x6400u + static_cast<uint32_t>(zero)) * 0x10001u; }   // 1024 + zero, twice
   __device__ static float to_float(T v) { return __half2float(v); }
   __device__ static T from_float(float v) { return __float2half_rn(v); }
@@ -105,13 +116,40 @@ struct Int4Type<true> {
   __device__ static T from_float(float v) { return __float2bfloat16_rn(v); }
 };
 
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {   // (a & b) | c
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
 // The pair of columns (2q, 2q + 1) of word `w` for row half h: (code - zero) * scale in both halves of the result.
 // `off` = Int4Type::offset(zero), `s2` = the scale twice.
 template <bool BF16, int H, int Q>
 __device__ __forceinline__ uint32_t int4_pair(uint32_t w, uint32_t off, uint32_t s2) {
   using I = Int4Type<BF16>;
-  const uint32_t v = ((w >> (8 * Q + 4 * H)) & 0x000f000fu) | I::kMagic;
-  return I::mul(I::sub(v, off), s2);
+  return I::mul(I::sub(and_or(w >> (8 * Q + 4 * H), 0x000f000fu, I::kMagic), off), s2);
+}
+// The four pairs of a word at once: rows g and g + 8, columns (0, 1) and (2, 3).  In fp16 the high codes are not shifted down:
+// 1024 + 16 code, times 1/16, minus 64 + zero is exact too and saves two shifts (bf16 has too few mantissa bits for that).
+template <bool BF16>
+__device__ __forceinline__ void int4_word(uint32_t w, uint32_t off_lo, uint32_t off_hi, uint32_t s_lo, uint32_t s_hi, uint32_t (&a)[4]) {
+  using I = Int4Type<BF16>;
+  if constexpr (BF16) {
+    a[0] = int4_pair<BF16, 0, 0>(w, off_lo, s_lo);
+    a[1] = int4_pair<BF16, 1, 0>(w, off_hi, s_hi);
+    a[2] = int4_pair<BF16, 0, 1>(w, off_lo, s_lo);
+    a[3] = int4_pair<BF16, 1, 1>(w, off_hi, s_hi);
+  } else {   // off_hi: -(64 + zero), see int4_offset_hi
+    const uint32_t v = w >> 8;
+    a[0] = I::mul(I::sub(and_or(w, 0x000f000fu, I::kMagic), off_lo), s_lo);
+    a[1] = I::mul(I::fma(and_or(w, 0x00f000f0u, I::kMagic), 0x2c002c00u, off_hi), s_hi);
+    a[2] = I::mul(I::sub(and_or(v, 0x000f000fu, I::kMagic), off_lo), s_lo);
+    a[3] = I::mul(I::fma(and_or(v, 0x00f000f0u, I::kMagic), 0x2c002c00u, off_hi), s_hi);
+  }
+}
+// what int4_word wants as the offset of row g + 8: fp16 -(64 + zero) twice (0xd400 = -64, steps of 1/16)
+template <bool BF16>
+__device__ __forceinline__ uint32_t int4_offset_hi(int zero) {
+  return BF16 ? Int4Type<BF16>::offset(zero) : (0xd400u + 16u * static_cast<uint32_t>(zero)) * 0x10001u;
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t int4_scale2(const void* scales, long long i) {

@@ -4,6 +4,8 @@
 // A warp owns R row tiles of the weight (16 rows each) and every eighth 64-column tile of K; one 16-byte load per lane and
 // tile gives the A fragments of four mma.sync m16n8k16, whose B fragments are 32 consecutive bytes of a row of X per
 // lane.  The eight warps' accumulators are summed through shared memory.
+#include <type_traits>
+
 #include "int4.cuh"
 
 namespace vqg {
@@ -19,6 +21,13 @@ struct SmallParams {
   ExpertRows rows;
 };
 
+// weights are read once: past L1
+__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 enum { kDense = 0, kGated = 1, kDown = 2 };
 
 template <bool BF16>
@@ -33,51 +42,90 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One lane's share of a weight tile, as loaded.
-struct TileRegs {
-  uint4 w;
-  uint32_t s_lo, s_hi, o_lo, o_hi;   // scales (twice) and offsets of rows g and g + 8
+// What a lane holds of B neighbouring 64-column steps of R row tiles between load and use: weights, and scales and zero
+// points of rows g and g + 8, one for every SPAN steps (2 where a group is a multiple of 128 columns).
+template <bool ZEROS, int R, int B, int SPAN>
+struct Held {
+  static constexpr int S = B / SPAN;
+  uint4 w[B][R];
+  unsigned short s_lo[S][R], s_hi[S][R];
+  uint8_t z_lo[ZEROS ? S : 1][R], z_hi[ZEROS ? S : 1][R];
 };
 
-// row0 = first row of the tile, kt = tile column, (g, t) = position of the lane
-template <bool BF16>
-__device__ __forceinline__ TileRegs load_tile(const Int4Weight& w, const uint8_t* packed, const unsigned short* scales,
-                                              const uint8_t* zeros, int tile_row, int kt, int g, int t) {
-  using I = Int4Type<BF16>;
-  TileRegs r;
-  r.w = __ldg(reinterpret_cast<const uint4*>(packed + (static_cast<long long>(tile_row) * w.k_tiles() + kt) * 512) + t * 8 + g);
-  const int k = kt * 64 + t * 16;
-  const int lo = tile_row * 16 + g, hi = lo + 8;
-  r.s_lo = r.s_hi = 0;               // a scale of zero where there is no row or column: the fill of the last tiles is not used
-  r.o_lo = r.o_hi = I::offset(8);
-  if (k < w.K) {
-    const long long at = static_cast<long long>(k / w.group) * w.N;
-    if (lo < w.N) r.s_lo = __ldg(scales + at + lo) * 0x10001u;
-    if (hi < w.N) r.s_hi = __ldg(scales + at + hi) * 0x10001u;
-    if (zeros) {
-      if (lo < w.N) r.o_lo = I::offset(__ldg(zeros + at + lo) & 15);
-      if (hi < w.N) r.o_hi = I::offset(__ldg(zeros + at + hi) & 15);
+// One expert's weight as a lane sees it.
+struct View {
+  const uint8_t* packed;          // at the lane's 16 bytes of tile (0, 0)
+  const unsigned short* scales;
+  const uint8_t* zeros;
+};
+
+// Steps kt ... kt + B - 1, all of them whole.  Rows that do not exist read the last one: their results are not written.
+template <bool ZEROS, int R, int B, int SPAN>
+__device__ __forceinline__ void load_step(Held<ZEROS, R, B, SPAN>& h, int b, const Int4Weight& w, const View& v, int tile_row, int kt,
+                                          int g, int t) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int tr = R == 1 ? tile_row : min(tile_row + i, w.row_tiles() - 1);
+    h.w[b][i] = ld_stream(v.packed + (static_cast<size_t>(tr) * w.k_tiles() + kt) * 512 + b * 512);
+    if (b % SPAN == 0) {
+      const size_t at = static_cast<size_t>(int4_group_of(w, (kt + b) * 64 + t * 16)) * w.N;
+      const int lo = min(tr * 16 + g, w.N - 1), hi = min(tr * 16 + g + 8, w.N - 1);
+      h.s_lo[b / SPAN][i] = __ldg(v.scales + at + lo);
+      h.s_hi[b / SPAN][i] = __ldg(v.scales + at + hi);
+      if constexpr (ZEROS) { h.z_lo[b / SPAN][i] = __ldg(v.zeros + at + lo); h.z_hi[b / SPAN][i] = __ldg(v.zeros + at + hi); }
     }
   }
-  return r;
 }
 
-template <bool BF16>
-__device__ __forceinline__ void decode_word(uint32_t word, const TileRegs& r, uint32_t (&a)[4]) {
-  a[0] = int4_pair<BF16, 0, 0>(word, r.o_lo, r.s_lo);
-  a[1] = int4_pair<BF16, 1, 0>(word, r.o_hi, r.s_hi);
-  a[2] = int4_pair<BF16, 0, 1>(word, r.o_lo, r.s_lo);
-  a[3] = int4_pair<BF16, 1, 1>(word, r.o_hi, r.s_hi);
+// Any steps: no column beyond K is read, and its weight is zero.
+template <bool ZEROS, int R>
+__device__ __forceinline__ void load_edge(Held<ZEROS, R, 1, 1>& h, const Int4Weight& w, const View& v, int tile_row, int kt, int g, int t) {
+  load_step<ZEROS, R, 1, 1>(h, 0, w, v, tile_row, kt, g, kt * 64 + t * 16 < w.K ? t : 0);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (kt * 64 + t * 16 >= w.K) h.s_lo[0][i] = h.s_hi[0][i] = 0;
+}
+
+// acc += W X^T over step b; x[j] are the lane's 32 bytes of row 8j + g of X
+template <bool BF16, bool ZEROS, int NT, int R, int B, int SPAN, int CH>
+__device__ __forceinline__ void multiply(const Held<ZEROS, R, B, SPAN>& h, int b, const uint4 (&x)[NT][2], float (&acc)[R][NT][CH][4]) {
+  uint32_t s_lo[R], s_hi[R], o_lo[R], o_hi[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    s_lo[i] = h.s_lo[b / SPAN][i] * 0x10001u;
+    s_hi[i] = h.s_hi[b / SPAN][i] * 0x10001u;
+    o_lo[i] = Int4Type<BF16>::offset(ZEROS ? h.z_lo[ZEROS ? b / SPAN : 0][i] & 15 : 8);
+    o_hi[i] = int4_offset_hi<BF16>(ZEROS ? h.z_hi[ZEROS ? b / SPAN : 0][i] & 15 : 8);
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const uint4& q4 = h.w[b][i];
+      const uint32_t word = s == 0 ? q4.x : s == 1 ? q4.y : s == 2 ? q4.z : q4.w;
+      uint32_t a[4];
+      int4_word<BF16>(word, o_lo[i], o_hi[i], s_lo[i], s_hi[i], a);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint4& q = x[j][s >> 1];
+        mma16816<BF16>(acc[i][j][s % CH], a, (s & 1) ? q.z : q.x, (s & 1) ? q.w : q.y);
+      }
+    }
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
-template <bool BF16, int MODE, int NT, int R>
-__global__ void __launch_bounds__(kWarps * 32)
+// Block (bx, by): row groups (R row tiles each) [groups * bx / grid, groups * (bx + 1) / grid) of the weight, rows `by` of X.
+// The eight warps take blocks of B steps in turn; a warp walks its blocks of all its row groups as one sequence in which every
+// step's registers are loaded again, for the next block, as soon as it is multiplied.
+template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int MIN_BLOCKS>
+__global__ void __launch_bounds__(kWarps * 32, MIN_BLOCKS)
 int4_small_kernel(const SmallParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
-  extern __shared__ float red[];   // [warp][R * NT * 4][lane]
+  constexpr int CH = R * NT == 1 ? 2 : 1;   // chains of accumulators: a matrix instruction waits for the one before it
+  constexpr int VALUES = R * NT * 4;        // sums of a lane per row group
+  extern __shared__ float red[];            // [row group][warp][VALUES][lane]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const Int4Weight& w = p.w;
@@ -94,94 +142,122 @@ int4_small_kernel(const SmallParams p) {
       if (expert < 0 || expert >= p.rows.E) return;
     }
   }
-  const uint8_t* packed = w.packed + expert * w.expert_bytes();
-  const unsigned short* scales = static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales();
-  const uint8_t* zeros = w.zeros ? w.zeros + expert * w.expert_scales() : nullptr;
+  const View v{w.packed + expert * w.expert_bytes() + (t * 8 + g) * 16,
+               static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
+               ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
+  const int groups = (w.row_tiles() + R - 1) / R;
+  const int rg0 = static_cast<int>(static_cast<long long>(groups) * blockIdx.x / gridDim.x);
+  const int rg1 = static_cast<int>(static_cast<long long>(groups) * (blockIdx.x + 1) / gridDim.x);
+  const int rows_here = min(count, 8 * NT);
+  // columns of the instruction beyond the rows read row 0 again: their results are not written
+  const T* xrow[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    long long r = first + (j * 8 + g < rows_here ? j * 8 + g : 0);
+    if constexpr (MODE == kGated) r = (p.rows.row_slot ? p.rows.row_slot[r] : r) / p.rows.top_k;
+    xrow[j] = static_cast<const T*>(p.x) + r * w.K + t * 16;
+  }
 
-  for (int done = 0; done < count; done += 8 * NT) {
-    if (MODE == kDense && done > 0) break;
-    const int rows_here = min(count - done, 8 * NT);
-    const T* xrow[NT];
+  const int whole = w.K / (64 * B);                       // blocks of B whole steps
+  const int mine = whole > warp ? (whole - warp + kWarps - 1) / kWarps : 0;
+  const int total = mine * (rg1 - rg0);
+  // the steps behind the whole blocks: one each, dealt out after the blocks
+  const int edge0 = whole * B + (warp + kWarps - whole % kWarps) % kWarps;
+  int l_rg = rg0, l_kt = warp * B;                        // next block to load
+  auto advance = [&]() {
+    l_kt += kWarps * B;
+    if (l_kt >= whole * B) { l_kt = warp * B; ++l_rg; }
+  };
+  Held<ZEROS, R, B, SPAN> held;
+  if (total > 0) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int c = j * 8 + g;
-      xrow[j] = nullptr;
-      if (c < rows_here) {
-        long long r = first + done + c;
-        if constexpr (MODE == kGated) r = (p.rows.row_slot ? p.rows.row_slot[r] : r) / p.rows.top_k;
-        xrow[j] = static_cast<const T*>(p.x) + r * w.K + t * 16;
-      }
-    }
-    float acc[R][NT][4];
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
-
-    for (int kt = warp; kt < w.k_tiles(); kt += kWarps) {
-      uint32_t b[NT][8];
+    for (int b = 0; b < B; ++b) load_step<ZEROS, R, B, SPAN>(held, b, w, v, l_rg * R, l_kt, g, t);
+    advance();
+  }
+  float acc[R][NT][CH][4] = {};
+  int kt = warp * B, rg = 0;
+  auto finish = [&]() {   // the whole blocks of a row group are done: the steps behind them, and the sums to shared memory
+    for (int e = edge0; e < w.k_tiles(); e += kWarps) {
+      Held<ZEROS, R, 1, 1> h;
+      load_edge<ZEROS, R>(h, w, v, (rg0 + rg) * R, e, g, t);
+      uint4 x[NT][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        uint4 u = make_uint4(0, 0, 0, 0), v = u;
-        if (xrow[j] && kt * 64 + t * 16 < w.K) {
-          u = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kt * 64));
-          v = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kt * 64) + 1);
-        }
-        b[j][0] = u.x; b[j][1] = u.y; b[j][2] = u.z; b[j][3] = u.w;
-        b[j][4] = v.x; b[j][5] = v.y; b[j][6] = v.z; b[j][7] = v.w;
-      }
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const int tile_row = blockIdx.x * R + i;
-        if (tile_row >= w.row_tiles()) break;
-        const TileRegs r = load_tile<BF16>(w, packed, scales, zeros, tile_row, kt, g, t);
-        const uint32_t words[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          uint32_t a[4];
-          decode_word<BF16>(words[s], r, a);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma16816<BF16>(acc[i][j], a, b[j][2 * s], b[j][2 * s + 1]);
+        x[j][0] = x[j][1] = make_uint4(0, 0, 0, 0);
+        if (e * 64 + t * 16 < w.K) {
+          x[j][0] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + e * 64));
+          x[j][1] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + e * 64) + 1);
         }
       }
+      multiply<BF16, ZEROS, NT, R, 1, 1, CH>(h, 0, x, acc);
     }
+    float* out = red + (rg * kWarps + warp) * (VALUES * 32) + lane;
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int a = 0; a < R; ++a)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int b = 0; b < NT; ++b)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) red[(warp * (R * NT * 4) + (i * NT + j) * 4 + c) * 32 + lane] = acc[i][j][c];
-    __syncthreads();
-    for (int u = warp; u < R * NT * 4; u += kWarps) {
-      float v = 0.f;
+        for (int c = 0; c < 4; ++c) {
+          out[((a * NT + b) * 4 + c) * 32] = CH == 2 ? acc[a][b][0][c] + acc[a][b][CH - 1][c] : acc[a][b][0][c];
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) v += red[(k * (R * NT * 4) + u) * 32 + lane];
-      const int c = u & 3, j = (u >> 2) % NT, i = (u >> 2) / NT;
-      const int n = (blockIdx.x * R + i) * 16 + g + (c >> 1) * 8;    // weight row
-      const int col = j * 8 + t * 2 + (c & 1);                       // row of the batch
-      if constexpr (MODE == kGated) {
-        const float other = __shfl_xor_sync(0xffffffffu, v, 4);      // rows 2i and 2i + 1 are four lanes apart
-        if ((g & 1) == 0 && n + 1 < w.N && col < rows_here)
-          static_cast<T*>(p.y)[(static_cast<long long>(first) + done + col) * (w.N / 2) + n / 2] = I::from_float(silu_mul(v, other));
-      } else if (n < w.N && col < rows_here) {
-        const long long r = first + done + col;
-        if constexpr (MODE == kDense) static_cast<T*>(p.y)[r * w.N + n] = I::from_float(v);
-        else static_cast<float*>(p.y)[static_cast<long long>(p.rows.row_slot[r]) * w.N + n] = v;
+          for (int d = 0; d < CH; ++d) acc[a][b][d][c] = 0.f;
+        }
+    kt = warp * B;
+    ++rg;
+  };
+  for (int n = 0; n < total; ++n) {
+    const bool more = n + 1 < total;
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      uint4 x[NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        x[j][0] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kt * 64) + b * 8);
+        x[j][1] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kt * 64) + b * 8 + 1);
+      }
+      multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(held, b, x, acc);
+      // (a scale is loaded again with the last step that it serves)
+      if (more && SPAN == 1) load_step<ZEROS, R, B, SPAN>(held, b, w, v, l_rg * R, l_kt, g, t);
+      if (more && SPAN == 2 && b % 2 == 1) {
+        load_step<ZEROS, R, B, SPAN>(held, b - 1, w, v, l_rg * R, l_kt, g, t);
+        load_step<ZEROS, R, B, SPAN>(held, b, w, v, l_rg * R, l_kt, g, t);
       }
     }
-    __syncthreads();
+    if (more) advance();
+    kt += kWarps * B;
+    if (kt >= whole * B) finish();
+  }
+  if (mine == 0)
+    while (rg < rg1 - rg0) finish();
+  __syncthreads();
+  for (int u = warp; u < (rg1 - rg0) * VALUES; u += kWarps) {
+    const int r = u / VALUES, q = u % VALUES;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) sum += red[((r * kWarps + k) * VALUES + q) * 32 + lane];
+    const int c = q & 3, j = (q >> 2) % NT, i = (q >> 2) / NT;
+    const int n = ((rg0 + r) * R + i) * 16 + g + (c >> 1) * 8;    // weight row
+    const int col = j * 8 + t * 2 + (c & 1);                       // row of the batch
+    if constexpr (MODE == kGated) {
+      const float other = __shfl_xor_sync(0xffffffffu, sum, 4);    // rows 2i and 2i + 1 are four lanes apart
+      if ((g & 1) == 0 && n + 1 < w.N && col < rows_here)
+        static_cast<T*>(p.y)[(static_cast<long long>(first) + col) * (w.N / 2) + n / 2] = I::from_float(silu_mul(sum, other));
+    } else if (n < w.N && col < rows_here) {
+      const long long row = first + col;
+      if constexpr (MODE == kDense) static_cast<T*>(p.y)[row * w.N + n] = I::from_float(sum);
+      else static_cast<float*>(p.y)[static_cast<long long>(p.rows.row_slot[row]) * w.N + n] = sum;
+    }
   }
 }
 
 // y[token] = sum_j weight_j * H[token * top_k + j] W_{e_j}^T: the K loops of all choices of a token, dealt out to the warps
 // one after the other, and the weighted sum in the same reduction.
-template <bool BF16>
-__global__ void __launch_bounds__(kWarps * 32)
+template <bool BF16, bool ZEROS>
+__global__ void __launch_bounds__(kWarps * 32, 3)
 int4_small_down_direct_kernel(const SmallParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
+  constexpr int B = 4;
   __shared__ float red[kWarps][2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -193,34 +269,42 @@ int4_small_down_direct_kernel(const SmallParams p) {
   const int end = static_cast<int>(static_cast<long long>(units) * (warp + 1) / kWarps);
   while (u < end) {
     const int j = u / kts, slot = token * p.rows.top_k + j;
-    const int stop = min(end, (j + 1) * kts);
+    const int kt0 = u - j * kts, kt1 = min(end - j * kts, kts);
+    u = j * kts + kt1;
     const int expert = p.rows.ids[slot];
-    if (expert < 0 || expert >= p.rows.E) { u = stop; continue; }
-    const uint8_t* packed = w.packed + expert * w.expert_bytes();
-    const unsigned short* scales = static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales();
-    const uint8_t* zeros = w.zeros ? w.zeros + expert * w.expert_scales() : nullptr;
+    if (expert < 0 || expert >= p.rows.E) continue;
+    const View v{w.packed + expert * w.expert_bytes() + (t * 8 + g) * 16,
+                 static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
+                 ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
     const T* h = static_cast<const T*>(p.x) + static_cast<long long>(slot) * w.K + t * 16;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (; u < stop; ++u) {
-      const int kt = u - j * kts;
-      uint4 b0 = make_uint4(0, 0, 0, 0), b1 = b0;
-      if (g == 0 && kt * 64 + t * 16 < w.K) {
-        b0 = __ldg(reinterpret_cast<const uint4*>(h + kt * 64));
-        b1 = __ldg(reinterpret_cast<const uint4*>(h + kt * 64) + 1);
-      }
-      const TileRegs r = load_tile<BF16>(w, packed, scales, zeros, tile_row, kt, g, t);
-      const uint32_t words[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
-      const uint32_t b[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+    float acc[1][1][2][4] = {};
+    int kt = kt0;
+    const int kt_whole = min(kt1, w.K / 64);
+    for (; kt + B <= kt_whole; kt += B) {
+      Held<ZEROS, 1, B, 1> held;
+      uint4 x[B][1][2];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        uint32_t a[4];
-        decode_word<BF16>(words[s], r, a);
-        mma16816<BF16>(acc, a, b[2 * s], b[2 * s + 1]);
+      for (int b = 0; b < B; ++b) {
+        load_step<ZEROS, 1, B, 1>(held, b, w, v, tile_row, kt, g, t);
+        x[b][0][0] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64) + b * 8);
+        x[b][0][1] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64) + b * 8 + 1);
       }
+#pragma unroll
+      for (int b = 0; b < B; ++b) multiply<BF16, ZEROS, 1, 1, B, 1, 2>(held, b, x[b], acc);
+    }
+    for (; kt < kt1; ++kt) {
+      Held<ZEROS, 1, 1, 1> held;
+      load_edge<ZEROS, 1>(held, w, v, tile_row, kt, g, t);
+      uint4 x[1][2] = {};
+      if (kt * 64 + t * 16 < w.K) {
+        x[0][0] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64));
+        x[0][1] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64) + 1);
+      }
+      multiply<BF16, ZEROS, 1, 1, 1, 1, 2>(held, 0, x, acc);
     }
     const float weight = p.rows.weights[slot];
-    lo += weight * acc[0];
-    hi += weight * acc[2];
+    lo += weight * (acc[0][0][0][0] + acc[0][0][1][0]);
+    hi += weight * (acc[0][0][0][2] + acc[0][0][1][2]);
   }
   if (t == 0) { red[warp][0][g] = lo; red[warp][1][g] = hi; }
   __syncthreads();
@@ -233,17 +317,45 @@ int4_small_down_direct_kernel(const SmallParams p) {
   }
 }
 
-template <bool BF16, int MODE, int NT, int R>
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms > 0 ? sms : 148;
+}
+
+// MAX_GROUPS: row groups whose sums a block has room for in shared memory
+template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int MIN_BLOCKS, int MAX_GROUPS>
 int launch_one(const SmallParams& p, int blocks_y, cudaStream_t s) {
-  const size_t smem = static_cast<size_t>(kWarps) * R * NT * 4 * 32 * sizeof(float);
-  auto kernel = int4_small_kernel<BF16, MODE, NT, R>;
+  auto kernel = int4_small_kernel<BF16, ZEROS, MODE, NT, R, B, SPAN, MIN_BLOCKS>;
+  const int groups = (p.w.row_tiles() + R - 1) / R;
+  // as many blocks as run at once, if that leaves them no more row groups than they have room for; else whole rounds of them
+  const int slots = max(1, sm_count() * MIN_BLOCKS / blocks_y);
+  const int rounds = (groups + slots * MAX_GROUPS - 1) / (slots * MAX_GROUPS);
+  const int blocks = static_cast<int>(min(static_cast<long long>(groups), static_cast<long long>(slots) * rounds));
+  const int per_block = (groups + blocks - 1) / blocks;
+  const size_t smem = static_cast<size_t>(per_block) * kWarps * R * NT * 4 * 32 * sizeof(float);
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return VQG_ERR_LAUNCH;
-  const dim3 grid((p.w.row_tiles() + R - 1) / R, blocks_y);
-  kernel<<<grid, kWarps * 32, smem, s>>>(p);
+  kernel<<<dim3(blocks, blocks_y), kWarps * 32, smem, s>>>(p);
   count_launch();
   return cuda_status(cudaGetLastError());
+}
+
+template <int MODE>
+int launch_rows(const SmallParams& p, int rows, int blocks_y, bool bf16, cudaStream_t s) {
+  auto go = [&](auto type, auto zeros) {
+    constexpr bool B = decltype(type)::value, Z = decltype(zeros)::value;
+    const bool pairs = p.w.group % 128 == 0;
+    if (rows <= 8) {
+      if (p.w.K < 64 * 4 * kWarps) return launch_one<B, Z, MODE, 1, 1, 2, 1, 3, 8>(p, blocks_y, s);
+      return pairs ? launch_one<B, Z, MODE, 1, 1, 4, 2, 3, 8>(p, blocks_y, s) : launch_one<B, Z, MODE, 1, 1, 4, 1, 3, 8>(p, blocks_y, s);
+    }
+    if (rows <= 16) return launch_one<B, Z, MODE, 2, 2, 2, 1, 2, 4>(p, blocks_y, s);
+    return launch_one<B, Z, MODE, 4, 2, 2, 1, 2, 2>(p, blocks_y, s);
+  };
+  if (p.w.zeros) return bf16 ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
+  return bf16 ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});
 }
 
 }  // namespace
@@ -251,25 +363,24 @@ int launch_one(const SmallParams& p, int blocks_y, cudaStream_t s) {
 int launch_int4_small(const Int4Weight& w, const void* x, void* y, int M, bool bf16, cudaStream_t s) {
   SmallParams p{};
   p.w = w; p.x = x; p.y = y; p.M = M;
-  if (M <= 8) return bf16 ? launch_one<true, kDense, 1, 1>(p, 1, s) : launch_one<false, kDense, 1, 1>(p, 1, s);
-  const int chunks = (M + 31) / 32;
+  const int rows = M < kInt4SmallRows ? M : kInt4SmallRows, chunks = (M + rows - 1) / rows;
   if (chunks > 65535) return VQG_ERR_UNSUPPORTED;
-  return bf16 ? launch_one<true, kDense, 4, 2>(p, chunks, s) : launch_one<false, kDense, 4, 2>(p, chunks, s);
+  return launch_rows<kDense>(p, rows, chunks, bf16, s);
 }
 
-int launch_int4_small_gated(const Int4Weight& w, const void* x, void* h, const ExpertRows& rows, int max_chunks, bool bf16,
-                            cudaStream_t s) {
+int launch_int4_small_gated(const Int4Weight& w, const void* x, void* h, const ExpertRows& rows, int chunk_rows, int max_chunks,
+                            bool bf16, cudaStream_t s) {
   SmallParams p{};
   p.w = w; p.x = x; p.y = h; p.rows = rows;
-  if (!rows.chunks) return bf16 ? launch_one<true, kGated, 1, 1>(p, rows.slots, s) : launch_one<false, kGated, 1, 1>(p, rows.slots, s);
-  return bf16 ? launch_one<true, kGated, 4, 2>(p, max_chunks, s) : launch_one<false, kGated, 4, 2>(p, max_chunks, s);
+  if (!rows.chunks) return launch_rows<kGated>(p, 1, rows.slots, bf16, s);
+  return launch_rows<kGated>(p, chunk_rows, max_chunks, bf16, s);
 }
 
-int launch_int4_small_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int max_chunks, bool bf16,
-                           cudaStream_t s) {
+int launch_int4_small_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int chunk_rows, int max_chunks,
+                           bool bf16, cudaStream_t s) {
   SmallParams p{};
   p.w = w; p.x = h; p.y = part; p.rows = rows;
-  return bf16 ? launch_one<true, kDown, 4, 2>(p, max_chunks, s) : launch_one<false, kDown, 4, 2>(p, max_chunks, s);
+  return launch_rows<kDown>(p, chunk_rows, max_chunks, bf16, s);
 }
 
 int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, const ExpertRows& rows, int tokens, bool bf16,
@@ -277,8 +388,9 @@ int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, c
   SmallParams p{};
   p.w = w; p.x = h; p.y = y; p.rows = rows;
   const dim3 grid(w.row_tiles(), tokens);
-  if (bf16) int4_small_down_direct_kernel<true><<<grid, kWarps * 32, 0, s>>>(p);
-  else int4_small_down_direct_kernel<false><<<grid, kWarps * 32, 0, s>>>(p);
+  auto go = [&](auto kernel) { kernel<<<grid, kWarps * 32, 0, s>>>(p); };
+  if (w.zeros) bf16 ? go(int4_small_down_direct_kernel<true, true>) : go(int4_small_down_direct_kernel<false, true>);
+  else bf16 ? go(int4_small_down_direct_kernel<true, false>) : go(int4_small_down_direct_kernel<false, false>);
   count_launch();
   return cuda_status(cudaGetLastError());
 }

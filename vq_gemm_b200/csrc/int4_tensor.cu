@@ -505,7 +505,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
       auto fetch = [&](int k, uint32_t& s2, uint32_t& off) {
         s2 = 0; off = I::offset(8);
         if (row_ok && k < w.K) {
-          const long long at = static_cast<long long>(k / w.group) * w.N;
+          const long long at = static_cast<long long>(int4_group_of(w, k)) * w.N;
           s2 = __ldg(sc + at) * 0x10001u;
           if (ze) off = I::offset(__ldg(ze + at) & 15);
         }
