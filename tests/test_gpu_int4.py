@@ -212,3 +212,25 @@ def test_module():
                           test_utils=("test_schema", "test_faketensor"))
     compiled = torch.compile(layer, backend="eager", fullgraph=True)
     assert torch.equal(compiled(x), layer(x))
+
+
+def test_quantiser_at_the_smallest_scales():
+    # bf16 scales down to the smallest subnormal number, whose reciprocal 32 bits do not hold
+    for power in (-100, -118, -124, -130, -133):
+        w = ((torch.arange(16 * 64).reshape(16, 64) % 23 - 11).float() * 2.0 ** power).to(BF16)
+        for symmetric in (True, False):
+            packed, scales, zeros = quantize.int4_quantize(w.cuda(), group=64, symmetric=symmetric)
+            codes, s, z = O.quantize(w, 64, symmetric)
+            assert same(scales, s) and torch.equal(quantize.int4_unpack(packed.cpu(), 16, 64), codes)
+            assert symmetric or torch.equal(zeros.cpu(), z)
+
+
+def test_quantiser_and_dequantisation_of_tensors_that_start_on_16_bytes_only():
+    w = (torch.randn(32 * 64 + 8, generator=torch.Generator().manual_seed(2)) * 0.05).half().cuda()[8:].view(32, 64)
+    assert w.data_ptr() % 32 == 16
+    packed, scales, _ = quantize.int4_quantize(w, group=64)
+    codes, s, _ = O.quantize(w.cpu(), 64, True)
+    assert same(scales, s) and torch.equal(quantize.int4_unpack(packed.cpu(), 32, 64), codes)
+    out = torch.zeros(32 * 64 + 8, dtype=F16, device="cuda")[8:].view(32, 64)
+    V.int4_dequant(packed, scales, out=out)
+    assert same(out, O.weights(packed, scales, None, 64).half())

@@ -14,6 +14,7 @@ int check_weight(const void* packed, const void* scales, const void* zeros, int 
   if (experts < 0 || N < 0 || K < 0 || (dtype != 0 && dtype != 1)) return VQG_ERR_BAD_ARG;
   if (experts == 0 || N == 0 || K == 0) return VQG_OK;
   if (!group_ok(K, group) || K > kInt4MaxK) return VQG_ERR_UNSUPPORTED;
+  if (static_cast<long long>(K / group) * N > 0x7fffffffLL) return VQG_ERR_UNSUPPORTED;   // 32-bit positions of scales
   if (!packed || !scales || !aligned(packed, 16) || !aligned(scales, 2)) return VQG_ERR_BAD_ARG;
   (void)zeros;   // bytes: any address
   return VQG_OK;

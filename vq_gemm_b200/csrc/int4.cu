@@ -8,6 +8,8 @@
 // over each group, every operation rounded to fp32, rint to the nearest even number; where the scale rounds to zero the
 // codes stand for zero.  A quotient of two 11-bit numbers that is not halfway between two whole numbers is further from
 // there than fp32 rounds, so the codes are those of exact arithmetic.
+#include <type_traits>
+
 #include "int4.cuh"
 
 namespace vqg {
@@ -21,9 +23,36 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   else return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
+// 32 bytes with one access where the address allows it (`wide`: it is a multiple of 32)
+__device__ __forceinline__ void load32(const void* p, bool wide, uint32_t (&v)[8]) {
+  if (wide) {
+    asm volatile("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "l"(p));
+  } else {
+    const uint4 a = __ldg(static_cast<const uint4*>(p)), b = __ldg(static_cast<const uint4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+}
+__device__ __forceinline__ void store32(void* p, bool wide, const uint32_t (&v)[8]) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+  } else {
+    static_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    static_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// From 192 + w / s (a multiple of 2^-16): w / s rounded to the nearest whole number, halves to the even one, plus the zero point,
+// held to 0 ... 15; in the low byte.  12582912 = 1.5 * 2^23 is even, and sums around it have no bits below one.
+__device__ __forceinline__ uint32_t code_of(float q192, float zero) {
+  const float r = (q192 + (12582912.f - 192.f)) + zero;
+  return __float_as_uint(fminf(fmaxf(r, 12582912.f), 12582927.f));
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads)
-int4_dequant_kernel(const Int4Weight w, void* __restrict__ out) {
+int4_dequant_kernel(const Int4Weight w, void* __restrict__ out, bool wide) {
   using I = Int4Type<BF16>;
   const int lane = threadIdx.x & 31, g = lane & 7, t = lane >> 3;
   const long long tiles = static_cast<long long>(w.row_tiles()) * w.k_tiles();
@@ -52,22 +81,28 @@ int4_dequant_kernel(const Int4Weight w, void* __restrict__ out) {
         v[2 * s] = h ? int4_pair<BF16, 1, 0>(words[s], off, s2) : int4_pair<BF16, 0, 0>(words[s], off, s2);
         v[2 * s + 1] = h ? int4_pair<BF16, 1, 1>(words[s], off, s2) : int4_pair<BF16, 0, 1>(words[s], off, s2);
       }
-      uint4* d = reinterpret_cast<uint4*>(dst + static_cast<long long>(row) * w.K + k);
-      d[0] = make_uint4(v[0], v[1], v[2], v[3]);
-      d[1] = make_uint4(v[4], v[5], v[6], v[7]);
+      store32(dst + static_cast<long long>(row) * w.K + k, wide, v);
     }
   }
 }
 
-// A warp owns 16 rows x `span` tile columns: whole groups (span = group / 64, or 1 where the group is 32, or the whole row).
-// Lane t*8 + g reads columns 16t ... +15 of rows g and g + 8 of each tile: the values whose codes its 16 bytes hold.
-template <bool BF16, bool ZEROS>
+// One unit of work is 16 rows x SPAN tile columns of 64: whole groups of 32, 64 or SPAN * 64 columns.  Lane t*8 + g reads columns
+// 16t ... +15 of rows g and g + 8 of each tile, the values whose codes its 16 bytes hold, and keeps them in registers between
+// the extremes and the codes, so the weight is read once.  (SPAN = 0: groups of more columns than registers hold; a second read
+// that the caches serve.)
+//
+// The division: w / s is w * (1 / s) but for a few steps of 2^-23, and a quotient of two 11-bit numbers is either halfway between
+// two whole numbers or at least 2^-13 from there; rounding the product to multiples of 2^-16 first (adding 192 does) turns
+// what is nearly halfway into exactly halfway, and the codes are those of the correctly rounded division.
+template <bool BF16, bool ZEROS, int SPAN>
 __global__ void __launch_bounds__(kThreads)
 int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed, void* __restrict__ scales,
-                     uint8_t* __restrict__ zeros, int N, int K, int group, int span) {
+                     uint8_t* __restrict__ zeros, int N, int K, int group, int span_all, bool wide) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
+  constexpr int HOLD = SPAN > 0 ? SPAN : 1;
   const int lane = threadIdx.x & 31, g = lane & 7, t = lane >> 3;
+  const int span = SPAN > 0 ? SPAN : span_all;
   const int row_tiles = (N + 15) / 16, k_tiles = (K + 63) / 64, spans = (k_tiles + span - 1) / span;
   const long long unit = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   if (unit >= static_cast<long long>(row_tiles) * spans) return;
@@ -77,30 +112,41 @@ int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed,
   const T* w = static_cast<const T*>(src) + static_cast<long long>(e) * N * K;
   uint8_t* codes = packed + static_cast<long long>(e) * row_tiles * k_tiles * 512;
   const long long sbase = static_cast<long long>(e) * (K / group) * N;
+  const T* at[2] = {w + static_cast<long long>(min(tr * 16 + g, N - 1)) * K + t * 16, w + static_cast<long long>(min(tr * 16 + 8 + g, N - 1)) * K + t * 16};
 
-  auto load = [&](int kt, int h, uint32_t (&v)[8]) {
-    const int row = tr * 16 + h * 8 + g, k = kt * 64 + t * 16;
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (row < N && k < K) {
-      const uint4* p = reinterpret_cast<const uint4*>(w + static_cast<long long>(row) * K + k);
-      a = __ldg(p); b = __ldg(p + 1);
-    }
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  };
-  float lo[2] = {0.f, 0.f}, hi[2] = {0.f, 0.f};
-  for (int kt = kt0; kt < kt1; ++kt)
+  uint32_t v[HOLD][2][8];
+  auto load = [&](int kt, uint32_t (&d)[2][8]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t v[8];
-      load(kt, h, v);
+      if (kt < k_tiles && kt * 64 + t * 16 < K) {
+        load32(at[h] + kt * 64, wide, d[h]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[h][i] = 0;
+      }
+    }
+  };
+  float lo[2] = {0.f, 0.f}, hi[2] = {0.f, 0.f};
+  auto extremes = [&](const uint32_t (&d)[2][8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 f = unpack2<BF16>(v[i]);
+        const float2 f = unpack2<BF16>(d[h][i]);
         if (ZEROS) { lo[h] = fminf(lo[h], fminf(f.x, f.y)); hi[h] = fmaxf(hi[h], fmaxf(f.x, f.y)); }
         else hi[h] = fmaxf(hi[h], fmaxf(fabsf(f.x), fabsf(f.y)));
       }
-    }
-  float s[2], z[2];
+  };
+  if constexpr (SPAN > 0) {
+#pragma unroll
+    for (int k = 0; k < SPAN; ++k) load(kt0 + k, v[k]);
+#pragma unroll
+    for (int k = 0; k < SPAN; ++k) extremes(v[k]);
+  } else {
+    for (int kt = kt0; kt < kt1; ++kt) { load(kt, v[0]); extremes(v[0]); }
+  }
+  float inv[2], dv[2], z[2];
+  bool tiny = false;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     // a group of 32 columns is two threads t, a longer one all four
@@ -111,33 +157,47 @@ int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed,
       if (group != 32) lo[h] = fminf(lo[h], __shfl_xor_sync(0xffffffffu, lo[h], 16));
     }
     const T st = I::from_float(ZEROS ? __fdiv_rn(hi[h] - lo[h], 15.f) : __fdiv_rn(hi[h], 7.f));
-    s[h] = I::to_float(st);
-    const float d = s[h] > 0.f ? s[h] : 1.f;
+    const float s = I::to_float(st);
+    const float d = s > 0.f ? s : 1.f;
     z[h] = ZEROS ? fminf(fmaxf(rintf(__fdiv_rn(-lo[h], d)), 0.f), 15.f) : 8.f;
+    inv[h] = __fdiv_rn(1.f, d);
+    dv[h] = d;
+    tiny = tiny || d < 1e-36f;
     const int row = tr * 16 + h * 8 + g, k = kt0 * 64 + t * 16;
     if (row < N && k < K && (group == 32 ? (t & 1) == 0 : t == 0)) {
-      const long long at = sbase + static_cast<long long>(k / group) * N + row;
-      static_cast<T*>(scales)[at] = st;
-      if (ZEROS) zeros[at] = static_cast<uint8_t>(z[h]);
+      const long long to = sbase + static_cast<long long>(k / group) * N + row;
+      static_cast<T*>(scales)[to] = st;
+      if (ZEROS) zeros[to] = static_cast<uint8_t>(z[h]);
     }
-    s[h] = d;
   }
-  for (int kt = kt0; kt < kt1; ++kt) {
+  tiny = __any_sync(0xffffffffu, tiny);
+  auto encode = [&](int kt, const uint32_t (&d)[2][8]) {
     uint32_t words[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t v[8];
-      load(kt, h, v);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {   // pair i: word i / 2, q = i % 2
-        const float2 f = unpack2<BF16>(v[i]);
-        const uint32_t c0 = static_cast<uint32_t>(fminf(fmaxf(rintf(__fdiv_rn(f.x, s[h])) + z[h], 0.f), 15.f));
-        const uint32_t c1 = static_cast<uint32_t>(fminf(fmaxf(rintf(__fdiv_rn(f.y, s[h])) + z[h], 0.f), 15.f));
-        words[i >> 1] |= (c0 | (c1 << 16)) << (8 * (i & 1) + 4 * h);
+        const float2 f = unpack2<BF16>(d[h][i]);
+        uint32_t c0, c1;
+        if (!tiny) {
+          c0 = code_of(__fmaf_rn(f.x, inv[h], 192.f), z[h]);
+          c1 = code_of(__fmaf_rn(f.y, inv[h], 192.f), z[h]);
+        } else {                      // 1 / s may overflow
+          c0 = code_of(__fdiv_rn(f.x, dv[h]) + 192.f, z[h]);
+          c1 = code_of(__fdiv_rn(f.y, dv[h]) + 192.f, z[h]);
+        }
+        const uint32_t pair = __byte_perm(c0, c1, 0x1410);
+        words[i >> 1] |= pair << (8 * (i & 1) + 4 * h);
       }
-    }
     reinterpret_cast<uint4*>(codes + (static_cast<long long>(tr) * k_tiles + kt) * 512)[lane] =
         make_uint4(words[0], words[1], words[2], words[3]);
+  };
+  if constexpr (SPAN > 0) {
+#pragma unroll
+    for (int k = 0; k < SPAN; ++k)
+      if (kt0 + k < k_tiles) encode(kt0 + k, v[k]);
+  } else {
+    for (int kt = kt0; kt < kt1; ++kt) { load(kt, v[0]); encode(kt, v[0]); }
   }
 }
 
@@ -153,8 +213,9 @@ int launch_int4_dequant(const Int4Weight& w, void* out, int experts, bool bf16, 
   const long long tiles = static_cast<long long>(w.row_tiles()) * w.k_tiles();
   const long long want = (tiles + kThreads / 32 - 1) / (kThreads / 32), most = 8LL * sm_count();
   const dim3 grid(static_cast<unsigned>(want < most ? want : most), experts);
-  if (bf16) int4_dequant_kernel<true><<<grid, kThreads, 0, s>>>(w, out);
-  else int4_dequant_kernel<false><<<grid, kThreads, 0, s>>>(w, out);
+  const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0;   // rows are multiples of 64 bytes
+  if (bf16) int4_dequant_kernel<true><<<grid, kThreads, 0, s>>>(w, out, wide);
+  else int4_dequant_kernel<false><<<grid, kThreads, 0, s>>>(w, out, wide);
   count_launch();
   return cuda_status(cudaGetLastError());
 }
@@ -166,13 +227,20 @@ int launch_int4_quantize(const void* w, uint8_t* packed, void* scales, uint8_t* 
   const long long blocks = (units + kThreads / 32 - 1) / (kThreads / 32);
   if (blocks > 0x7fffffffLL) return VQG_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks), experts);
+  const bool wide = reinterpret_cast<uintptr_t>(w) % 32 == 0;
   auto go = [&](auto kernel) {
-    kernel<<<grid, kThreads, 0, s>>>(w, packed, scales, zeros, N, K, group, span);
+    kernel<<<grid, kThreads, 0, s>>>(w, packed, scales, zeros, N, K, group, span, wide);
     count_launch();
     return cuda_status(cudaGetLastError());
   };
-  if (zeros) return bf16 ? go(int4_quantize_kernel<true, true>) : go(int4_quantize_kernel<false, true>);
-  return bf16 ? go(int4_quantize_kernel<true, false>) : go(int4_quantize_kernel<false, false>);
+  auto with = [&](auto n) {
+    constexpr int S = decltype(n)::value;
+    if (zeros) return bf16 ? go(int4_quantize_kernel<true, true, S>) : go(int4_quantize_kernel<false, true, S>);
+    return bf16 ? go(int4_quantize_kernel<true, false, S>) : go(int4_quantize_kernel<false, false, S>);
+  };
+  if (span == 1) return with(std::integral_constant<int, 1>{});
+  if (span == 2) return with(std::integral_constant<int, 2>{});
+  return with(std::integral_constant<int, 0>{});
 }
 
 }  // namespace vqg

@@ -1,9 +1,11 @@
 // Products of a few rows with 4-bit weights (format: int4.cuh): Y[m, n] = sum_k X[m, k] W[n, k], and the two products of
 // the experts of a mixture-of-experts layer over the rows that chose them.
 //
-// A warp owns R row tiles of the weight (16 rows each) and every eighth 64-column tile of K; one 16-byte load per lane and
-// tile gives the A fragments of four mma.sync m16n8k16, whose B fragments are 32 consecutive bytes of a row of X per
-// lane.  The eight warps' accumulators are summed through shared memory.
+// A warp takes blocks of B neighbouring 64-column steps of R row tiles (16 weight rows each).  A lane's 16 bytes of a tile give the
+// A fragments of four mma.sync m16n8k16, whose B fragments are 32 consecutive bytes of a row of X.  Every lane copies its
+// own 16 bytes of each tile asynchronously into its own places of a ring in shared memory, SLOTS blocks ahead, and reads them
+// back: nothing waits for another thread, and no register or scoreboard is tied up by a load from memory.  The eight warps'
+// sums of a row group meet in shared memory.
 #include <type_traits>
 
 #include "int4.cuh"
@@ -21,13 +23,6 @@ struct SmallParams {
   ExpertRows rows;
 };
 
-// weights are read once: past L1
-__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-
 enum { kDense = 0, kGated = 1, kDown = 2 };
 
 template <bool BF16>
@@ -42,58 +37,66 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// What a lane holds of B neighbouring 64-column steps of R row tiles between load and use: weights, and scales and zero
-// points of rows g and g + 8, one for every SPAN steps (2 where a group is a multiple of 128 columns).
+// Scales and zero points of rows g and g + 8 of R row tiles for B steps, one for every SPAN steps (2 where a group is a multiple
+// of 128 columns), as loaded.
 template <bool ZEROS, int R, int B, int SPAN>
-struct Held {
+struct Scales {
   static constexpr int S = B / SPAN;
-  uint4 w[B][R];
   unsigned short s_lo[S][R], s_hi[S][R];
   uint8_t z_lo[ZEROS ? S : 1][R], z_hi[ZEROS ? S : 1][R];
 };
 
 // One expert's weight as a lane sees it.
 struct View {
-  const uint8_t* packed;          // at the lane's 16 bytes of tile (0, 0)
+  const uint8_t* packed;
   const unsigned short* scales;
   const uint8_t* zeros;
 };
 
-// Steps kt ... kt + B - 1, all of them whole.  Rows that do not exist read the last one: their results are not written.
+// row_lo, row_hi: the lane's two rows in the first row tile; rows that do not exist read the last one, their results are not
+// written.
 template <bool ZEROS, int R, int B, int SPAN>
-__device__ __forceinline__ void load_step(Held<ZEROS, R, B, SPAN>& h, int b, const Int4Weight& w, const View& v, int tile_row, int kt,
-                                          int g, int t) {
+__device__ __forceinline__ void load_scales(Scales<ZEROS, R, B, SPAN>& h, const Int4Weight& w, const View& v, int tile_row, int kt,
+                                            int g, int t) {
+  int lo[R], hi[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int tr = R == 1 ? tile_row : min(tile_row + i, w.row_tiles() - 1);
-    h.w[b][i] = ld_stream(v.packed + (static_cast<size_t>(tr) * w.k_tiles() + kt) * 512 + b * 512);
-    if (b % SPAN == 0) {
-      const size_t at = static_cast<size_t>(int4_group_of(w, (kt + b) * 64 + t * 16)) * w.N;
-      const int lo = min(tr * 16 + g, w.N - 1), hi = min(tr * 16 + g + 8, w.N - 1);
-      h.s_lo[b / SPAN][i] = __ldg(v.scales + at + lo);
-      h.s_hi[b / SPAN][i] = __ldg(v.scales + at + hi);
-      if constexpr (ZEROS) { h.z_lo[b / SPAN][i] = __ldg(v.zeros + at + lo); h.z_hi[b / SPAN][i] = __ldg(v.zeros + at + hi); }
+    lo[i] = min((tile_row + i) * 16 + g, w.N - 1);
+    hi[i] = min((tile_row + i) * 16 + g + 8, w.N - 1);
+  }
+#pragma unroll
+  for (int b = 0; b < B; b += SPAN) {
+    const int at = int4_group_of(w, min((kt + b) * 64 + t * 16, w.K - 16)) * w.N;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      h.s_lo[b / SPAN][i] = __ldg(v.scales + static_cast<uint32_t>(at + lo[i]));
+      h.s_hi[b / SPAN][i] = __ldg(v.scales + static_cast<uint32_t>(at + hi[i]));
+      if constexpr (ZEROS) {
+        h.z_lo[b / SPAN][i] = __ldg(v.zeros + static_cast<uint32_t>(at + lo[i]));
+        h.z_hi[b / SPAN][i] = __ldg(v.zeros + static_cast<uint32_t>(at + hi[i]));
+      }
     }
   }
 }
 
-// Any steps: no column beyond K is read, and its weight is zero.
-template <bool ZEROS, int R>
-__device__ __forceinline__ void load_edge(Held<ZEROS, R, 1, 1>& h, const Int4Weight& w, const View& v, int tile_row, int kt, int g, int t) {
-  load_step<ZEROS, R, 1, 1>(h, 0, w, v, tile_row, kt, g, kt * 64 + t * 16 < w.K ? t : 0);
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-    if (kt * 64 + t * 16 >= w.K) h.s_lo[0][i] = h.s_hi[0][i] = 0;
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
-// acc += W X^T over step b; x[j] are the lane's 32 bytes of row 8j + g of X
+// acc += W X^T over step b, whose packed weights lie at `at` (row tiles 512 bytes apart) in shared memory;
+// x[j] are the lane's 32 bytes of row 8j + g of X
 template <bool BF16, bool ZEROS, int NT, int R, int B, int SPAN, int CH>
-__device__ __forceinline__ void multiply(const Held<ZEROS, R, B, SPAN>& h, int b, const uint4 (&x)[NT][2], float (&acc)[R][NT][CH][4]) {
-  uint32_t s_lo[R], s_hi[R], o_lo[R], o_hi[R];
+__device__ __forceinline__ void multiply(const Scales<ZEROS, R, B, SPAN>& h, int b, bool in, uint32_t at,
+                                         const uint4 (&x)[NT][2], float (&acc)[R][NT][CH][4]) {
+  uint32_t s_lo[R], s_hi[R], o_lo[R], o_hi[R], q[R][4];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    s_lo[i] = h.s_lo[b / SPAN][i] * 0x10001u;
-    s_hi[i] = h.s_hi[b / SPAN][i] * 0x10001u;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[i][0]), "=r"(q[i][1]), "=r"(q[i][2]), "=r"(q[i][3]) : "r"(at + i * 512));
+    s_lo[i] = in ? h.s_lo[b / SPAN][i] * 0x10001u : 0u;
+    s_hi[i] = in ? h.s_hi[b / SPAN][i] * 0x10001u : 0u;
     o_lo[i] = Int4Type<BF16>::offset(ZEROS ? h.z_lo[ZEROS ? b / SPAN : 0][i] & 15 : 8);
     o_hi[i] = int4_offset_hi<BF16>(ZEROS ? h.z_hi[ZEROS ? b / SPAN : 0][i] & 15 : 8);
   }
@@ -101,14 +104,12 @@ __device__ __forceinline__ void multiply(const Held<ZEROS, R, B, SPAN>& h, int b
   for (int s = 0; s < 4; ++s)
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const uint4& q4 = h.w[b][i];
-      const uint32_t word = s == 0 ? q4.x : s == 1 ? q4.y : s == 2 ? q4.z : q4.w;
       uint32_t a[4];
-      int4_word<BF16>(word, o_lo[i], o_hi[i], s_lo[i], s_hi[i], a);
+      int4_word<BF16>(q[i][s], o_lo[i], o_hi[i], s_lo[i], s_hi[i], a);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const uint4& q = x[j][s >> 1];
-        mma16816<BF16>(acc[i][j][s % CH], a, (s & 1) ? q.z : q.x, (s & 1) ? q.w : q.y);
+        const uint4& c = x[j][s >> 1];
+        mma16816<BF16>(acc[i][j][s % CH], a, (s & 1) ? c.z : c.x, (s & 1) ? c.w : c.y);
       }
     }
 }
@@ -116,16 +117,17 @@ __device__ __forceinline__ void multiply(const Held<ZEROS, R, B, SPAN>& h, int b
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
 // Block (bx, by): row groups (R row tiles each) [groups * bx / grid, groups * (bx + 1) / grid) of the weight, rows `by` of X.
-// The eight warps take blocks of B steps in turn; a warp walks its blocks of all its row groups as one sequence in which every
-// step's registers are loaded again, for the next block, as soon as it is multiplied.
-template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int MIN_BLOCKS>
+// The eight warps take the blocks of a row group in turn, one row group after the other.
+template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int SLOTS, int MIN_BLOCKS>
 __global__ void __launch_bounds__(kWarps * 32, MIN_BLOCKS)
 int4_small_kernel(const SmallParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
   constexpr int CH = R * NT == 1 ? 2 : 1;   // chains of accumulators: a matrix instruction waits for the one before it
   constexpr int VALUES = R * NT * 4;        // sums of a lane per row group
-  extern __shared__ float red[];            // [row group][warp][VALUES][lane]
+  constexpr int BYTES = R * B * 512;
+  extern __shared__ __align__(128) unsigned char smem[];   // rings, sums [row group][warp][VALUES][lane]
+  float* red = reinterpret_cast<float*>(smem + kWarps * SLOTS * BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const Int4Weight& w = p.w;
@@ -145,10 +147,41 @@ int4_small_kernel(const SmallParams p) {
   const View v{w.packed + expert * w.expert_bytes() + (t * 8 + g) * 16,
                static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
                ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
-  const int groups = (w.row_tiles() + R - 1) / R;
+  const int groups = (w.row_tiles() + R - 1) / R, k_tiles = w.k_tiles();
   const int rg0 = static_cast<int>(static_cast<long long>(groups) * blockIdx.x / gridDim.x);
   const int rg1 = static_cast<int>(static_cast<long long>(groups) * (blockIdx.x + 1) / gridDim.x);
   const int rows_here = min(count, 8 * NT);
+
+  // the warp's sequence of blocks, and the next one to copy
+  const int blocks = (k_tiles + B - 1) / B;
+  const int mine = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0;
+  const int total = mine * (rg1 - rg0);
+  const uint32_t ring = smem_u32(smem) + warp * (SLOTS * BYTES) + lane * 16;
+  int l_rg = rg0, l_kt = warp * B, left = total;
+  auto fill = [&](uint32_t slot) {
+    if (left > 0) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int tr = R == 1 ? l_rg : min(l_rg * R + i, w.row_tiles() - 1);
+        const uint8_t* src = v.packed + (static_cast<size_t>(tr) * k_tiles + l_kt) * 512;
+        if (l_kt + B <= k_tiles) {
+#pragma unroll
+          for (int b = 0; b < B; ++b) copy16(slot + (b * R + i) * 512, src + b * 512);
+        } else {
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+            if (l_kt + b < k_tiles) copy16(slot + (b * R + i) * 512, src + b * 512);
+        }
+      }
+      --left;
+      l_kt += kWarps * B;
+      if (l_kt >= k_tiles) { l_kt = warp * B; ++l_rg; }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) fill(ring + i * BYTES);
+
   // columns of the instruction beyond the rows read row 0 again: their results are not written
   const T* xrow[NT];
 #pragma unroll
@@ -157,84 +190,73 @@ int4_small_kernel(const SmallParams p) {
     if constexpr (MODE == kGated) r = (p.rows.row_slot ? p.rows.row_slot[r] : r) / p.rows.top_k;
     xrow[j] = static_cast<const T*>(p.x) + r * w.K + t * 16;
   }
-
-  const int whole = w.K / (64 * B);                       // blocks of B whole steps
-  const int mine = whole > warp ? (whole - warp + kWarps - 1) / kWarps : 0;
-  const int total = mine * (rg1 - rg0);
-  // the steps behind the whole blocks: one each, dealt out after the blocks
-  const int edge0 = whole * B + (warp + kWarps - whole % kWarps) % kWarps;
-  int l_rg = rg0, l_kt = warp * B;                        // next block to load
-  auto advance = [&]() {
-    l_kt += kWarps * B;
-    if (l_kt >= whole * B) { l_kt = warp * B; ++l_rg; }
-  };
-  Held<ZEROS, R, B, SPAN> held;
-  if (total > 0) {
+  auto load_x = [&](uint4 (&d)[NT][2], int step) {
 #pragma unroll
-    for (int b = 0; b < B; ++b) load_step<ZEROS, R, B, SPAN>(held, b, w, v, l_rg * R, l_kt, g, t);
-    advance();
-  }
+    for (int j = 0; j < NT; ++j) {
+      d[j][0] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + step * 64));
+      d[j][1] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + step * 64) + 1);
+    }
+  };
   float acc[R][NT][CH][4] = {};
+  Scales<ZEROS, R, B, SPAN> ahead;
   int kt = warp * B, rg = 0;
-  auto finish = [&]() {   // the whole blocks of a row group are done: the steps behind them, and the sums to shared memory
-    for (int e = edge0; e < w.k_tiles(); e += kWarps) {
-      Held<ZEROS, R, 1, 1> h;
-      load_edge<ZEROS, R>(h, w, v, (rg0 + rg) * R, e, g, t);
-      uint4 x[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        x[j][0] = x[j][1] = make_uint4(0, 0, 0, 0);
-        if (e * 64 + t * 16 < w.K) {
-          x[j][0] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + e * 64));
-          x[j][1] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + e * 64) + 1);
-        }
-      }
-      multiply<BF16, ZEROS, NT, R, 1, 1, CH>(h, 0, x, acc);
-    }
-    float* out = red + (rg * kWarps + warp) * (VALUES * 32) + lane;
-#pragma unroll
-    for (int a = 0; a < R; ++a)
-#pragma unroll
-      for (int b = 0; b < NT; ++b)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          out[((a * NT + b) * 4 + c) * 32] = CH == 2 ? acc[a][b][0][c] + acc[a][b][CH - 1][c] : acc[a][b][0][c];
-#pragma unroll
-          for (int d = 0; d < CH; ++d) acc[a][b][d][c] = 0.f;
-        }
-    kt = warp * B;
-    ++rg;
-  };
+  uint32_t at = ring;
+  if (total > 0) load_scales<ZEROS, R, B, SPAN>(ahead, w, v, rg0 * R, kt, g, t);
   for (int n = 0; n < total; ++n) {
-    const bool more = n + 1 < total;
+    const Scales<ZEROS, R, B, SPAN> sc = ahead;
+    int kt_next = kt + kWarps * B;
+    const bool last = kt_next >= k_tiles;                  // of the row group
+    if (last) kt_next = warp * B;
+    if (n + 1 < total) load_scales<ZEROS, R, B, SPAN>(ahead, w, v, (rg0 + rg + last) * R, kt_next, g, t);
+    if ((kt + B) * 64 <= w.K) {
+      uint4 x[2][NT][2];
+      load_x(x[0], kt);
+      copy_wait<SLOTS - 1>();
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      uint4 x[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        x[j][0] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kt * 64) + b * 8);
-        x[j][1] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + kt * 64) + b * 8 + 1);
+      for (int b = 0; b < B; ++b) {
+        if (b + 1 < B) load_x(x[(b + 1) & 1], kt + b + 1);
+        multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, true, at + b * (R * 512), x[b & 1], acc);
       }
-      multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(held, b, x, acc);
-      // (a scale is loaded again with the last step that it serves)
-      if (more && SPAN == 1) load_step<ZEROS, R, B, SPAN>(held, b, w, v, l_rg * R, l_kt, g, t);
-      if (more && SPAN == 2 && b % 2 == 1) {
-        load_step<ZEROS, R, B, SPAN>(held, b - 1, w, v, l_rg * R, l_kt, g, t);
-        load_step<ZEROS, R, B, SPAN>(held, b, w, v, l_rg * R, l_kt, g, t);
+    } else {   // the row ends inside the block
+      copy_wait<SLOTS - 1>();
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        if (kt + b < k_tiles) {
+          const bool in = (kt + b) * 64 + t * 16 < w.K;
+          uint4 x[NT][2];
+          if (in) load_x(x, kt + b);
+          else {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) x[j][0] = x[j][1] = make_uint4(0, 0, 0, 0);
+          }
+          multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, in, at + b * (R * 512), x, acc);
+        }
       }
     }
-    if (more) advance();
-    kt += kWarps * B;
-    if (kt >= whole * B) finish();
+    fill(at);
+    at = at == ring + (SLOTS - 1) * BYTES ? ring : at + BYTES;
+    kt = kt_next;
+    if (last) {
+      float* out = red + (rg * kWarps + warp) * (VALUES * 32) + lane;
+#pragma unroll
+      for (int a = 0; a < R; ++a)
+#pragma unroll
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            out[((a * NT + b) * 4 + c) * 32] = CH == 2 ? acc[a][b][0][c] + acc[a][b][CH - 1][c] : acc[a][b][0][c];
+#pragma unroll
+            for (int d = 0; d < CH; ++d) acc[a][b][d][c] = 0.f;
+          }
+      ++rg;
+    }
   }
-  if (mine == 0)
-    while (rg < rg1 - rg0) finish();
   __syncthreads();
+  const int with_work = min(kWarps, blocks);   // warps that had a block at all
   for (int u = warp; u < (rg1 - rg0) * VALUES; u += kWarps) {
     const int r = u / VALUES, q = u % VALUES;
     float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) sum += red[((r * kWarps + k) * VALUES + q) * 32 + lane];
+    for (int k = 0; k < with_work; ++k) sum += red[((r * kWarps + k) * VALUES + q) * 32 + lane];
     const int c = q & 3, j = (q >> 2) % NT, i = (q >> 2) / NT;
     const int n = ((rg0 + r) * R + i) * 16 + g + (c >> 1) * 8;    // weight row
     const int col = j * 8 + t * 2 + (c & 1);                       // row of the batch
@@ -257,51 +279,64 @@ __global__ void __launch_bounds__(kWarps * 32, 3)
 int4_small_down_direct_kernel(const SmallParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
-  constexpr int B = 4;
+  constexpr int B = 2, SLOTS = 4;
+  __shared__ __align__(128) unsigned char rings[kWarps][SLOTS][B * 512];
   __shared__ float red[kWarps][2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const Int4Weight& w = p.w;
   const int token = blockIdx.y, tile_row = blockIdx.x;
-  const int kts = w.k_tiles(), units = kts * p.rows.top_k;
-  float lo = 0.f, hi = 0.f;
-  int u = static_cast<int>(static_cast<long long>(units) * warp / kWarps);
+  const int kts = w.k_tiles(), blocks = (kts + B - 1) / B, units = blocks * p.rows.top_k;
+  // the warp's share of the blocks of all choices; blocks of dropped choices are passed over
+  int u = static_cast<int>(static_cast<long long>(units) * warp / kWarps), ahead = u;
   const int end = static_cast<int>(static_cast<long long>(units) * (warp + 1) / kWarps);
-  while (u < end) {
-    const int j = u / kts, slot = token * p.rows.top_k + j;
-    const int kt0 = u - j * kts, kt1 = min(end - j * kts, kts);
-    u = j * kts + kt1;
-    const int expert = p.rows.ids[slot];
-    if (expert < 0 || expert >= p.rows.E) continue;
-    const View v{w.packed + expert * w.expert_bytes() + (t * 8 + g) * 16,
-                 static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
+  const int* ids = p.rows.ids + token * p.rows.top_k;
+  auto dropped = [&](int unit) {
+    const int e = ids[unit / blocks];
+    return e < 0 || e >= p.rows.E;
+  };
+  const uint32_t ring = smem_u32(rings[warp]) + lane * 16;
+  auto fill = [&](uint32_t slot) {
+    while (ahead < end && dropped(ahead)) ++ahead;
+    if (ahead < end) {
+      const int kt = (ahead % blocks) * B;
+      const uint8_t* src = w.packed + ids[ahead / blocks] * w.expert_bytes() + (static_cast<size_t>(tile_row) * kts + kt) * 512 + (t * 8 + g) * 16;
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        if (kt + b < kts) copy16(slot + b * 512, src + b * 512);
+      ++ahead;
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) fill(ring + i * (B * 512));
+  float lo = 0.f, hi = 0.f;
+  uint32_t at = ring;
+  for (; u < end; ++u) {
+    if (dropped(u)) continue;
+    const int j = u / blocks, slot = token * p.rows.top_k + j, expert = ids[j], kt = (u % blocks) * B;
+    const View v{w.packed, static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
                  ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
     const T* h = static_cast<const T*>(p.x) + static_cast<long long>(slot) * w.K + t * 16;
     float acc[1][1][2][4] = {};
-    int kt = kt0;
-    const int kt_whole = min(kt1, w.K / 64);
-    for (; kt + B <= kt_whole; kt += B) {
-      Held<ZEROS, 1, B, 1> held;
-      uint4 x[B][1][2];
+    Scales<ZEROS, 1, B, 1> sc;
+    load_scales<ZEROS, 1, B, 1>(sc, w, v, tile_row, kt, g, t);
+    uint4 x[B][1][2];
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        load_step<ZEROS, 1, B, 1>(held, b, w, v, tile_row, kt, g, t);
-        x[b][0][0] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64) + b * 8);
-        x[b][0][1] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64) + b * 8 + 1);
+    for (int b = 0; b < B; ++b) {
+      x[b][0][0] = x[b][0][1] = make_uint4(0, 0, 0, 0);
+      if ((kt + b) * 64 + t * 16 < w.K) {
+        x[b][0][0] = __ldg(reinterpret_cast<const uint4*>(h + (kt + b) * 64));
+        x[b][0][1] = __ldg(reinterpret_cast<const uint4*>(h + (kt + b) * 64) + 1);
       }
+    }
+    copy_wait<SLOTS - 1>();
 #pragma unroll
-      for (int b = 0; b < B; ++b) multiply<BF16, ZEROS, 1, 1, B, 1, 2>(held, b, x[b], acc);
-    }
-    for (; kt < kt1; ++kt) {
-      Held<ZEROS, 1, 1, 1> held;
-      load_edge<ZEROS, 1>(held, w, v, tile_row, kt, g, t);
-      uint4 x[1][2] = {};
-      if (kt * 64 + t * 16 < w.K) {
-        x[0][0] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64));
-        x[0][1] = __ldg(reinterpret_cast<const uint4*>(h + kt * 64) + 1);
-      }
-      multiply<BF16, ZEROS, 1, 1, 1, 1, 2>(held, 0, x, acc);
-    }
+    for (int b = 0; b < B; ++b)
+      if (kt + b < kts)
+        multiply<BF16, ZEROS, 1, 1, B, 1, 2>(sc, b, (kt + b) * 64 + t * 16 < w.K, at + b * 512, x[b], acc);
+    fill(at);
+    at = at == ring + (SLOTS - 1) * (B * 512) ? ring : at + B * 512;
     const float weight = p.rows.weights[slot];
     lo += weight * (acc[0][0][0][0] + acc[0][0][1][0]);
     hi += weight * (acc[0][0][0][2] + acc[0][0][1][2]);
@@ -324,16 +359,16 @@ int sm_count() {
 }
 
 // MAX_GROUPS: row groups whose sums a block has room for in shared memory
-template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int MIN_BLOCKS, int MAX_GROUPS>
+template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int SLOTS, int MIN_BLOCKS, int MAX_GROUPS>
 int launch_one(const SmallParams& p, int blocks_y, cudaStream_t s) {
-  auto kernel = int4_small_kernel<BF16, ZEROS, MODE, NT, R, B, SPAN, MIN_BLOCKS>;
+  auto kernel = int4_small_kernel<BF16, ZEROS, MODE, NT, R, B, SPAN, SLOTS, MIN_BLOCKS>;
   const int groups = (p.w.row_tiles() + R - 1) / R;
   // as many blocks as run at once, if that leaves them no more row groups than they have room for; else whole rounds of them
   const int slots = max(1, sm_count() * MIN_BLOCKS / blocks_y);
   const int rounds = (groups + slots * MAX_GROUPS - 1) / (slots * MAX_GROUPS);
   const int blocks = static_cast<int>(min(static_cast<long long>(groups), static_cast<long long>(slots) * rounds));
   const int per_block = (groups + blocks - 1) / blocks;
-  const size_t smem = static_cast<size_t>(per_block) * kWarps * R * NT * 4 * 32 * sizeof(float);
+  const size_t smem = kWarps * SLOTS * R * B * 512 + static_cast<size_t>(per_block) * kWarps * R * NT * 4 * 32 * sizeof(float);
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return VQG_ERR_LAUNCH;
@@ -348,11 +383,11 @@ int launch_rows(const SmallParams& p, int rows, int blocks_y, bool bf16, cudaStr
     constexpr bool B = decltype(type)::value, Z = decltype(zeros)::value;
     const bool pairs = p.w.group % 128 == 0;
     if (rows <= 8) {
-      if (p.w.K < 64 * 4 * kWarps) return launch_one<B, Z, MODE, 1, 1, 2, 1, 3, 8>(p, blocks_y, s);
-      return pairs ? launch_one<B, Z, MODE, 1, 1, 4, 2, 3, 8>(p, blocks_y, s) : launch_one<B, Z, MODE, 1, 1, 4, 1, 3, 8>(p, blocks_y, s);
+      if (p.w.K < 64 * 4 * kWarps) return launch_one<B, Z, MODE, 1, 1, 2, 1, 4, 3, 8>(p, blocks_y, s);
+      return pairs ? launch_one<B, Z, MODE, 1, 1, 4, 2, 3, 3, 8>(p, blocks_y, s) : launch_one<B, Z, MODE, 1, 1, 4, 1, 3, 3, 8>(p, blocks_y, s);
     }
-    if (rows <= 16) return launch_one<B, Z, MODE, 2, 2, 2, 1, 2, 4>(p, blocks_y, s);
-    return launch_one<B, Z, MODE, 4, 2, 2, 1, 2, 2>(p, blocks_y, s);
+    if (rows <= 16) return launch_one<B, Z, MODE, 2, 2, 2, 1, 3, 2, 4>(p, blocks_y, s);
+    return launch_one<B, Z, MODE, 4, 2, 2, 1, 3, 2, 2>(p, blocks_y, s);
   };
   if (p.w.zeros) return bf16 ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
   return bf16 ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});

@@ -36,7 +36,7 @@ def _ws(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
     to another tensor of the same graph."""
     if nbytes == 0:
         return None
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    key = (device.index, _stream_ptr(device))
     cur = _workspaces.get(key)
     if cur is None or cur.numel() < nbytes:
         if cur is not None:
@@ -48,15 +48,15 @@ def _ws(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
 
 
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
-    dev = tensors[0].device
+    index = tensors[0].get_device()
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError("vq_gemm_b200 has no CPU path: all tensors must be CUDA tensors")
-        if t.device != dev:
+        if t.get_device() != index:
             raise RuntimeError("all tensors must be on the same CUDA device")
         if not t.is_contiguous():
             raise RuntimeError("tensors must be contiguous")
-    return dev
+    return tensors[0].device
 
 
 def _idx_bytes(indices: torch.Tensor) -> int:
@@ -68,7 +68,15 @@ def _idx_bytes(indices: torch.Tensor) -> int:
 
 
 def _stream_ptr(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _launch(dev: torch.device, fn, *args) -> int:
+    """fn(*args, stream) with ``dev`` current; entering a device that is current already costs microseconds."""
+    if torch._C._cuda_getDevice() == dev.index:
+        return fn(*args, _stream_ptr(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _stream_ptr(dev))
 
 
 def auto_path(M: int, N: int, K: int, v: int, C: int, index_bits: int = 8, rows_per_codebook: int = 0, layout: str = "bl") -> str:
@@ -352,13 +360,12 @@ def int4_gemm(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
     M, K = x.shape
     N, group = _int4_weight(packed, scales, zeros, K, False)
     if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=dev)
+        out = x.new_empty((M, N))
     elif tuple(out.shape) != (M, N) or out.dtype != x.dtype or not out.is_contiguous() or out.device != dev:
         raise RuntimeError("out must be a contiguous [M, N] tensor of x's type on the inputs' device")
-    with torch.cuda.device(dev):
-        ws = _ws(dev, lib.vqg_int4_workspace_bytes(M, N, K))
-        st = lib.vqg_int4_gemm(x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), M, N, K, group,
-                               _INT4_TYPES[x.dtype], _ptr(ws), 0 if ws is None else ws.numel(), _stream_ptr(dev))
+    ws = _ws(dev, lib.vqg_int4_workspace_bytes(M, N, K))
+    st = _launch(dev, lib.vqg_int4_gemm, x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), M, N, K,
+                 group, _INT4_TYPES[x.dtype], _ptr(ws), 0 if ws is None else ws.numel())
     _lib.check(st, "int4_gemm")
     return out
 
@@ -378,9 +385,8 @@ def int4_dequant(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[tor
         out = torch.empty(shape, dtype=scales.dtype, device=dev)
     elif tuple(out.shape) != shape or out.dtype != scales.dtype or out.device != dev or not out.is_contiguous():
         raise RuntimeError(f"out must be a contiguous tensor of shape {shape} and of the type of scales on {dev}")
-    with torch.cuda.device(dev):
-        st = lib.vqg_int4_dequant(packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), E, N, K, group,
-                                  _INT4_TYPES[scales.dtype], _stream_ptr(dev))
+    st = _launch(dev, lib.vqg_int4_dequant, packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), E, N, K, group,
+                 _INT4_TYPES[scales.dtype])
     _lib.check(st, "int4_dequant")
     return out
 
@@ -410,12 +416,10 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     top_groups = groups if top_groups is None else top_groups
     if E < 1 or not 1 <= top_k <= E or groups < 1 or E % groups or not 1 <= top_groups <= groups:
         raise RuntimeError(f"cannot choose {top_k} of {E} experts in {top_groups} of {groups} groups")
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    experts = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        st = lib.vqg_route_experts(logits.data_ptr(), _ptr(bias), weights.data_ptr(), experts.data_ptr(), T, E, top_k,
-                                   int(scoring == "sigmoid"), groups, top_groups, int(group_score == "max"),
-                                   int(renormalize), scale, _LOGIT_TYPES[logits.dtype], _stream_ptr(dev))
+    weights = logits.new_empty((T, top_k), dtype=torch.float32)
+    experts = logits.new_empty((T, top_k), dtype=torch.int32)
+    st = _launch(dev, lib.vqg_route_experts, logits.data_ptr(), _ptr(bias), weights.data_ptr(), experts.data_ptr(), T, E, top_k,
+                 scoring == "sigmoid", groups, top_groups, group_score == "max", renormalize, scale, _LOGIT_TYPES[logits.dtype])
     _lib.check(st, "route_experts")
     return weights, experts
 
@@ -446,15 +450,13 @@ def int4_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, 
     if dn_rows != hidden or dn_p.shape[0] != E:
         raise RuntimeError(f"down must be [{E}, {hidden}, {inner}] to follow gate_up")
     if out is None:
-        out = torch.empty((T, hidden), dtype=x.dtype, device=dev)
+        out = x.new_empty((T, hidden))
     elif tuple(out.shape) != (T, hidden) or out.dtype != x.dtype or not out.is_contiguous() or out.device != dev:
         raise RuntimeError("out must be a contiguous [T, hidden] tensor of x's type on the inputs' device")
-    with torch.cuda.device(dev):
-        ws = torch.empty(lib.vqg_int4_experts_workspace_bytes(T, top_k, E, hidden, inner), dtype=torch.uint8, device=dev)
-        st = lib.vqg_int4_experts(x.data_ptr(), experts.data_ptr(), weights.data_ptr(), up_p.data_ptr(), up_s.data_ptr(),
-                                  _ptr(up_z), dn_p.data_ptr(), dn_s.data_ptr(), _ptr(dn_z), out.data_ptr(), T, top_k, E,
-                                  hidden, inner, up_group, down_group, _INT4_TYPES[x.dtype], ws.data_ptr(), ws.numel(),
-                                  _stream_ptr(dev))
+    ws = torch.empty(lib.vqg_int4_experts_workspace_bytes(T, top_k, E, hidden, inner), dtype=torch.uint8, device=dev)
+    st = _launch(dev, lib.vqg_int4_experts, x.data_ptr(), experts.data_ptr(), weights.data_ptr(), up_p.data_ptr(),
+                 up_s.data_ptr(), _ptr(up_z), dn_p.data_ptr(), dn_s.data_ptr(), _ptr(dn_z), out.data_ptr(), T, top_k, E, hidden,
+                 inner, up_group, down_group, _INT4_TYPES[x.dtype], ws.data_ptr(), ws.numel())
     _lib.check(st, "int4_experts")
     return out
 

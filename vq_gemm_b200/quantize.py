@@ -21,7 +21,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _idx_bytes, _require_cuda, _stream_ptr
+from .ops import _idx_bytes, _launch, _ptr, _require_cuda, _stream_ptr
 
 
 def _shape(weight: torch.Tensor, codebook: torch.Tensor, rows_per_codebook: int):
@@ -177,10 +177,8 @@ def int4_quantize(weight: torch.Tensor, *, group: int = 128, symmetric: bool = T
     packed = torch.empty(lead + (-(-N // 16), -(-K // 64), 512), dtype=torch.uint8, device=dev)
     scales = torch.empty(lead + (K // group, N), dtype=weight.dtype, device=dev)
     zeros = None if symmetric else torch.empty(lead + (K // group, N), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        st = lib.vqg_int4_quantize(weight.data_ptr(), packed.data_ptr(), scales.data_ptr(),
-                                   None if zeros is None else zeros.data_ptr(), lead[0] if lead else 1, N, K, group,
-                                   int(weight.dtype == torch.bfloat16), _stream_ptr(dev))
+    st = _launch(dev, lib.vqg_int4_quantize, weight.data_ptr(), packed.data_ptr(), scales.data_ptr(), _ptr(zeros),
+                 lead[0] if lead else 1, N, K, group, weight.dtype == torch.bfloat16)
     _lib.check(st, "quantize.int4_quantize")
     return packed, scales, zeros
 
