@@ -8,6 +8,8 @@
 //   weight = p[id], divided by their sum if asked, times `scale`
 //
 // An expert whose logit is -inf or NaN is never chosen; slots for which nothing is left get id -1 and weight 0.
+#include <type_traits>
+
 #include "int4.cuh"
 
 namespace vqg {
@@ -17,6 +19,7 @@ constexpr int kRouteWarps = 4;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr double kNone = -1e300;   // choice of an expert that cannot be chosen, in 64 bits; -inf in 32
 
+// type: 0 fp16, 1 bf16, 2 fp32
 __device__ __forceinline__ float load_logit(const void* p, int type, long long i) {
   if (type == 2) return __ldg(static_cast<const float*>(p) + i);
   const unsigned short v = __ldg(static_cast<const unsigned short*>(p) + i);
@@ -30,6 +33,7 @@ struct RouteParams {
   int* ids;
   int T, E, top_k, type, sigmoid, groups, top_groups, group_max, renormalize;
   float scale;
+  unsigned size_magic;   // e / (E / groups) = e * size_magic >> 32 for e < 512: ceil(2^32 / size); 0 for a size of one
 };
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -140,23 +144,27 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
 // One warp per token, in 32 bits, with a proof that 64 would choose the same: choices that follow one another in the order (and
 // the last kept and first dropped group) must be further apart than the arithmetic below can be wrong; rows where they are
 // not are done again in 64 bits.  Without bias and groups the order is that of the logits themselves, which are compared
-// exactly.  A row of 256 experts costs some 500 warp instructions, most of them in the top_k rounds (a maximum over the warp,
-// the lowest index that has it, a new maximum for the lane that lost it): the kernel is bound by issue, not by its bytes.
-template <int EPL>
+// exactly.
+//
+// Selection: at least top_k + 1 choices are as large as the (top_k + 1)-th largest of the 32 lanes' maxima, and few more are
+// (about ten in all for 8 of 256).  Those go to a list in shared memory and are ranked by comparing each with all of them.
+// The kernel is bound by issue, not by its bytes.
+template <int EPL, int TYPE>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_kernel(const RouteParams p) {
-  __shared__ double s_choice[kRouteWarps][EPL * 32];
+  __shared__ double s_all[kRouteWarps][EPL * 32 + EPL * 16 + 50];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * kRouteWarps + warp;
   if (token >= p.T) return;
+  double* scratch = s_all[warp];
   const bool plain = !p.bias && p.groups == 1;
   float choice[EPL], prob[EPL];   // prob: exp(logit - top) or the sigmoid
   float top = -INFINITY;
+  const long long row = static_cast<long long>(token) * p.E + lane;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
     float l = -INFINITY;
-    if (e < p.E) l = fmaxf(load_logit(p.logits, p.type, static_cast<long long>(token) * p.E + e), -INFINITY);   // NaN: -inf
+    if (lane + 32 * i < p.E) l = fmaxf(load_logit(p.logits, TYPE, row + 32 * i), -INFINITY);   // NaN: -inf
     choice[i] = l;
     top = fmaxf(top, l);
   }
@@ -165,7 +173,7 @@ route_kernel(const RouteParams p) {
   float inverse = 1.f;            // of the softmax's sum
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) prob[i] = 1.f / (1.f + expf(-choice[i]));
+    for (int i = 0; i < EPL; ++i) prob[i] = __fdividef(1.f, 1.f + expf(-choice[i]));
   } else {
     float sum = 0.f;
 #pragma unroll
@@ -176,24 +184,23 @@ route_kernel(const RouteParams p) {
     sum = warp_sum(sum);
     inverse = sum > 0.f ? 1.f / sum : 0.f;
   }
-  // 32-bit errors, relative to p: the exponential 2^-22, its sum with one and the division 2^-24 each; in the softmax also the
+  // 32-bit errors, relative to p: the exponential 2^-22, its sum with one 2^-24, the reciprocal 2^-22; in the softmax also the
   // exponent's difference (at most 2^-25 of it, times what is left of p) and a sum of at most 16 + 5 roundings.  Adding the bias
   // rounds once more.  `slack` is twice what that comes to, relative to what goes in.
   const float slack = p.sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18);
   if (!plain) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 32 * i;
       if (choice[i] > -INFINITY) {
         prob[i] *= inverse;
-        choice[i] = p.bias ? fmaxf(prob[i] + __ldg(p.bias + e), -INFINITY) : prob[i];
+        choice[i] = p.bias ? fmaxf(prob[i] + __ldg(p.bias + lane + 32 * i), -INFINITY) : prob[i];
       }
     }
     inverse = 1.f;
   }
   if (p.groups > 1) {
     const int size = p.E / p.groups;
-    float* s = reinterpret_cast<float*>(s_choice[warp]);
+    float* s = reinterpret_cast<float*>(scratch);
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
       if (lane + 32 * i < p.E) s[lane + 32 * i] = choice[i];
@@ -203,8 +210,8 @@ route_kernel(const RouteParams p) {
     const int group = lane >> (5 - shift), sub = lane & (per - 1);
     float first = -INFINITY, second = -INFINITY;
     if (group < p.groups) {
-      const int n = (size - sub + per - 1) / per;
-      int at = n > 0 ? group % n : 0;
+      const int n = (size - sub + per - 1) >> (5 - shift);
+      int at = n > group ? group : 0;
       for (int i = 0; i < n; ++i) {
         const float c = s[group * size + sub + per * at];
         if (++at == n) at = 0;
@@ -230,61 +237,80 @@ route_kernel(const RouteParams p) {
     const float low = keep && score > -INFINITY ? score - 2.f * slack * size_of : INFINITY;
     const float high = mine && !keep && score > -INFINITY ? score + 2.f * slack * size_of : -INFINITY;
     sure = sure && -warp_max(-low) > warp_max(high);
-    unsigned kept = __ballot_sync(kAll, keep);        // bit of each kept group's first lane
+    const unsigned kept = __ballot_sync(kAll, keep);        // bit of each kept group's first lane
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 32 * i;
-      if (e < p.E && !(kept >> ((e / size) << (5 - shift)) & 1u)) choice[i] = -INFINITY;
+      const unsigned e = static_cast<unsigned>(lane + 32 * i), of = p.size_magic ? __umulhi(e, p.size_magic) : e;
+      if (!(kept >> (of << (5 - shift)) & 1u)) choice[i] = -INFINITY;
     }
+    __syncwarp();
   }
-  // the lane's largest choice, the lowest index first
-  float best = -INFINITY, best_p = 0.f;
-  int best_e = 0x7fffffff;
-  auto rescan = [&]() {
-    best = -INFINITY; best_p = 0.f; best_e = 0x7fffffff;
+  // the (top_k + 1)-th largest of the lanes' maxima: a bitonic sort, largest first
+  float bound = -INFINITY;
+  if (p.top_k < 32) {
+    float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (choice[i] > best) { best = choice[i]; best_p = prob[i]; best_e = lane + 32 * i; }
-  };
-  rescan();
-  float chosen = 0.f, total = 0.f, last = INFINITY, last_p = 0.f;
-  int id = -1;
-  for (int j = 0; j <= p.top_k; ++j) {
-    const float m = warp_max(best);
-    if (m == -INFINITY) break;
-    if (m == INFINITY) sure = false;                   // (a bias of +inf)
-    const int e = static_cast<int>(__reduce_min_sync(kAll, best == m ? static_cast<unsigned>(best_e) : 0x7fffffffu));
-    const float pe = __shfl_sync(kAll, best_p, e & 31);
-    // is this one surely behind the one before it?
-    if (plain) {
-      // different logits have different exponentials unless they are nearly equal or far out; equal ones are equal in 64 bits too
-      sure = sure && (last == INFINITY || last == m || (last - m > 1e-12f && (p.sigmoid ? last < 16.f && m > -600.f : m - top > -600.f)));
-      if (last == m && p.sigmoid && m <= -600.f) sure = false;
-    } else {
-      sure = sure && (last == INFINITY || last - m > slack * (last_p + pe + fabsf(last) + fabsf(m)));
-    }
-    if (j == p.top_k) break;
-    last = m;
-    last_p = pe;
-    if (lane == j) { chosen = pe; id = e; }
-    total += pe;
-    if (best_e == e) {
+    for (int i = 0; i < EPL; ++i) m = fmaxf(m, choice[i]);
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (e == lane + 32 * i) choice[i] = -INFINITY;
-      rescan();
-    }
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int d = k >> 1; d; d >>= 1) {
+        const float o = __shfl_xor_sync(kAll, m, d);
+        m = ((lane & d) == 0) == ((lane & k) == 0) ? fmaxf(m, o) : fminf(m, o);
+      }
+    bound = __shfl_sync(kAll, m, p.top_k);
   }
-  if (id >= 0 && total < 1e-6f) sure = false;         // weights that 32 bits may not tell from zero
+  // the list: choice and expert, and p, of each candidate; behind it the first top_k + 1 in order
+  float2* list = reinterpret_cast<float2*>(scratch);
+  float* list_p = reinterpret_cast<float*>(scratch + EPL * 32);
+  float* sorted_c = list_p + EPL * 32;
+  float* sorted_p = sorted_c + 33;
+  int* sorted_e = reinterpret_cast<int*>(sorted_p + 33);
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const bool in = choice[i] >= bound && choice[i] > -INFINITY;
+    const unsigned votes = __ballot_sync(kAll, in);
+    if (in) {
+      const int at = count + __popc(votes & ((1u << lane) - 1u));
+      list[at] = make_float2(choice[i], __int_as_float(lane + 32 * i));
+      list_p[at] = prob[i];
+    }
+    count += __popc(votes);
+  }
+  __syncwarp();
+  const int wanted = min(p.top_k, count);
+  for (int c = lane; c < count; c += 32) {
+    const float2 mine = list[c];
+    const int e = __float_as_int(mine.y);
+    int rank = 0;
+    for (int o = 0; o < count; ++o) {
+      const float2 other = list[o];
+      rank += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
+    }
+    if (rank <= p.top_k) { sorted_c[rank] = mine.x; sorted_p[rank] = list_p[c]; sorted_e[rank] = e; }
+  }
+  __syncwarp();
+  const float chosen_p = lane < wanted ? sorted_p[lane] : 0.f;
+  const int id = lane < wanted ? sorted_e[lane] : -1;
+  if (lane + 1 < min(count, p.top_k + 1)) {   // is number lane + 1 surely behind number lane?
+    const float a = sorted_c[lane], b = sorted_c[lane + 1];
+    if (plain)   // different logits have different exponentials unless they are nearly equal or far out; equal ones are equal in 64 bits too
+      sure = sure && (p.sigmoid ? b > -600.f && (a == b || (a - b > 1e-12f && a < 16.f)) : a == b || (a - b > 1e-12f && b - top > -600.f));
+    else
+      sure = sure && a < INFINITY && a - b > slack * (sorted_p[lane] + sorted_p[lane + 1] + fabsf(a) + fabsf(b));
+  }
+  const float total = warp_sum(chosen_p);
+  if (wanted > 0 && total < 1e-6f) sure = false;      // weights that 32 bits may not tell from zero
   if (__ballot_sync(kAll, !sure)) {
     __syncwarp();
-    route_row_64<EPL>(p, token, s_choice[warp]);
+    route_row_64<EPL>(p, token, scratch);
     return;
   }
   if (lane < p.top_k) {
-    chosen = p.renormalize ? (total > 0.f ? chosen / total : 0.f) : chosen * inverse;
+    const float weight = p.renormalize ? (total > 0.f ? chosen_p / total : 0.f) : chosen_p * inverse;
     const long long o = static_cast<long long>(token) * p.top_k + lane;
-    p.weights[o] = chosen * p.scale;
+    p.weights[o] = weight * p.scale;
     p.ids[o] = id;
   }
 }
@@ -351,18 +377,27 @@ int launch_route_experts(const void* logits, int logits_type, const float* bias,
                          int top_k, int scoring, int groups, int top_groups, int group_score, bool renormalize, float scale,
                          cudaStream_t s) {
   RouteParams p{logits, bias, weights, ids, T, E, top_k, logits_type, scoring, groups, top_groups, group_score,
-                renormalize ? 1 : 0, scale};
+                renormalize ? 1 : 0, scale, 0};
+  const int size = E / groups;
+  p.size_magic = size > 1 ? static_cast<unsigned>(((1ULL << 32) + size - 1) / size) : 0u;
   const int blocks = (T + kRouteWarps - 1) / kRouteWarps;
   auto go = [&](auto kernel) {
     kernel<<<blocks, kRouteWarps * 32, 0, s>>>(p);
     count_launch();
     return cuda_status(cudaGetLastError());
   };
-  if (E <= 64) return go(route_kernel<2>);
-  if (E <= 128) return go(route_kernel<4>);
-  if (E <= 256) return go(route_kernel<8>);
-  if (E <= 512) return go(route_kernel<16>);
-  return VQG_ERR_UNSUPPORTED;
+  auto with = [&](auto type) {
+    constexpr int Y = decltype(type)::value;
+    if (E <= 32) return go(route_kernel<1, Y>);
+    if (E <= 64) return go(route_kernel<2, Y>);
+    if (E <= 128) return go(route_kernel<4, Y>);
+    if (E <= 256) return go(route_kernel<8, Y>);
+    return go(route_kernel<16, Y>);
+  };
+  if (E > 512) return static_cast<int>(VQG_ERR_UNSUPPORTED);
+  if (logits_type == 0) return with(std::integral_constant<int, 0>{});
+  if (logits_type == 1) return with(std::integral_constant<int, 1>{});
+  return with(std::integral_constant<int, 2>{});
 }
 
 int launch_expert_plan(const int* ids, int slots, int E, int chunk_rows, int* row_slot, int4* chunks, int* n_chunks,
