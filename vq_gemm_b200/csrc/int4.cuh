@@ -128,23 +128,21 @@ __device__ __forceinline__ uint32_t int4_pair(uint32_t w, uint32_t off, uint32_t
   using I = Int4Type<BF16>;
   return I::mul(I::sub(and_or(w >> (8 * Q + 4 * H), 0x000f000fu, I::kMagic), off), s2);
 }
-// The four pairs of a word at once: rows g and g + 8, columns (0, 1) and (2, 3).  In fp16 the high codes are not shifted down:
-// 1024 + 16 code, times 1/16, minus 64 + zero is exact too and saves two shifts (bf16 has too few mantissa bits for that).
+// The same for row half 1 with the offset that int4_offset_hi gives.  In fp16 the high codes are not shifted down: 1024 + 16 code,
+// times 1/16, minus 64 + zero is exact too and saves the shift (bf16 has too few mantissa bits for that).
+template <bool BF16, int Q>
+__device__ __forceinline__ uint32_t int4_pair_hi(uint32_t w, uint32_t off_hi, uint32_t s2) {
+  using I = Int4Type<BF16>;
+  if constexpr (BF16) return int4_pair<BF16, 1, Q>(w, off_hi, s2);
+  else return I::mul(I::fma(and_or(w >> (8 * Q), 0x00f000f0u, I::kMagic), 0x2c002c00u, off_hi), s2);
+}
+// The four pairs of a word at once: rows g and g + 8, columns (0, 1) and (2, 3).
 template <bool BF16>
 __device__ __forceinline__ void int4_word(uint32_t w, uint32_t off_lo, uint32_t off_hi, uint32_t s_lo, uint32_t s_hi, uint32_t (&a)[4]) {
-  using I = Int4Type<BF16>;
-  if constexpr (BF16) {
-    a[0] = int4_pair<BF16, 0, 0>(w, off_lo, s_lo);
-    a[1] = int4_pair<BF16, 1, 0>(w, off_hi, s_hi);
-    a[2] = int4_pair<BF16, 0, 1>(w, off_lo, s_lo);
-    a[3] = int4_pair<BF16, 1, 1>(w, off_hi, s_hi);
-  } else {   // off_hi: -(64 + zero), see int4_offset_hi
-    const uint32_t v = w >> 8;
-    a[0] = I::mul(I::sub(and_or(w, 0x000f000fu, I::kMagic), off_lo), s_lo);
-    a[1] = I::mul(I::fma(and_or(w, 0x00f000f0u, I::kMagic), 0x2c002c00u, off_hi), s_hi);
-    a[2] = I::mul(I::sub(and_or(v, 0x000f000fu, I::kMagic), off_lo), s_lo);
-    a[3] = I::mul(I::fma(and_or(v, 0x00f000f0u, I::kMagic), 0x2c002c00u, off_hi), s_hi);
-  }
+  a[0] = int4_pair<BF16, 0, 0>(w, off_lo, s_lo);
+  a[1] = int4_pair_hi<BF16, 0>(w, off_hi, s_hi);
+  a[2] = int4_pair<BF16, 0, 1>(w, off_lo, s_lo);
+  a[3] = int4_pair_hi<BF16, 1>(w, off_hi, s_hi);
 }
 // what int4_word wants as the offset of row g + 8: fp16 -(64 + zero) twice (0xd400 = -64, steps of 1/16)
 template <bool BF16>

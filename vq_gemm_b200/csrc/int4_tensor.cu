@@ -40,8 +40,8 @@ constexpr uint32_t kTmemCols = 512, kAccCols = 256, kStageCols = KS * BK / 2;
 constexpr uint32_t kPacked = STAGES * kXStage;
 constexpr uint32_t kStaging = kPacked + STAGES * kPStage; // [256 rows][128 weight rows] of 16 bits
 constexpr uint32_t kBars = kStaging + BM * BNH * 2;
-constexpr uint32_t kNumBars = 4 * STAGES + 3;             // full, empty, packed full, packed empty; accumulator full, empty; epilogue
-constexpr uint32_t kTmemSlot = kBars + kNumBars * 8;
+constexpr uint32_t kNumBars = 4 * STAGES + 5;             // full, empty, packed full, packed empty; accumulator full, empty; epilogue; sums
+constexpr uint32_t kTmemSlot = kBars + (kNumBars + 1) / 2 * 16;
 constexpr uint32_t kSmem = kTmemSlot + 16;
 static_assert(kSmem + 1024 <= 227 * 1024, "shared memory");
 static_assert(kAccCols + STAGES * kStageCols <= kTmemCols, "tensor memory");
@@ -127,6 +127,10 @@ struct Walk {
     return true;
   }
 };
+// Weight row, within the CTA's 128, that tensor-memory lane 32 q + l holds.  Quarters 0 and 1 hold rows 0 ... 7 of the row tiles,
+// whose codes are the low four bits of the bytes, quarters 2 and 3 rows 8 ... 15: the shifts of a decoding warp are then
+// constants.  Eight neighbouring lanes are eight neighbouring rows.
+__device__ __forceinline__ int row_of_lane(int q, int l) { return ((q & 1) * 4 + (l >> 3)) * 16 + (q >> 1) * 8 + (l & 7); }
 __device__ __forceinline__ int mma_rows(int rows) { return (rows + 31) & ~31; }
 
 __device__ __forceinline__ void mma_pair_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -168,7 +172,7 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
 
 template <bool BF16, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParams p) {
+int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_x32, const TensorParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
   extern __shared__ unsigned char smem_dyn[];
@@ -187,6 +191,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
   const uint32_t bar_acc_full = base + kBars + 8 * (4 * STAGES);
   const uint32_t bar_acc_empty = base + kBars + 8 * (4 * STAGES + 1);
   const uint32_t bar_epi = base + kBars + 8 * (4 * STAGES + 2);
+  auto bar_red = [&](int i) { return base + kBars + 8 * (4 * STAGES + 3 + i); };
   const uint32_t to_peer = map_to_cta(base, rank ^ 1u) - base;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + kTmemSlot);
 
@@ -202,6 +207,8 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
     mbar_init(bar_acc_full, 1);
     mbar_init(bar_acc_empty, 8);
     mbar_init(bar_epi, 4);
+    mbar_init(bar_red(0), 1);
+    mbar_init(bar_red(1), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
@@ -217,7 +224,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ------------------------------- X producer ---------------------------------------------
       if (lane == 0) {
@@ -227,15 +234,17 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
         Walk<MODE> walk(pair_id, n_pairs, p);
         Segment g;
         while (ok && walk.next(g, p)) {
-          const int half = mma_rows(g.rows) / 2, boxes = (half + 31) / 32;
+          const int half = mma_rows(g.rows) / 2;
+          const int boxes = half > 64 ? 1 : (half + 31) / 32;       // one box of 128 rows, or one or two of 32
+          const CUtensorMap* map = half > 64 ? &tmap_x : &tmap_x32;
+          const int box_rows = half > 64 ? 128 : 32;
           const int row = g.row0 + static_cast<int>(rank) * half;
           for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
             if (!(ok = mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
-            mbar_expect_tx(bar_full(stage), KS * boxes * 4096);
+            mbar_expect_tx(bar_full(stage), KS * boxes * box_rows * (BK * 2));
             for (int u = 0; u < KS; ++u)
               for (int b = 0; b < boxes; ++b)
-                tma_load_2d(base + stage * kXStage + u * kXStep + b * 4096, &tmap_x, (kt * KS + u) * BK, row + 32 * b,
-                            bar_full(stage));
+                tma_load_2d(base + stage * kXStage + u * kXStep + b * 4096, map, (kt * KS + u) * BK, row + 32 * b, bar_full(stage));
             if (++stage == STAGES) { stage = 0; phase ^= 1; }
           }
         }
@@ -315,8 +324,8 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
   } else if (warp < 8) {
     // ------------------------------- epilogue -----------------------------------------------------
     // lane = weight row, column = row of X
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-    const int quarter = warp & 3;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int quarter = warp & 3, my_row = row_of_lane(quarter, lane);
     uint32_t acc_phase = 0, epi_phase = 0;
     bool ok = true;
     const uint32_t leader_acc_empty = bar_acc_empty + (rank == 0 ? 0u : to_peer);
@@ -333,6 +342,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(leader_acc_empty);
     };
+    uint32_t red_phase[2] = {0, 0};
     volatile int* last_flag = reinterpret_cast<volatile int*>(base_ptr + kTmemSlot + 8);
     constexpr int OUT_COLS = MODE == kGated ? BNH / 2 : BNH;   // output columns of this CTA's half tile
     constexpr int ROW_BYTES = OUT_COLS * 2;
@@ -347,9 +357,9 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
       acc_phase ^= 1;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       if constexpr (MODE == kDown) {
-        // fp32 rows of the slots: 32 lanes are 32 consecutive floats, stored straight from the registers
-        float* part = static_cast<float*>(p.y) + n0 + quarter * 32 + lane;
-        const bool row_ok = n0 + quarter * 32 + lane < w.N;
+        // fp32 rows of the slots, stored straight from the registers: eight lanes are 32 consecutive bytes
+        float* part = static_cast<float*>(p.y) + n0 + my_row;
+        const bool row_ok = n0 + my_row < w.N;
 #pragma unroll 1
         for (int c = 0; c < cols; c += 32) {
           uint32_t r[32];
@@ -367,7 +377,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
         if (g.whole) {
           if constexpr (MODE == kGated) {
             // lanes 2i and 2i + 1 hold gate and up of output column i; one exchange finishes two columns of the tile
-            T* col = reinterpret_cast<T*>(stg) + ((quarter * 32 + lane) >> 1);
+            T* col = reinterpret_cast<T*>(stg) + (my_row >> 1);
             const bool odd = (lane & 1) != 0;
             uint32_t ra[32];
 #pragma unroll 1
@@ -401,7 +411,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
                 for (int j = 0; j < 8; ++j) hp[(c + 1) * 8 + j] = pack_pair<BF16>(__uint_as_float(qb[2 * j]), __uint_as_float(qb[2 * j + 1]));
               }
             }
-            unsigned short* col = reinterpret_cast<unsigned short*>(stg) + quarter * 32 + lane;
+            unsigned short* col = reinterpret_cast<unsigned short*>(stg) + my_row;
 #pragma unroll
             for (int q = 0; q < BM / 2; ++q) {
               if (2 * q < cols) {
@@ -424,7 +434,11 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
           const int t0u = g.tile * p.units_per_tile;
           const int b_first = pair_of_unit(t0u, p.q, p.r);
           const int b_last = pair_of_unit(t0u + p.units_per_tile - 1, p.q, p.r);
+          // The contributor that arrives last sums all partials in pair order, so the result does not depend on who that is.
+          // They come through the staging tile by bulk copies of 64 rows of X, two in flight: loads by 128 threads alone were
+          // a chain of L2 round trips (45 us for five contributors).
           __threadfence();
+          asm volatile("fence.proxy.async.global;" ::: "memory");
           if (!(ok = epi_sync())) break;
           if (warp == 4 && lane == 0) {
             int* ctr = p.ws_counter + g.tile * 2 + static_cast<int>(rank);
@@ -433,37 +447,64 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
             *last_flag = last;
           }
           if (!(ok = epi_sync())) break;
-          const int last = *last_flag;
-          if (!last) {
-            if (!(ok = epi_sync())) break;
-            continue;
-          }
-          __threadfence();
-          // a thread sums four weight rows of one row of X at a time, eight loads in flight per contributor
-          const int et = quarter * 32 + lane, row4 = (et & 31) * 4, msub = et >> 5;
-          constexpr int INFL = 8;
-#pragma unroll 1
-          for (int i0 = 0; i0 < cols / 4; i0 += INFL) {
-            float4 sum[INFL];
-#pragma unroll
-            for (int j = 0; j < INFL; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int b = b_first; b <= b_last; ++b) {
+          if (*last_flag) {
+            __threadfence();
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            const int contributors = b_last - b_first + 1, chunks = (cols + 63) / 64, steps = contributors * chunks;
+            auto fetch = [&](int step) {
+              const int b = b_first + step % contributors, chunk = step / contributors;
               const int sl = (pair_begin(b, p.q, p.r) > t0u) ? 0 : 1;
-              const float* src = p.ws_partial + ((static_cast<size_t>(b) * 2 + sl) * 2 + rank) * kPartialFloats + row4;
-              float4 v[INFL];
-#pragma unroll
-              for (int j = 0; j < INFL; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(src + static_cast<size_t>(4 * (i0 + j) + msub) * BNH));
-#pragma unroll
-              for (int j = 0; j < INFL; ++j) { sum[j].x += v[j].x; sum[j].y += v[j].y; sum[j].z += v[j].z; sum[j].w += v[j].w; }
+              const float* src = p.ws_partial + ((static_cast<size_t>(b) * 2 + sl) * 2 + rank) * kPartialFloats + static_cast<size_t>(chunk) * 64 * BNH;
+              const uint32_t bytes = min(64, cols - chunk * 64) * BNH * 4;
+              mbar_expect_tx(bar_red(step & 1), bytes);
+              bulk_load(base + kStaging + (step & 1) * 32768, src, bytes, bar_red(step & 1));
+            };
+            if (warp == 4 && lane == 0) {
+              fence_async_smem();
+              fetch(0);
+              if (steps > 1) fetch(1);
             }
+            // four consecutive lanes' rows of every fourth row of X
+            const int et = quarter * 32 + lane, lane4 = (et & 31) * 4, msub = et >> 5;
+            const int n4 = n0 + row_of_lane(lane4 >> 5, lane4 & 31);
+            float4 sum[16];
+            for (int step = 0; ok && step < steps; ++step) {
+              const int b = step % contributors, chunk = step / contributors;
+              if (b == 0) {
 #pragma unroll
-            for (int j = 0; j < INFL; ++j) {
-              uint2 o;
-              o.x = pack_pair<BF16>(sum[j].x, sum[j].y);
-              o.y = pack_pair<BF16>(sum[j].z, sum[j].w);
-              *reinterpret_cast<uint2*>(stg + (4 * (i0 + j) + msub) * 256 + row4 * 2) = o;
+                for (int j = 0; j < 16; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+              }
+              if (!(ok = mbar_wait(bar_red(step & 1), red_phase[step & 1], p.status, DS_SPLITK_TIMEOUT))) break;
+              red_phase[step & 1] ^= 1;
+              const float4* src = reinterpret_cast<const float4*>(stg + (step & 1) * 32768) + (et & 31);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float4 v = src[(4 * j + msub) * 32];
+                sum[j].x += v.x; sum[j].y += v.y; sum[j].z += v.z; sum[j].w += v.w;
+              }
+              if (!(ok = epi_sync())) break;                 // the buffer has been read
+              if (warp == 4 && lane == 0 && step + 2 < steps) { fence_async_smem(); fetch(step + 2); }
+              if (b == contributors - 1) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  const int m = chunk * 64 + 4 * j + msub;
+                  if (m < g.rows) {
+                    T* out = static_cast<T*>(p.y) + static_cast<long long>(g.row0 + m) * w.N + n4;
+                    if (w.N % 4 == 0) {
+                      if (n4 < w.N) *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<BF16>(sum[j].x, sum[j].y), pack_pair<BF16>(sum[j].z, sum[j].w));
+                    } else {
+                      const float v[4] = {sum[j].x, sum[j].y, sum[j].z, sum[j].w};
+#pragma unroll
+                      for (int c = 0; c < 4; ++c)
+                        if (n4 + c < w.N) out[c] = I::from_float(v[c]);
+                    }
+                  }
+                }
+              }
             }
           }
+          if (!ok || !(ok = epi_sync())) break;   // the flag and the staging tile are free again
+          continue;
         }
         if (!(ok = epi_sync())) break;   // the whole tile is in shared memory
         const int out_n = MODE == kGated ? w.N / 2 : w.N, out0 = MODE == kGated ? n0 / 2 : n0;
@@ -487,8 +528,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
   } else {
     // ------------------------------- decoding -----------------------------------------------------
     const int quarter = warp & 3, sub = (warp - 8) >> 2;       // the step of a stage that this warp decodes
-    const int r = quarter * 32 + lane;                         // weight row in the CTA = tensor-memory lane
-    const uint32_t sh = (r & 8) ? 4 : 0;                       // rows 8 ... 15 of a tile sit in the high four bits
+    const int r = row_of_lane(quarter, lane);                  // weight row in the CTA
     const uint32_t src = base + kPacked + (r / 16) * (KS * 512) + sub * 512 + (r & 7) * 16;
     const uint32_t a_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols + sub * (BK / 2);
     int stage = 0;
@@ -496,29 +536,37 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
     bool ok = true;
     Walk<MODE> walk(pair_id, n_pairs, p);
     Segment g;
+    const bool halves = w.group == 32;                         // columns 0 ... 31 and 32 ... 63 of a step have scales of their own
     while (ok && walk.next(g, p)) {
       const int n = g.n0 + static_cast<int>(rank) * BNH + r;
       const bool row_ok = n < w.N;
-      const unsigned short* sc = static_cast<const unsigned short*>(w.scales) + g.expert * w.expert_scales() + n;
-      const uint8_t* ze = w.zeros ? w.zeros + g.expert * w.expert_scales() + n : nullptr;
-      // scale (twice) and offset of columns k ... k + 15; nothing there: a scale of zero, so that no fill reaches the sum
-      auto fetch = [&](int k, uint32_t& s2, uint32_t& off) {
-        s2 = 0; off = I::offset(8);
-        if (row_ok && k < w.K) {
-          const long long at = static_cast<long long>(int4_group_of(w, k)) * w.N;
-          s2 = __ldg(sc + at) * 0x10001u;
-          if (ze) off = I::offset(__ldg(ze + at) & 15);
+      // Scales and zero points, a stage ahead and as loaded: nothing is computed from them before the stage in hand is done, or
+      // the warp would wait for memory here.  Rows and columns that do not exist read the last ones and get a scale of zero, so
+      // that no fill reaches a sum.
+      const int nc = min(n, w.N - 1);
+      const unsigned short* sc = static_cast<const unsigned short*>(w.scales) + g.expert * w.expert_scales() + nc;
+      const uint8_t* ze = w.zeros ? w.zeros + g.expert * w.expert_scales() + nc : nullptr;
+      unsigned short raw[2] = {0, 0};
+      uint8_t zero[2] = {8, 8};
+      auto fetch = [&](int kt) {
+        const int k = (kt * KS + sub) * BK;
+        const int at = int4_group_of(w, min(k, w.K - 32)) * w.N;
+        raw[0] = __ldg(sc + at);
+        if (ze) zero[0] = __ldg(ze + at);
+        if (halves) {
+          const int at2 = int4_group_of(w, min(k + 32, w.K - 32)) * w.N;
+          raw[1] = __ldg(sc + at2);
+          if (ze) zero[1] = __ldg(ze + at2);
         }
       };
-      uint32_t s_lo, s_hi, o_lo, o_hi;     // columns 0 ... 31 and 32 ... 63 of the step
-      fetch((g.kt_begin * KS + sub) * BK, s_lo, o_lo);
-      fetch((g.kt_begin * KS + sub) * BK + 32, s_hi, o_hi);
+      fetch(g.kt_begin);
       for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
-        const uint32_t s2[2] = {s_lo, s_hi}, off[2] = {o_lo, o_hi};
-        if (kt + 1 < g.kt_end) {
-          fetch(((kt + 1) * KS + sub) * BK, s_lo, o_lo);
-          fetch(((kt + 1) * KS + sub) * BK + 32, s_hi, o_hi);
-        }
+        const int k = (kt * KS + sub) * BK;
+        uint32_t s2[2], off[2];
+        s2[0] = row_ok && k < w.K ? raw[0] * 0x10001u : 0u;
+        s2[1] = row_ok && k + 32 < w.K ? (halves ? raw[1] : raw[0]) * 0x10001u : 0u;
+        const int z0 = zero[0] & 15, z1 = halves ? zero[1] & 15 : z0;
+        if (kt + 1 < g.kt_end) fetch(kt + 1);
         if (!(ok = mbar_wait(bar_pfull(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
         uint32_t c[16], a[32];
 #pragma unroll
@@ -526,11 +574,20 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const TensorParam
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                        : "=r"(c[4 * t]), "=r"(c[4 * t + 1]), "=r"(c[4 * t + 2]), "=r"(c[4 * t + 3])
                        : "r"(src + stage * kPStage + t * 128));
+        if (quarter < 2) {
+          off[0] = I::offset(z0); off[1] = I::offset(z1);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t v = c[i] >> sh;
-          a[2 * i] = I::mul(I::sub((v & 0x000f000fu) | I::kMagic, off[i >> 3]), s2[i >> 3]);
-          a[2 * i + 1] = I::mul(I::sub(((v >> 8) & 0x000f000fu) | I::kMagic, off[i >> 3]), s2[i >> 3]);
+          for (int i = 0; i < 16; ++i) {
+            a[2 * i] = int4_pair<BF16, 0, 0>(c[i], off[i >> 3], s2[i >> 3]);
+            a[2 * i + 1] = int4_pair<BF16, 0, 1>(c[i], off[i >> 3], s2[i >> 3]);
+          }
+        } else {
+          off[0] = int4_offset_hi<BF16>(z0); off[1] = int4_offset_hi<BF16>(z1);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            a[2 * i] = int4_pair_hi<BF16, 0>(c[i], off[i >> 3], s2[i >> 3]);
+            a[2 * i + 1] = int4_pair_hi<BF16, 1>(c[i], off[i >> 3], s2[i >> 3]);
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_pempty(stage));
@@ -578,13 +635,13 @@ EncodeFn encode_fn() {
   }();
   return fn;
 }
-// 16-bit row-major [rows, cols], box of 32 rows x 64 columns, zero fill (the columns that fill up the last step among it)
-bool make_x_map(CUtensorMap* map, const void* ptr, int rows, int cols, bool bf16) {
+// 16-bit row-major [rows, cols], box of box_rows rows x 64 columns, zero fill (the columns that fill up the last step among it)
+bool make_x_map(CUtensorMap* map, const void* ptr, int rows, int cols, int box_rows, bool bf16) {
   EncodeFn fn = encode_fn();
   if (!fn) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
-  const cuuint32_t box[2] = {BK, 32};
+  const cuuint32_t box[2] = {BK, static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1, 1};
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(ptr), dims,
             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -598,10 +655,12 @@ int sm_pairs() {
 constexpr size_t kPairPartialBytes = 2 * 2 * static_cast<size_t>(BM) * BNH * sizeof(float);
 
 template <typename Kernel>
-int launch(Kernel kernel, int pairs, const CUtensorMap& map, const TensorParams& p, cudaStream_t s) {
+int launch(Kernel kernel, int pairs, const void* x, int rows, bool bf16, const TensorParams& p, cudaStream_t s) {
   constexpr int smem = kSmem + 1024;
+  CUtensorMap map, map32;
+  if (!make_x_map(&map, x, rows, p.w.K, 128, bf16) || !make_x_map(&map32, x, rows, p.w.K, 32, bf16)) return VQG_ERR_LAUNCH;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return VQG_ERR_LAUNCH;
-  kernel<<<2 * pairs, kThreads, smem, s>>>(map, p);
+  kernel<<<2 * pairs, kThreads, smem, s>>>(map, map32, p);
   count_launch();
   return cuda_status(cudaGetLastError());
 }
@@ -613,8 +672,6 @@ size_t int4_tensor_workspace_bytes() {
 }
 
 int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool bf16, void* ws, size_t ws_bytes, cudaStream_t s) {
-  CUtensorMap map;
-  if (!make_x_map(&map, x, M, w.K, bf16)) return VQG_ERR_LAUNCH;
   TensorParams p{};
   p.w = w; p.y = y; p.M = M;
   p.status = device_status_ptr();
@@ -634,14 +691,12 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   p.r = static_cast<int>(units % pairs);
   p.ws_counter = split ? static_cast<int*>(ws) : nullptr;
   p.ws_partial = split ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes) : nullptr;
-  return bf16 ? launch(int4_tensor_kernel<true, kDense>, pairs, map, p, s) : launch(int4_tensor_kernel<false, kDense>, pairs, map, p, s);
+  return bf16 ? launch(int4_tensor_kernel<true, kDense>, pairs, x, M, true, p, s) : launch(int4_tensor_kernel<false, kDense>, pairs, x, M, false, p, s);
 }
 
 namespace {
 int launch_experts(const Int4Weight& w, const void* x, void* y, const ExpertRows& rows, int max_chunks, bool bf16, bool gated,
                    cudaStream_t s) {
-  CUtensorMap map;
-  if (!make_x_map(&map, x, rows.slots, w.K, bf16)) return VQG_ERR_LAUNCH;
   TensorParams p{};
   p.w = w; p.y = y; p.rows = rows;
   p.status = device_status_ptr();
@@ -649,8 +704,8 @@ int launch_experts(const Int4Weight& w, const void* x, void* y, const ExpertRows
   const long long most = static_cast<long long>(max_chunks) * p.n_tiles;
   if (most > 0x7fffffffLL) return VQG_ERR_UNSUPPORTED;
   const int pairs = most < sm_pairs() ? static_cast<int>(most) : sm_pairs();
-  if (gated) return bf16 ? launch(int4_tensor_kernel<true, kGated>, pairs, map, p, s) : launch(int4_tensor_kernel<false, kGated>, pairs, map, p, s);
-  return bf16 ? launch(int4_tensor_kernel<true, kDown>, pairs, map, p, s) : launch(int4_tensor_kernel<false, kDown>, pairs, map, p, s);
+  if (gated) return bf16 ? launch(int4_tensor_kernel<true, kGated>, pairs, x, rows.slots, true, p, s) : launch(int4_tensor_kernel<false, kGated>, pairs, x, rows.slots, false, p, s);
+  return bf16 ? launch(int4_tensor_kernel<true, kDown>, pairs, x, rows.slots, true, p, s) : launch(int4_tensor_kernel<false, kDown>, pairs, x, rows.slots, false, p, s);
 }
 }  // namespace
 
