@@ -227,26 +227,25 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
       // ------------------------------- X producer ---------------------------------------------
-      if (lane == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        Walk<MODE> walk(pair_id, n_pairs, p);
-        Segment g;
-        while (ok && walk.next(g, p)) {
-          const int half = mma_rows(g.rows) / 2;
-          const int boxes = half > 64 ? 1 : (half + 31) / 32;       // one box of 128 rows, or one or two of 32
-          const CUtensorMap* map = half > 64 ? &tmap_x : &tmap_x32;
-          const int box_rows = half > 64 ? 128 : 32;
-          const int row = g.row0 + static_cast<int>(rank) * half;
-          for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
-            if (!(ok = mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
-            mbar_expect_tx(bar_full(stage), KS * boxes * box_rows * (BK * 2));
-            for (int u = 0; u < KS; ++u)
-              for (int b = 0; b < boxes; ++b)
-                tma_load_2d(base + stage * kXStage + u * kXStep + b * 4096, map, (kt * KS + u) * BK, row + 32 * b, bar_full(stage));
-            if (++stage == STAGES) { stage = 0; phase ^= 1; }
-          }
+      // the whole warp walks; lane u * boxes + b issues one box (a single lane would need longer than a stage takes)
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      Walk<MODE> walk(pair_id, n_pairs, p);
+      Segment g;
+      while (ok && walk.next(g, p)) {
+        const int half = mma_rows(g.rows) / 2;
+        const int boxes = half > 64 ? 1 : (half + 31) / 32;       // one box of 128 rows, or one or two of 32
+        const CUtensorMap* map = half > 64 ? &tmap_x : &tmap_x32;
+        const int box_rows = half > 64 ? 128 : 32;
+        const int u = lane / boxes, b = lane % boxes;
+        const int row = g.row0 + static_cast<int>(rank) * half + 32 * b;
+        for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+          if (!(ok = mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
+          if (lane == 0) mbar_expect_tx(bar_full(stage), KS * boxes * box_rows * (BK * 2));
+          __syncwarp();
+          if (u < KS) tma_load_2d(base + stage * kXStage + u * kXStep + b * 4096, map, (kt * KS + u) * BK, row, bar_full(stage));
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
     } else if (warp == 1) {
@@ -298,26 +297,24 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       }
     } else if (warp == 2) {
       // ------------------------------- packed-weight producer -----------------------------------
-      if (lane == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        Walk<MODE> walk(pair_id, n_pairs, p);
-        Segment g;
-        const int k_tiles = w.k_tiles();
-        while (ok && walk.next(g, p)) {
-          const int tile0 = (g.n0 + static_cast<int>(rank) * BNH) / 16;
-          const int tiles = max(0, min(BNH / 16, w.row_tiles() - tile0));
-          const uint8_t* src = w.packed + g.expert * w.expert_bytes() + static_cast<long long>(tile0) * k_tiles * 512;
-          for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
-            if (!(ok = mbar_wait(bar_pempty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
-            const uint32_t bytes = min(KS, k_tiles - kt * KS) * 512;
-            mbar_expect_tx(bar_pfull(stage), tiles * bytes);
-            for (int i = 0; i < tiles; ++i)
-              bulk_load(base + kPacked + stage * kPStage + i * (KS * 512), src + (static_cast<long long>(i) * k_tiles + kt * KS) * 512,
-                        bytes, bar_pfull(stage));
-            if (++stage == STAGES) { stage = 0; phase ^= 1; }
-          }
+      // lane i copies the stage's columns of row tile i
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      Walk<MODE> walk(pair_id, n_pairs, p);
+      Segment g;
+      const int k_tiles = w.k_tiles();
+      while (ok && walk.next(g, p)) {
+        const int tile0 = (g.n0 + static_cast<int>(rank) * BNH) / 16;
+        const int tiles = max(0, min(BNH / 16, w.row_tiles() - tile0));
+        const uint8_t* src = w.packed + g.expert * w.expert_bytes() + static_cast<long long>(tile0 + lane) * k_tiles * 512;
+        for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+          if (!(ok = mbar_wait(bar_pempty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
+          const uint32_t bytes = min(KS, k_tiles - kt * KS) * 512;
+          if (lane == 0) mbar_expect_tx(bar_pfull(stage), tiles * bytes);
+          __syncwarp();
+          if (lane < tiles) bulk_load(base + kPacked + stage * kPStage + lane * (KS * 512), src + kt * (KS * 512), bytes, bar_pfull(stage));
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
     }
@@ -455,11 +452,13 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
               const int b = b_first + step % contributors, chunk = step / contributors;
               const int sl = (pair_begin(b, p.q, p.r) > t0u) ? 0 : 1;
               const float* src = p.ws_partial + ((static_cast<size_t>(b) * 2 + sl) * 2 + rank) * kPartialFloats + static_cast<size_t>(chunk) * 64 * BNH;
-              const uint32_t bytes = min(64, cols - chunk * 64) * BNH * 4;
-              mbar_expect_tx(bar_red(step & 1), bytes);
-              bulk_load(base + kStaging + (step & 1) * 32768, src, bytes, bar_red(step & 1));
+              const uint32_t bytes = min(64, cols - chunk * 64) * (BNH * 4 / 8);   // in eight copies
+              if (lane == 0) mbar_expect_tx(bar_red(step & 1), 8 * bytes);
+              __syncwarp();
+              if (lane < 8)
+                bulk_load(base + kStaging + (step & 1) * 32768 + lane * bytes, reinterpret_cast<const uint8_t*>(src) + lane * bytes, bytes, bar_red(step & 1));
             };
-            if (warp == 4 && lane == 0) {
+            if (warp == 4) {
               fence_async_smem();
               fetch(0);
               if (steps > 1) fetch(1);
@@ -483,7 +482,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 sum[j].x += v.x; sum[j].y += v.y; sum[j].z += v.z; sum[j].w += v.w;
               }
               if (!(ok = epi_sync())) break;                 // the buffer has been read
-              if (warp == 4 && lane == 0 && step + 2 < steps) { fence_async_smem(); fetch(step + 2); }
+              if (warp == 4 && step + 2 < steps) { fence_async_smem(); fetch(step + 2); }
               if (b == contributors - 1) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
@@ -540,33 +539,39 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     while (ok && walk.next(g, p)) {
       const int n = g.n0 + static_cast<int>(rank) * BNH + r;
       const bool row_ok = n < w.N;
-      // Scales and zero points, a stage ahead and as loaded: nothing is computed from them before the stage in hand is done, or
+      // Scales and zero points, two stages ahead and as loaded: nothing is computed from them before the stage in hand is done, or
       // the warp would wait for memory here.  Rows and columns that do not exist read the last ones and get a scale of zero, so
       // that no fill reaches a sum.
       const int nc = min(n, w.N - 1);
       const unsigned short* sc = static_cast<const unsigned short*>(w.scales) + g.expert * w.expert_scales() + nc;
       const uint8_t* ze = w.zeros ? w.zeros + g.expert * w.expert_scales() + nc : nullptr;
-      unsigned short raw[2] = {0, 0};
-      uint8_t zero[2] = {8, 8};
+      struct Raw {
+        unsigned short s[2];
+        uint8_t z[2];
+      };
       auto fetch = [&](int kt) {
+        Raw f{{0, 0}, {8, 8}};
         const int k = (kt * KS + sub) * BK;
         const int at = int4_group_of(w, min(k, w.K - 32)) * w.N;
-        raw[0] = __ldg(sc + at);
-        if (ze) zero[0] = __ldg(ze + at);
+        f.s[0] = __ldg(sc + at);
+        if (ze) f.z[0] = __ldg(ze + at);
         if (halves) {
           const int at2 = int4_group_of(w, min(k + 32, w.K - 32)) * w.N;
-          raw[1] = __ldg(sc + at2);
-          if (ze) zero[1] = __ldg(ze + at2);
+          f.s[1] = __ldg(sc + at2);
+          if (ze) f.z[1] = __ldg(ze + at2);
         }
+        return f;
       };
-      fetch(g.kt_begin);
+      Raw next = fetch(g.kt_begin), after = fetch(g.kt_begin + 1);
       for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
         const int k = (kt * KS + sub) * BK;
+        const Raw now = next;
+        next = after;
+        after = fetch(kt + 2);
         uint32_t s2[2], off[2];
-        s2[0] = row_ok && k < w.K ? raw[0] * 0x10001u : 0u;
-        s2[1] = row_ok && k + 32 < w.K ? (halves ? raw[1] : raw[0]) * 0x10001u : 0u;
-        const int z0 = zero[0] & 15, z1 = halves ? zero[1] & 15 : z0;
-        if (kt + 1 < g.kt_end) fetch(kt + 1);
+        s2[0] = row_ok && k < w.K ? now.s[0] * 0x10001u : 0u;
+        s2[1] = row_ok && k + 32 < w.K ? (halves ? now.s[1] : now.s[0]) * 0x10001u : 0u;
+        const int z0 = now.z[0] & 15, z1 = halves ? now.z[1] & 15 : z0;
         if (!(ok = mbar_wait(bar_pfull(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
         uint32_t c[16], a[32];
 #pragma unroll
