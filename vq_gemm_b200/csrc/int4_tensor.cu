@@ -15,8 +15,10 @@
 //
 // Rows of a tile: 256 at most, rounded up to 32 for the instruction, so a short tile costs what it needs on the tensor pipe.
 // Tensor memory: columns [0, 256) accumulator, [256 + 64 s, +64) A stage s (two 64-column steps).
-// Schedule of the dense product: as in tensor3.cu, the K loops of all tiles are dealt out evenly over the pairs and pieces
-// of tiles are summed in pair order by whoever arrives last.  Experts: whole tiles, dealt out in turn.
+// Schedule of the dense product: the K loops of all tiles are cut into units and dealt out evenly over the pairs.  Pieces of
+// tiles go to the workspace in fp32 and a second kernel sums them in pair order: with 16 tiles over 74 pairs (256 x 4096 x
+// 4096) a sum by the contributor that arrives last, 128 threads at two 32 KiB copies in flight, took 45 of 68 thousand
+// cycles; a kernel of its own has all SMs for it.  Experts: whole tiles, dealt out in turn.
 // Every wait is bounded; no TMA load uses cluster multicast.
 #include "int4.cuh"
 #include "tc_ptx.cuh"
@@ -40,7 +42,7 @@ constexpr uint32_t kTmemCols = 512, kAccCols = 256, kStageCols = KS * BK / 2;
 constexpr uint32_t kPacked = STAGES * kXStage;
 constexpr uint32_t kStaging = kPacked + STAGES * kPStage; // [256 rows][128 weight rows] of 16 bits
 constexpr uint32_t kBars = kStaging + BM * BNH * 2;
-constexpr uint32_t kNumBars = 4 * STAGES + 5;             // full, empty, packed full, packed empty; accumulator full, empty; epilogue; sums
+constexpr uint32_t kNumBars = 4 * STAGES + 3;             // full, empty, packed full, packed empty; accumulator full, empty; epilogue
 constexpr uint32_t kTmemSlot = kBars + (kNumBars + 1) / 2 * 16;
 constexpr uint32_t kSmem = kTmemSlot + 16;
 static_assert(kSmem + 1024 <= 227 * 1024, "shared memory");
@@ -56,7 +58,6 @@ struct TensorParams {
   int m_tiles, n_tiles;
   int unit_stages, units_per_tile, q, r;   // see tensor3.cu
   float* ws_partial;         // [pair][piece][rank][256][128] fp32
-  int* ws_counter;           // [tile][rank]
   ExpertRows rows;
 };
 
@@ -191,7 +192,6 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   const uint32_t bar_acc_full = base + kBars + 8 * (4 * STAGES);
   const uint32_t bar_acc_empty = base + kBars + 8 * (4 * STAGES + 1);
   const uint32_t bar_epi = base + kBars + 8 * (4 * STAGES + 2);
-  auto bar_red = [&](int i) { return base + kBars + 8 * (4 * STAGES + 3 + i); };
   const uint32_t to_peer = map_to_cta(base, rank ^ 1u) - base;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + kTmemSlot);
 
@@ -207,8 +207,6 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     mbar_init(bar_acc_full, 1);
     mbar_init(bar_acc_empty, 8);
     mbar_init(bar_epi, 4);
-    mbar_init(bar_red(0), 1);
-    mbar_init(bar_red(1), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
@@ -222,6 +220,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -339,8 +338,6 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(leader_acc_empty);
     };
-    uint32_t red_phase[2] = {0, 0};
-    volatile int* last_flag = reinterpret_cast<volatile int*>(base_ptr + kTmemSlot + 8);
     constexpr int OUT_COLS = MODE == kGated ? BNH / 2 : BNH;   // output columns of this CTA's half tile
     constexpr int ROW_BYTES = OUT_COLS * 2;
     constexpr size_t kPartialFloats = static_cast<size_t>(BM) * BNH;
@@ -428,82 +425,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
 #pragma unroll
             for (int j = 0; j < 32; ++j) __stcg(part + static_cast<size_t>(c + j) * BNH, __uint_as_float(r[j]));
           }
-          const int t0u = g.tile * p.units_per_tile;
-          const int b_first = pair_of_unit(t0u, p.q, p.r);
-          const int b_last = pair_of_unit(t0u + p.units_per_tile - 1, p.q, p.r);
-          // The contributor that arrives last sums all partials in pair order, so the result does not depend on who that is.
-          // They come through the staging tile by bulk copies of 64 rows of X, two in flight: loads by 128 threads alone were
-          // a chain of L2 round trips (45 us for five contributors).
-          __threadfence();
-          asm volatile("fence.proxy.async.global;" ::: "memory");
-          if (!(ok = epi_sync())) break;
-          if (warp == 4 && lane == 0) {
-            int* ctr = p.ws_counter + g.tile * 2 + static_cast<int>(rank);
-            const int last = atomicAdd(ctr, 1) == b_last - b_first;
-            if (last) *ctr = 0;
-            *last_flag = last;
-          }
-          if (!(ok = epi_sync())) break;
-          if (*last_flag) {
-            __threadfence();
-            asm volatile("fence.proxy.async.global;" ::: "memory");
-            const int contributors = b_last - b_first + 1, chunks = (cols + 63) / 64, steps = contributors * chunks;
-            auto fetch = [&](int step) {
-              const int b = b_first + step % contributors, chunk = step / contributors;
-              const int sl = (pair_begin(b, p.q, p.r) > t0u) ? 0 : 1;
-              const float* src = p.ws_partial + ((static_cast<size_t>(b) * 2 + sl) * 2 + rank) * kPartialFloats + static_cast<size_t>(chunk) * 64 * BNH;
-              const uint32_t bytes = min(64, cols - chunk * 64) * (BNH * 4 / 8);   // in eight copies
-              if (lane == 0) mbar_expect_tx(bar_red(step & 1), 8 * bytes);
-              __syncwarp();
-              if (lane < 8)
-                bulk_load(base + kStaging + (step & 1) * 32768 + lane * bytes, reinterpret_cast<const uint8_t*>(src) + lane * bytes, bytes, bar_red(step & 1));
-            };
-            if (warp == 4) {
-              fence_async_smem();
-              fetch(0);
-              if (steps > 1) fetch(1);
-            }
-            // four consecutive lanes' rows of every fourth row of X
-            const int et = quarter * 32 + lane, lane4 = (et & 31) * 4, msub = et >> 5;
-            const int n4 = n0 + row_of_lane(lane4 >> 5, lane4 & 31);
-            float4 sum[16];
-            for (int step = 0; ok && step < steps; ++step) {
-              const int b = step % contributors, chunk = step / contributors;
-              if (b == 0) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-              }
-              if (!(ok = mbar_wait(bar_red(step & 1), red_phase[step & 1], p.status, DS_SPLITK_TIMEOUT))) break;
-              red_phase[step & 1] ^= 1;
-              const float4* src = reinterpret_cast<const float4*>(stg + (step & 1) * 32768) + (et & 31);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float4 v = src[(4 * j + msub) * 32];
-                sum[j].x += v.x; sum[j].y += v.y; sum[j].z += v.z; sum[j].w += v.w;
-              }
-              if (!(ok = epi_sync())) break;                 // the buffer has been read
-              if (warp == 4 && step + 2 < steps) { fence_async_smem(); fetch(step + 2); }
-              if (b == contributors - 1) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  const int m = chunk * 64 + 4 * j + msub;
-                  if (m < g.rows) {
-                    T* out = static_cast<T*>(p.y) + static_cast<long long>(g.row0 + m) * w.N + n4;
-                    if (w.N % 4 == 0) {
-                      if (n4 < w.N) *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<BF16>(sum[j].x, sum[j].y), pack_pair<BF16>(sum[j].z, sum[j].w));
-                    } else {
-                      const float v[4] = {sum[j].x, sum[j].y, sum[j].z, sum[j].w};
-#pragma unroll
-                      for (int c = 0; c < 4; ++c)
-                        if (n4 + c < w.N) out[c] = I::from_float(v[c]);
-                    }
-                  }
-                }
-              }
-            }
-          }
-          if (!ok || !(ok = epi_sync())) break;   // the flag and the staging tile are free again
-          continue;
+          continue;                        // int4_tensor_sum_kernel adds the pieces up
         }
         if (!(ok = epi_sync())) break;   // the whole tile is in shared memory
         const int out_n = MODE == kGated ? w.N / 2 : w.N, out0 = MODE == kGated ? n0 / 2 : n0;
@@ -617,6 +539,42 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   }
 }
 
+// Sums the pieces of the tiles that several pairs shared, in pair order.  blockIdx.y = pair: the tile that its range ends inside,
+// if this pair is the first to work on it; blockIdx.x and the thread: rank, row of X, four neighbouring weight rows.
+template <bool BF16>
+__global__ void __launch_bounds__(256)
+int4_tensor_sum_kernel(const TensorParams p) {
+  using I = Int4Type<BF16>;
+  using T = typename I::T;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int end = pair_begin(blockIdx.y + 1, p.q, p.r);
+  if (end % p.units_per_tile == 0) return;
+  const int tile = end / p.units_per_tile, t0u = tile * p.units_per_tile;
+  const int b_first = pair_of_unit(t0u, p.q, p.r), b_last = pair_of_unit(t0u + p.units_per_tile - 1, p.q, p.r);
+  if (b_first != static_cast<int>(blockIdx.y)) return;
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  const int lane4 = (i & 31) * 4, rank = (i >> 5) & 1, m = i >> 6;
+  const int row0 = (tile % p.m_tiles) * BM, n = (tile / p.m_tiles) * BN + rank * BNH + row_of_lane(lane4 >> 5, lane4 & 31);
+  if (m >= BM || row0 + m >= p.M || n >= p.w.N) return;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int b = b_first; b <= b_last; ++b) {
+    const int piece = pair_begin(b, p.q, p.r) > t0u ? 0 : 1;
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(
+        p.ws_partial + ((static_cast<size_t>(b) * 2 + piece) * 2 + rank) * (static_cast<size_t>(BM) * BNH) + static_cast<size_t>(m) * BNH + lane4));
+    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+  }
+  T* out = static_cast<T*>(p.y) + static_cast<long long>(row0 + m) * p.w.N + n;
+  if (p.w.N % 4 == 0) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_pair<BF16>(sum.x, sum.y), pack_pair<BF16>(sum.z, sum.w));
+  } else {
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (n + c < p.w.N) out[c] = I::from_float(v[c]);
+  }
+}
+
 // Rows of X in the order of the plan (one block per row).
 __global__ void __launch_bounds__(128)
 gather_rows_kernel(const uint4* __restrict__ x, const ExpertRows rows, uint4* __restrict__ out, int vecs) {
@@ -687,16 +645,30 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   if (tiles > 0x7fffffffLL / (stages + 1)) return VQG_ERR_UNSUPPORTED;
   const bool split = ws && reinterpret_cast<uintptr_t>(ws) % 256 == 0 &&
                      ws_bytes >= kCounterBytes + static_cast<size_t>(max_pairs) * kPairPartialBytes && stages > 1 &&
-                     tiles % max_pairs != 0 && tiles * 2 * sizeof(int) <= kCounterBytes;
+                     tiles % max_pairs != 0;
   p.unit_stages = split ? (stages >= 8 ? 2 : 1) : stages;
   p.units_per_tile = (stages + p.unit_stages - 1) / p.unit_stages;
   const long long units = tiles * p.units_per_tile;
   const int pairs = units < max_pairs ? static_cast<int>(units) : max_pairs;
   p.q = static_cast<int>(units / pairs);
   p.r = static_cast<int>(units % pairs);
-  p.ws_counter = split ? static_cast<int*>(ws) : nullptr;
   p.ws_partial = split ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes) : nullptr;
-  return bf16 ? launch(int4_tensor_kernel<true, kDense>, pairs, x, M, true, p, s) : launch(int4_tensor_kernel<false, kDense>, pairs, x, M, false, p, s);
+  const int st = bf16 ? launch(int4_tensor_kernel<true, kDense>, pairs, x, M, true, p, s)
+                      : launch(int4_tensor_kernel<false, kDense>, pairs, x, M, false, p, s);
+  if (st != VQG_OK || !split || pairs == 1) return st;
+  // enqueued so that it can take its place on the SMs as the first kernel leaves them; it waits for that one to complete
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(((M < BM ? M : BM) * 64 + 255) / 256, pairs - 1);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, int4_tensor_sum_kernel<true>, p) : cudaLaunchKernelEx(&cfg, int4_tensor_sum_kernel<false>, p);
+  count_launch();
+  return cuda_status(e);
 }
 
 namespace {
