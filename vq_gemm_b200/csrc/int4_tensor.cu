@@ -158,7 +158,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
@@ -351,39 +351,101 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       acc_phase ^= 1;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       if constexpr (MODE == kDown) {
-        // fp32 rows of the slots, stored straight from the registers: eight lanes are 32 consecutive bytes
-        float* part = static_cast<float*>(p.y) + n0 + my_row;
-        const bool row_ok = n0 + my_row < w.N;
-#pragma unroll 1
-        for (int c = 0; c < cols; c += 32) {
-          uint32_t r[32];
-          const int mine = c + lane < g.rows ? __ldg(p.rows.row_slot + g.row0 + c + lane) : -1;
-          tmem_ld32(t_row + c, r);
-          if (c + 32 >= cols) release();
+        // fp32 rows of the slots.  Rows 128 ... 255 of X wait in registers while rows 0 ... 127 go to the staging tile, so that
+        // tensor memory is free after one reading of it; each row leaves shared memory as one bulk copy of up to 512 bytes, which
+        // the stores of the next tile's accumulation do not wait for.  (Stores from the registers, a row address each, kept the
+        // accumulator for 12 to 19 thousand cycles per tile.)
+        float* part = static_cast<float*>(p.y) + n0;
+        const uint32_t bytes = n0 < w.N ? min(BNH, w.N - n0) * 4 : 0;     // a multiple of 128
+        float* col = reinterpret_cast<float*>(stg) + my_row;
+        auto send = [&](int first) {       // rows first ... first + 127 of the tile, one per lane
+          fence_async_smem();
+          if (!(ok = epi_sync())) return;
+          const int m = first + quarter * 32 + lane;
+          if (m < g.rows && bytes) {
+            const int slot = __ldg(p.rows.row_slot + g.row0 + m);
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                         ::"l"(part + static_cast<long long>(slot) * w.N), "r"(base + kStaging + (quarter * 32 + lane) * 512), "r"(bytes) : "memory");
+          }
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        };
+        auto sent = [&]() {                // the staging tile has been read
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          ok = epi_sync();
+        };
+        uint32_t late[4][32];
+        if (cols > 128) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int slot = __shfl_sync(0xffffffffu, mine, j);
-            if (slot >= 0 && row_ok) __stcs(part + static_cast<long long>(slot) * w.N, __uint_as_float(r[j]));
+          for (int i = 0; i < 4; ++i)
+            if (128 + 32 * i < cols) tmem_ld32_async(t_row + 128 + 32 * i, late[i]);
+        }
+#pragma unroll 1
+        for (int c = 0; c < min(cols, 128); c += 32) {
+          uint32_t r[32];
+          tmem_ld32_async(t_row + c, r);
+          tmem_ld_wait(r);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) col[(c + j) * BNH] = __uint_as_float(r[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_wait(late[i]);
+        release();
+        send(0);
+        if (ok && cols > 128) {
+          sent();
+          if (ok) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (128 + 32 * i < cols) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) col[(32 * i + j) * BNH] = __uint_as_float(late[i][j]);
+              }
+            send(128);
           }
         }
+        if (ok) sent();
+        if (!ok) break;
         continue;
       } else {
         if (g.whole) {
           if constexpr (MODE == kGated) {
-            // lanes 2i and 2i + 1 hold gate and up of output column i; one exchange finishes two columns of the tile
-            T* col = reinterpret_cast<T*>(stg) + (my_row >> 1);
+            // Lanes 2i and 2i + 1 hold gate and up of output column i.  One exchange per two rows of X: the even lane finishes the
+            // first, the odd lane the second.  The results wait in registers, two to one, until tensor memory is handed back.
+            uint32_t hp[BM / 4];
+            uint32_t qa[16], qb[16];
             const bool odd = (lane & 1) != 0;
-            uint32_t ra[32];
-#pragma unroll 1
-            for (int c = 0; c < cols; c += 32) {
-              tmem_ld32(t_row + c, ra);
-              if (c + 32 >= cols) release();
+            auto finish = [&](const uint32_t (&q)[16], uint32_t* out) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float send = odd ? __uint_as_float(ra[j]) : __uint_as_float(ra[j + 1]);
-                const float recv = __shfl_xor_sync(0xffffffffu, send, 1);
-                const float v = odd ? silu_mul(recv, __uint_as_float(ra[j + 1])) : silu_mul(__uint_as_float(ra[j]), recv);
-                col[(c + j + (odd ? 1 : 0)) * OUT_COLS] = I::from_float(v);
+              for (int j = 0; j < 16; j += 4) {
+                float v[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const float first = __uint_as_float(q[j + 2 * i]), second = __uint_as_float(q[j + 2 * i + 1]);
+                  const float recv = __shfl_xor_sync(0xffffffffu, odd ? first : second, 1);
+                  v[i] = silu_mul(odd ? recv : first, odd ? second : recv);
+                }
+                out[j / 4] = pack_pair<BF16>(v[0], v[1]);
+              }
+            };
+            tmem_ld16_async(t_row, qa);
+#pragma unroll
+            for (int c = 0; c < BM / 16; c += 2) {
+              if (c * 16 < cols) {
+                tmem_ld_wait16(qa);
+                tmem_ld16_async(t_row + (c + 1) * 16, qb);
+                finish(qa, hp + c * 4);
+                tmem_ld_wait16(qb);
+                if (c * 16 + 32 < cols) tmem_ld16_async(t_row + (c + 2) * 16, qa);
+                else release();
+                finish(qb, hp + (c + 1) * 4);
+              }
+            }
+            unsigned short* col = reinterpret_cast<unsigned short*>(stg) + (my_row >> 1) + (odd ? OUT_COLS : 0);
+#pragma unroll
+            for (int q = 0; q < BM / 4; ++q) {
+              if (4 * q < cols) {
+                col[(4 * q) * OUT_COLS] = static_cast<unsigned short>(hp[q] & 0xffffu);
+                col[(4 * q + 2) * OUT_COLS] = static_cast<unsigned short>(hp[q] >> 16);
               }
             }
           } else {
@@ -446,6 +508,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         if (!(ok = epi_sync())) break;   // the staging tile is rewritten by the next one
       }
     }
+    if constexpr (MODE == kDown) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // every copy is complete
   } else {
     // ------------------------------- decoding -----------------------------------------------------
     const int quarter = warp & 3, sub = (warp - 8) >> 2;       // the step of a stage that this warp decodes

@@ -315,41 +315,69 @@ route_kernel(const RouteParams p) {
   }
 }
 
-// Slots by expert, one block: counts in shared memory, an exclusive scan, places by atomics.  The order of an expert's rows
+// Slots by expert, one cluster of blocks: every block counts its share of the slots in shared memory, reads the others' counts from
+// theirs, and so knows where its rows of each expert begin; places within that by atomics.  The order of an expert's rows
 // depends on the atomics; no result does, every row of a product being computed on its own.
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kPlanBlocks = 8;
+__device__ __forceinline__ int cluster_load(const int* local, int rank) {
+  uint32_t at;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __global__ void __launch_bounds__(kPlanThreads)
 expert_plan_kernel(const int* __restrict__ ids, int slots, int E, int chunk_rows, int* __restrict__ row_slot,
                    int4* __restrict__ chunks, int* __restrict__ n_chunks) {
-  extern __shared__ int sm[];   // count [E], first row [E], first chunk [E]
-  int* count = sm;
-  int* row0 = sm + E;
-  int* chunk0 = sm + 2 * E;
-  for (int e = threadIdx.x; e < E; e += kPlanThreads) count[e] = 0;
+  __shared__ int count[512], place[512], scan[2][16];
+  const int blocks = gridDim.x, me = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < 512) count[tid] = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < slots; i += kPlanThreads) {
+  const int begin = static_cast<int>(static_cast<long long>(slots) * me / blocks), end = static_cast<int>(static_cast<long long>(slots) * (me + 1) / blocks);
+  for (int i = begin + tid; i < end; i += kPlanThreads) {
     const int e = ids[i];
     if (e >= 0 && e < E) atomicAdd(count + e, 1);
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int r = 0, c = 0;
-    for (int e = 0; e < E; ++e) {
-      row0[e] = r; chunk0[e] = c;
-      r += count[e]; c += (count[e] + chunk_rows - 1) / chunk_rows;
+  if (blocks > 1) cluster_sync(); else __syncthreads();
+  // thread e: rows of expert e in all, and in the blocks before this one; then rows and chunks of the experts before it
+  int all = 0, before = 0, rows = 0, parts = 0;
+  if (tid < 512) {
+    if (tid < E) {
+      for (int b = 0; b < blocks; ++b) {
+        const int c = b == me ? count[tid] : cluster_load(count + tid, b);
+        if (b < me) before += c;
+        all += c;
+      }
     }
-    n_chunks[0] = c;
-    n_chunks[1] = r;
+    rows = all;
+    parts = (all + chunk_rows - 1) / chunk_rows;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int r = __shfl_up_sync(kAll, rows, d), c = __shfl_up_sync(kAll, parts, d);
+      if (lane >= d) { rows += r; parts += c; }
+    }
+    if (lane == 31) { scan[0][warp] = rows; scan[1][warp] = parts; }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kPlanThreads)
-    for (int i = 0, c = chunk0[e]; i < count[e]; i += chunk_rows, ++c)
-      chunks[c] = make_int4(e, row0[e] + i, min(chunk_rows, count[e] - i), 0);
+  if (tid < 512) {
+    for (int k = 0; k < warp; ++k) { rows += scan[0][k]; parts += scan[1][k]; }
+    if (me == 0 && tid == 511) { n_chunks[0] = parts; n_chunks[1] = rows; }
+    rows -= all;
+    parts -= (all + chunk_rows - 1) / chunk_rows;
+    place[tid] = rows + before;
+    if (me == 0)
+      for (int i = 0; i < all; i += chunk_rows) chunks[parts++] = make_int4(tid, rows + i, min(chunk_rows, all - i), 0);
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < slots; i += kPlanThreads) {
+  for (int i = begin + tid; i < end; i += kPlanThreads) {
     const int e = ids[i];
-    if (e >= 0 && e < E) row_slot[atomicAdd(row0 + e, 1)] = i;
+    if (e >= 0 && e < E) row_slot[atomicAdd(place + e, 1)] = i;
   }
+  if (blocks > 1) cluster_sync();   // nobody leaves while its counts may be read
 }
 
 template <bool BF16>
@@ -402,10 +430,21 @@ int launch_route_experts(const void* logits, int logits_type, const float* bias,
 
 int launch_expert_plan(const int* ids, int slots, int E, int chunk_rows, int* row_slot, int4* chunks, int* n_chunks,
                        cudaStream_t s) {
-  expert_plan_kernel<<<1, kPlanThreads, static_cast<size_t>(E) * 3 * sizeof(int), s>>>(ids, slots, E, chunk_rows, row_slot,
-                                                                                       chunks, n_chunks);
+  // one block for a few thousand slots, a cluster of eight above (one block took 25 us for 32768 slots)
+  cudaLaunchConfig_t cfg{};
+  const int blocks = slots > 4 * kPlanThreads ? kPlanBlocks : 1;
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, expert_plan_kernel, ids, slots, E, chunk_rows, row_slot, chunks, n_chunks);
   count_launch();
-  return cuda_status(cudaGetLastError());
+  return cuda_status(e);
 }
 
 int launch_expert_combine(const float* part, const ExpertRows& rows, void* y, int tokens, int cols, bool bf16, cudaStream_t s) {
