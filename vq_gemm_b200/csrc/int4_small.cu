@@ -2,10 +2,12 @@
 // the experts of a mixture-of-experts layer over the rows that chose them.
 //
 // A warp takes blocks of B neighbouring 64-column steps of R row tiles (16 weight rows each).  A lane's 16 bytes of a tile give the
-// A fragments of four mma.sync m16n8k16, whose B fragments are 32 consecutive bytes of a row of X.  Every lane copies its
-// own 16 bytes of each tile asynchronously into its own places of a ring in shared memory, SLOTS blocks ahead, and reads them
-// back: nothing waits for another thread, and no register or scoreboard is tied up by a load from memory.  The eight warps'
-// sums of a row group meet in shared memory.
+// A fragments of four mma.sync m16n8k16, whose B fragments are 32 consecutive bytes of a row of X.  Every warp copies its tiles
+// asynchronously into a ring of its own in shared memory, SLOTS blocks ahead: no warp waits for another, and no register or
+// scoreboard is tied up by a load from memory.  The copies go in memory order, lane i the i-th 16 bytes (in the order in
+// which the lanes need them a quarter warp would touch four lines instead of one, which alone cost 14 of 46 us at 1 x
+// 28672 x 8192), into places that are swizzled so that neither side has bank conflicts: see place().  The eight warps' sums
+// of a row group meet in shared memory.
 #include <type_traits>
 
 #include "int4.cuh"
@@ -79,6 +81,10 @@ __device__ __forceinline__ void load_scales(Scales<ZEROS, R, B, SPAN>& h, const 
   }
 }
 
+// Place of the tile's 16-byte piece t * 8 + g.  Eight lanes of one instruction are one t and all g when they write, two
+// neighbouring g and all t when they read; either way the places fall into eight different groups of banks.
+__device__ __forceinline__ uint32_t place(int g, int t) { return static_cast<uint32_t>(t * 8 + (g ^ (2 * t))) * 16; }
+
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -144,7 +150,7 @@ int4_small_kernel(const SmallParams p) {
       if (expert < 0 || expert >= p.rows.E) return;
     }
   }
-  const View v{w.packed + expert * w.expert_bytes() + (t * 8 + g) * 16,
+  const View v{w.packed + expert * w.expert_bytes() + lane * 16,
                static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
                ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
   const int groups = (w.row_tiles() + R - 1) / R, k_tiles = w.k_tiles();
@@ -156,7 +162,8 @@ int4_small_kernel(const SmallParams p) {
   const int blocks = (k_tiles + B - 1) / B;
   const int mine = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0;
   const int total = mine * (rg1 - rg0);
-  const uint32_t ring = smem_u32(smem) + warp * (SLOTS * BYTES) + lane * 16;
+  const uint32_t ring = smem_u32(smem) + warp * (SLOTS * BYTES);
+  const uint32_t put = place(lane & 7, lane >> 3), get = place(g, t);
   int l_rg = rg0, l_kt = warp * B, left = total;
   auto fill = [&](uint32_t slot) {
     if (left > 0) {
@@ -166,11 +173,11 @@ int4_small_kernel(const SmallParams p) {
         const uint8_t* src = v.packed + (static_cast<size_t>(tr) * k_tiles + l_kt) * 512;
         if (l_kt + B <= k_tiles) {
 #pragma unroll
-          for (int b = 0; b < B; ++b) copy16(slot + (b * R + i) * 512, src + b * 512);
+          for (int b = 0; b < B; ++b) copy16(slot + put + (b * R + i) * 512, src + b * 512);
         } else {
 #pragma unroll
           for (int b = 0; b < B; ++b)
-            if (l_kt + b < k_tiles) copy16(slot + (b * R + i) * 512, src + b * 512);
+            if (l_kt + b < k_tiles) copy16(slot + put + (b * R + i) * 512, src + b * 512);
         }
       }
       --left;
@@ -212,13 +219,15 @@ int4_small_kernel(const SmallParams p) {
       uint4 x[2][NT][2];
       load_x(x[0], kt);
       copy_wait<SLOTS - 1>();
+      __syncwarp();
 #pragma unroll
       for (int b = 0; b < B; ++b) {
         if (b + 1 < B) load_x(x[(b + 1) & 1], kt + b + 1);
-        multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, true, at + b * (R * 512), x[b & 1], acc);
+        multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, true, at + get + b * (R * 512), x[b & 1], acc);
       }
     } else {   // the row ends inside the block
       copy_wait<SLOTS - 1>();
+      __syncwarp();
 #pragma unroll
       for (int b = 0; b < B; ++b) {
         if (kt + b < k_tiles) {
@@ -229,10 +238,11 @@ int4_small_kernel(const SmallParams p) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) x[j][0] = x[j][1] = make_uint4(0, 0, 0, 0);
           }
-          multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, in, at + b * (R * 512), x, acc);
+          multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, in, at + get + b * (R * 512), x, acc);
         }
       }
     }
+    __syncwarp();                                          // the slot has been read
     fill(at);
     at = at == ring + (SLOTS - 1) * BYTES ? ring : at + BYTES;
     kt = kt_next;
@@ -295,15 +305,16 @@ int4_small_down_direct_kernel(const SmallParams p) {
     const int e = ids[unit / blocks];
     return e < 0 || e >= p.rows.E;
   };
-  const uint32_t ring = smem_u32(rings[warp]) + lane * 16;
+  const uint32_t ring = smem_u32(rings[warp]);
+  const uint32_t put = place(lane & 7, lane >> 3), get = place(g, t);
   auto fill = [&](uint32_t slot) {
     while (ahead < end && dropped(ahead)) ++ahead;
     if (ahead < end) {
       const int kt = (ahead % blocks) * B;
-      const uint8_t* src = w.packed + ids[ahead / blocks] * w.expert_bytes() + (static_cast<size_t>(tile_row) * kts + kt) * 512 + (t * 8 + g) * 16;
+      const uint8_t* src = w.packed + ids[ahead / blocks] * w.expert_bytes() + (static_cast<size_t>(tile_row) * kts + kt) * 512 + lane * 16;
 #pragma unroll
       for (int b = 0; b < B; ++b)
-        if (kt + b < kts) copy16(slot + b * 512, src + b * 512);
+        if (kt + b < kts) copy16(slot + put + b * 512, src + b * 512);
       ++ahead;
     }
     copy_commit();
@@ -331,10 +342,12 @@ int4_small_down_direct_kernel(const SmallParams p) {
       }
     }
     copy_wait<SLOTS - 1>();
+    __syncwarp();
 #pragma unroll
     for (int b = 0; b < B; ++b)
       if (kt + b < kts)
-        multiply<BF16, ZEROS, 1, 1, B, 1, 2>(sc, b, (kt + b) * 64 + t * 16 < w.K, at + b * 512, x[b], acc);
+        multiply<BF16, ZEROS, 1, 1, B, 1, 2>(sc, b, (kt + b) * 64 + t * 16 < w.K, at + get + b * 512, x[b], acc);
+    __syncwarp();
     fill(at);
     at = at == ring + (SLOTS - 1) * (B * 512) ? ring : at + B * 512;
     const float weight = p.rows.weights[slot];
