@@ -15,13 +15,14 @@
 namespace vqg {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 8;                    // of a block of the direct down product
+constexpr size_t kSmallSmem = 227 * 1024;    // shared memory of a block, at most
 
 struct SmallParams {
   Int4Weight w;
   const void* x;
   void* y;
-  int M;
+  int M, chunks;             // chunks: of the dense product; for experts at most as many
   ExpertRows rows;
 };
 
@@ -30,11 +31,11 @@ enum { kDense = 0, kGated = 1, kDown = 2 };
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -95,12 +96,13 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 // acc += W X^T over step b, whose packed weights lie at `at` (row tiles 512 bytes apart) in shared memory;
 // x[j] are the lane's 32 bytes of row 8j + g of X
 template <bool BF16, bool ZEROS, int NT, int R, int B, int SPAN, int CH>
-__device__ __forceinline__ void multiply(const Scales<ZEROS, R, B, SPAN>& h, int b, bool in, uint32_t at,
+__device__ __forceinline__ void multiply(const Scales<ZEROS, R, B, SPAN>& h, int b, bool in, const unsigned char* at,
                                          const uint4 (&x)[NT][2], float (&acc)[R][NT][CH][4]) {
   uint32_t s_lo[R], s_hi[R], o_lo[R], o_hi[R], q[R][4];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[i][0]), "=r"(q[i][1]), "=r"(q[i][2]), "=r"(q[i][3]) : "r"(at + i * 512));
+    const uint4 c = *reinterpret_cast<const uint4*>(at + i * 512);
+    q[i][0] = c.x; q[i][1] = c.y; q[i][2] = c.z; q[i][3] = c.w;
     s_lo[i] = in ? h.s_lo[b / SPAN][i] * 0x10001u : 0u;
     s_hi[i] = in ? h.s_hi[b / SPAN][i] * 0x10001u : 0u;
     o_lo[i] = Int4Type<BF16>::offset(ZEROS ? h.z_lo[ZEROS ? b / SPAN : 0][i] & 15 : 8);
@@ -122,163 +124,201 @@ __device__ __forceinline__ void multiply(const Scales<ZEROS, R, B, SPAN>& h, int
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
-// Block (bx, by): row groups (R row tiles each) [groups * bx / grid, groups * (bx + 1) / grid) of the weight, rows `by` of X.
-// The eight warps take the blocks of a row group in turn, one row group after the other.
-template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int SLOTS, int MIN_BLOCKS>
-__global__ void __launch_bounds__(kWarps * 32, MIN_BLOCKS)
+// The work is chunks of rows of X (one for the dense product; the plan's or one per slot for experts) times the weight's row
+// groups (R row tiles each).  The grid is what runs at once; gridDim.x / chunks blocks share a chunk, and there are teams of TW
+// warps in a block, team n of the chunk's taking row groups [groups * n / teams, groups * (n + 1) / teams).  The warps of a
+// team take the blocks of a row group in turn; their sums meet every RGF row groups.  XS: the rows of X lie in shared memory,
+// 16 bytes apart from a multiple of 128, so that the reads of a quarter warp (two rows, four runs of 16 columns) have no bank
+// conflicts; else they are read from memory in the loop.
+template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int SLOTS, int WARPS, int TW, int MIN_BLOCKS, int RGF, bool XS>
+__global__ void __launch_bounds__(WARPS * 32, MIN_BLOCKS)
 int4_small_kernel(const SmallParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
+  constexpr int TEAMS = WARPS / TW;
   constexpr int CH = R * NT == 1 ? 2 : 1;   // chains of accumulators: a matrix instruction waits for the one before it
   constexpr int VALUES = R * NT * 4;        // sums of a lane per row group
   constexpr int BYTES = R * B * 512;
-  extern __shared__ __align__(128) unsigned char smem[];   // rings, sums [row group][warp][VALUES][lane]
-  float* red = reinterpret_cast<float*>(smem + kWarps * SLOTS * BYTES);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int RED = TW == 1 ? 0 : RGF * VALUES * 128;     // per warp
+  extern __shared__ __align__(128) unsigned char smem[];   // rings, sums [team][row group][warp][VALUES][lane], X
+  const int warp = (threadIdx.x >> 5) % TW, team = threadIdx.x / (TW * 32), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const Int4Weight& w = p.w;
-
-  // the rows of this block
-  int first = blockIdx.y * (8 * NT), count = p.M - first, expert = 0;
-  if constexpr (MODE != kDense) {
-    if (p.rows.chunks) {
-      if (static_cast<int>(blockIdx.y) >= *p.rows.n_chunks) return;
-      const int4 c = p.rows.chunks[blockIdx.y];
-      expert = c.x; first = c.y; count = c.z;
-    } else {
-      expert = p.rows.ids[blockIdx.y]; first = blockIdx.y; count = 1;
-      if (expert < 0 || expert >= p.rows.E) return;
-    }
-  }
-  const View v{w.packed + expert * w.expert_bytes() + lane * 16,
-               static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
-               ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
-  const int groups = (w.row_tiles() + R - 1) / R, k_tiles = w.k_tiles();
-  const int rg0 = static_cast<int>(static_cast<long long>(groups) * blockIdx.x / gridDim.x);
-  const int rg1 = static_cast<int>(static_cast<long long>(groups) * (blockIdx.x + 1) / gridDim.x);
-  const int rows_here = min(count, 8 * NT);
-
-  // the warp's sequence of blocks, and the next one to copy
-  const int blocks = (k_tiles + B - 1) / B;
-  const int mine = blocks > warp ? (blocks - warp + kWarps - 1) / kWarps : 0;
-  const int total = mine * (rg1 - rg0);
-  const uint32_t ring = smem_u32(smem) + warp * (SLOTS * BYTES);
+  float* red = reinterpret_cast<float*>(smem + WARPS * SLOTS * BYTES) + team * (TW * RED / 4);
+  unsigned char* xs = smem + WARPS * (SLOTS * BYTES + RED);
+  unsigned char* ring = smem + (team * TW + warp) * (SLOTS * BYTES);
   const uint32_t put = place(lane & 7, lane >> 3), get = place(g, t);
-  int l_rg = rg0, l_kt = warp * B, left = total;
-  auto fill = [&](uint32_t slot) {
-    if (left > 0) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const int tr = R == 1 ? l_rg : min(l_rg * R + i, w.row_tiles() - 1);
-        const uint8_t* src = v.packed + (static_cast<size_t>(tr) * k_tiles + l_kt) * 512;
-        if (l_kt + B <= k_tiles) {
-#pragma unroll
-          for (int b = 0; b < B; ++b) copy16(slot + put + (b * R + i) * 512, src + b * 512);
-        } else {
-#pragma unroll
-          for (int b = 0; b < B; ++b)
-            if (l_kt + b < k_tiles) copy16(slot + put + (b * R + i) * 512, src + b * 512);
-        }
-      }
-      --left;
-      l_kt += kWarps * B;
-      if (l_kt >= k_tiles) { l_kt = warp * B; ++l_rg; }
-    }
-    copy_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < SLOTS; ++i) fill(ring + i * BYTES);
+  const int groups = (w.row_tiles() + R - 1) / R, k_tiles = w.k_tiles(), pitch = k_tiles * 128 + 16;
+  const bool works = warp * B < k_tiles;                    // the warp has a block of a row group
 
-  // columns of the instruction beyond the rows read row 0 again: their results are not written
-  const T* xrow[NT];
+  const int chunks = MODE == kDense ? p.chunks : p.rows.chunks ? *p.rows.n_chunks : p.rows.slots;
+  const int per = max(1, static_cast<int>(gridDim.x) / max(1, chunks));    // blocks per chunk
+  const int part = blockIdx.x % per, stride = gridDim.x / per;
+  for (int chunk = blockIdx.x / per; chunk < chunks; chunk += stride) {
+    if (static_cast<int>(blockIdx.x) >= stride * per) break;               // (left over)
+    int first = chunk * (8 * NT), count = p.M - first, expert = 0;
+    if constexpr (MODE != kDense) {
+      if (p.rows.chunks) {
+        const int4 c = p.rows.chunks[chunk];
+        expert = c.x; first = c.y; count = c.z;
+      } else {
+        expert = p.rows.ids[chunk]; first = chunk; count = 1;
+        if (expert < 0 || expert >= p.rows.E) continue;
+      }
+    }
+    const View v{w.packed + expert * w.expert_bytes() + lane * 16,
+                 static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
+                 ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
+    const long long teams = static_cast<long long>(per) * TEAMS, me = static_cast<long long>(part) * TEAMS + team;
+    const int rg0 = static_cast<int>(groups * me / teams), rg1 = static_cast<int>(groups * (me + 1) / teams);
+    const int rows_here = min(count, 8 * NT);
+
+    // the warp's sequence of blocks, and the next one to copy
+    int l_rg = works ? rg0 : rg1, l_kt = warp * B;
+    auto fill = [&](unsigned char* to) {
+      const uint32_t slot = smem_u32(to);
+      if (l_rg < rg1) {
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    long long r = first + (j * 8 + g < rows_here ? j * 8 + g : 0);
-    if constexpr (MODE == kGated) r = (p.rows.row_slot ? p.rows.row_slot[r] : r) / p.rows.top_k;
-    xrow[j] = static_cast<const T*>(p.x) + r * w.K + t * 16;
-  }
-  auto load_x = [&](uint4 (&d)[NT][2], int step) {
+        for (int i = 0; i < R; ++i) {
+          const int tr = R == 1 ? l_rg : min(l_rg * R + i, w.row_tiles() - 1);
+          const uint8_t* src = v.packed + (static_cast<size_t>(tr) * k_tiles + l_kt) * 512;
+          if (l_kt + B <= k_tiles) {
+#pragma unroll
+            for (int b = 0; b < B; ++b) copy16(slot + put + (b * R + i) * 512, src + b * 512);
+          } else {
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+              if (l_kt + b < k_tiles) copy16(slot + put + (b * R + i) * 512, src + b * 512);
+          }
+        }
+        l_kt += TW * B;
+        if (l_kt >= k_tiles) { l_kt = warp * B; ++l_rg; }
+      }
+      copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) fill(ring + i * BYTES);
+
+    auto x_row = [&](int c) -> const T* {
+      long long r = first + c;
+      if constexpr (MODE == kGated) r = (p.rows.row_slot ? p.rows.row_slot[r] : r) / p.rows.top_k;
+      return static_cast<const T*>(p.x) + r * w.K;
+    };
+    // columns of the instruction beyond the rows read row 0 again: their results are not written
+    const T* xrow[NT];
+    const unsigned char* xat[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      d[j][0] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + step * 64));
-      d[j][1] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + step * 64) + 1);
+      const int c = j * 8 + g < rows_here ? j * 8 + g : 0;
+      if constexpr (XS) xat[j] = xs + c * pitch + t * 32;
+      else xrow[j] = x_row(c) + t * 16;
     }
-  };
-  float acc[R][NT][CH][4] = {};
-  Scales<ZEROS, R, B, SPAN> ahead;
-  int kt = warp * B, rg = 0;
-  uint32_t at = ring;
-  if (total > 0) load_scales<ZEROS, R, B, SPAN>(ahead, w, v, rg0 * R, kt, g, t);
-  for (int n = 0; n < total; ++n) {
-    const Scales<ZEROS, R, B, SPAN> sc = ahead;
-    int kt_next = kt + kWarps * B;
-    const bool last = kt_next >= k_tiles;                  // of the row group
-    if (last) kt_next = warp * B;
-    if (n + 1 < total) load_scales<ZEROS, R, B, SPAN>(ahead, w, v, (rg0 + rg + last) * R, kt_next, g, t);
-    if ((kt + B) * 64 <= w.K) {
-      uint4 x[2][NT][2];
-      load_x(x[0], kt);
-      copy_wait<SLOTS - 1>();
-      __syncwarp();
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        if (b + 1 < B) load_x(x[(b + 1) & 1], kt + b + 1);
-        multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, true, at + get + b * (R * 512), x[b & 1], acc);
+    Scales<ZEROS, R, B, SPAN> ahead;
+    if (works && rg0 < rg1) load_scales<ZEROS, R, B, SPAN>(ahead, w, v, rg0 * R, warp * B, g, t);
+    if constexpr (XS) {   // columns that fill up the last step are zero
+      for (int c = threadIdx.x / 32; c < rows_here; c += WARPS) {
+        const uint4* src = reinterpret_cast<const uint4*>(x_row(c));
+        for (int i = lane; i < k_tiles * 8; i += 32)
+          *reinterpret_cast<uint4*>(xs + c * pitch + i * 16) = i * 8 < w.K ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
       }
-    } else {   // the row ends inside the block
-      copy_wait<SLOTS - 1>();
-      __syncwarp();
+      __syncthreads();
+    }
+    auto load_x = [&](uint4 (&d)[NT][2], int step, bool in) {
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        if (kt + b < k_tiles) {
-          const bool in = (kt + b) * 64 + t * 16 < w.K;
-          uint4 x[NT][2];
-          if (in) load_x(x, kt + b);
-          else {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) x[j][0] = x[j][1] = make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (XS) {
+          d[j][0] = *reinterpret_cast<const uint4*>(xat[j] + step * 128);
+          d[j][1] = *reinterpret_cast<const uint4*>(xat[j] + step * 128 + 16);
+        } else {
+          d[j][0] = d[j][1] = make_uint4(0, 0, 0, 0);
+          if (in) {
+            d[j][0] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + step * 64));
+            d[j][1] = __ldg(reinterpret_cast<const uint4*>(xrow[j] + step * 64) + 1);
           }
-          multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, in, at + get + b * (R * 512), x, acc);
         }
       }
-    }
-    __syncwarp();                                          // the slot has been read
-    fill(at);
-    at = at == ring + (SLOTS - 1) * BYTES ? ring : at + BYTES;
-    kt = kt_next;
-    if (last) {
-      float* out = red + (rg * kWarps + warp) * (VALUES * 32) + lane;
+    };
+    // a value of a row group's sums, by its place in the lane's accumulators
+    auto write = [&](int rg, int q, float sum) {
+      const int c = q & 3, j = (q >> 2) % NT, i = (q >> 2) / NT;
+      const int n = (rg * R + i) * 16 + g + (c >> 1) * 8;      // weight row
+      const int col = j * 8 + t * 2 + (c & 1);                 // row of the chunk
+      if constexpr (MODE == kGated) {
+        const float other = __shfl_xor_sync(0xffffffffu, sum, 4);          // rows 2i and 2i + 1 are four lanes apart
+        if ((g & 1) == 0 && n + 1 < w.N && col < rows_here)
+          static_cast<T*>(p.y)[(static_cast<long long>(first) + col) * (w.N / 2) + n / 2] = I::from_float(silu_mul(sum, other));
+      } else if (n < w.N && col < rows_here) {
+        const long long row = first + col;
+        if constexpr (MODE == kDense) static_cast<T*>(p.y)[row * w.N + n] = I::from_float(sum);
+        else static_cast<float*>(p.y)[static_cast<long long>(p.rows.row_slot[row]) * w.N + n] = sum;
+      }
+    };
+    float acc[R][NT][CH][4] = {};
+    unsigned char* at = ring;
+    for (int rg = rg0; rg < rg1; ++rg) {
+      for (int kt = warp * B; kt < k_tiles; kt += TW * B) {
+        const Scales<ZEROS, R, B, SPAN> sc = ahead;
+        const bool last = kt + TW * B >= k_tiles;              // of the row group
+        if (!last || rg + 1 < rg1)
+          load_scales<ZEROS, R, B, SPAN>(ahead, w, v, (rg + last) * R, last ? warp * B : kt + TW * B, g, t);
+        if ((kt + B) * 64 <= w.K) {
+          uint4 x[2][NT][2];
+          if constexpr (!XS) load_x(x[0], kt, true);
+          copy_wait<SLOTS - 1>();
+          __syncwarp();
+          if constexpr (XS) load_x(x[0], kt, true);
 #pragma unroll
-      for (int a = 0; a < R; ++a)
-#pragma unroll
-        for (int b = 0; b < NT; ++b)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            out[((a * NT + b) * 4 + c) * 32] = CH == 2 ? acc[a][b][0][c] + acc[a][b][CH - 1][c] : acc[a][b][0][c];
-#pragma unroll
-            for (int d = 0; d < CH; ++d) acc[a][b][d][c] = 0.f;
+          for (int b = 0; b < B; ++b) {
+            if (b + 1 < B) load_x(x[(b + 1) & 1], kt + b + 1, true);
+            multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, true, at + get + b * (R * 512), x[b & 1], acc);
           }
-      ++rg;
+        } else {   // the row ends inside the block
+          copy_wait<SLOTS - 1>();
+          __syncwarp();
+#pragma unroll
+          for (int b = 0; b < B; ++b) {
+            if (kt + b < k_tiles) {
+              const bool in = (kt + b) * 64 + t * 16 < w.K;
+              uint4 x[NT][2];
+              load_x(x, kt + b, in);
+              multiply<BF16, ZEROS, NT, R, B, SPAN, CH>(sc, b, in, at + get + b * (R * 512), x, acc);
+            }
+          }
+        }
+        __syncwarp();                                          // the slot has been read
+        fill(at);
+        at = at == ring + (SLOTS - 1) * BYTES ? ring : at + BYTES;
+      }
+      const int n_red = (rg - rg0) % RGF;
+      if (works) {
+        float* out = red + (n_red * TW + warp) * (VALUES * 32) + lane;
+#pragma unroll
+        for (int a = 0; a < R; ++a)
+#pragma unroll
+          for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float sum = CH == 2 ? acc[a][b][0][c] + acc[a][b][CH - 1][c] : acc[a][b][0][c];
+              if constexpr (TW == 1) write(rg, (a * NT + b) * 4 + c, sum);
+              else out[((a * NT + b) * 4 + c) * 32] = sum;
+#pragma unroll
+              for (int d = 0; d < CH; ++d) acc[a][b][d][c] = 0.f;
+            }
+      }
+      if constexpr (TW > 1) {
+        if (n_red + 1 < RGF && rg + 1 < rg1) continue;
+        asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TW * 32) : "memory");
+        const int with_work = min(TW, (k_tiles + B - 1) / B);   // warps that had a block at all
+        for (int u = warp; u < (n_red + 1) * VALUES; u += TW) {
+          const int r = u / VALUES, q = u % VALUES;
+          float sum = 0.f;
+          for (int k = 0; k < with_work; ++k) sum += red[((r * TW + k) * VALUES + q) * 32 + lane];
+          write(rg - n_red + r, q, sum);
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TW * 32) : "memory");
+      }
     }
-  }
-  __syncthreads();
-  const int with_work = min(kWarps, blocks);   // warps that had a block at all
-  for (int u = warp; u < (rg1 - rg0) * VALUES; u += kWarps) {
-    const int r = u / VALUES, q = u % VALUES;
-    float sum = 0.f;
-    for (int k = 0; k < with_work; ++k) sum += red[((r * kWarps + k) * VALUES + q) * 32 + lane];
-    const int c = q & 3, j = (q >> 2) % NT, i = (q >> 2) / NT;
-    const int n = ((rg0 + r) * R + i) * 16 + g + (c >> 1) * 8;    // weight row
-    const int col = j * 8 + t * 2 + (c & 1);                       // row of the batch
-    if constexpr (MODE == kGated) {
-      const float other = __shfl_xor_sync(0xffffffffu, sum, 4);    // rows 2i and 2i + 1 are four lanes apart
-      if ((g & 1) == 0 && n + 1 < w.N && col < rows_here)
-        static_cast<T*>(p.y)[(static_cast<long long>(first) + col) * (w.N / 2) + n / 2] = I::from_float(silu_mul(sum, other));
-    } else if (n < w.N && col < rows_here) {
-      const long long row = first + col;
-      if constexpr (MODE == kDense) static_cast<T*>(p.y)[row * w.N + n] = I::from_float(sum);
-      else static_cast<float*>(p.y)[static_cast<long long>(p.rows.row_slot[row]) * w.N + n] = sum;
-    }
+    if constexpr (XS) __syncthreads();                          // the rows of X may be overwritten
   }
 }
 
@@ -305,9 +345,10 @@ int4_small_down_direct_kernel(const SmallParams p) {
     const int e = ids[unit / blocks];
     return e < 0 || e >= p.rows.E;
   };
-  const uint32_t ring = smem_u32(rings[warp]);
+  unsigned char* ring = &rings[warp][0][0];
   const uint32_t put = place(lane & 7, lane >> 3), get = place(g, t);
-  auto fill = [&](uint32_t slot) {
+  auto fill = [&](unsigned char* to) {
+    const uint32_t slot = smem_u32(to);
     while (ahead < end && dropped(ahead)) ++ahead;
     if (ahead < end) {
       const int kt = (ahead % blocks) * B;
@@ -322,7 +363,7 @@ int4_small_down_direct_kernel(const SmallParams p) {
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) fill(ring + i * (B * 512));
   float lo = 0.f, hi = 0.f;
-  uint32_t at = ring;
+  unsigned char* at = ring;
   for (; u < end; ++u) {
     if (dropped(u)) continue;
     const int j = u / blocks, slot = token * p.rows.top_k + j, expert = ids[j], kt = (u % blocks) * B;
@@ -371,36 +412,60 @@ int sm_count() {
   return sms > 0 ? sms : 148;
 }
 
-// MAX_GROUPS: row groups whose sums a block has room for in shared memory
-template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int SLOTS, int MIN_BLOCKS, int MAX_GROUPS>
-int launch_one(const SmallParams& p, int blocks_y, cudaStream_t s) {
-  auto kernel = int4_small_kernel<BF16, ZEROS, MODE, NT, R, B, SPAN, SLOTS, MIN_BLOCKS>;
-  const int groups = (p.w.row_tiles() + R - 1) / R;
-  // as many blocks as run at once, if that leaves them no more row groups than they have room for; else whole rounds of them
-  const int slots = max(1, sm_count() * MIN_BLOCKS / blocks_y);
-  const int rounds = (groups + slots * MAX_GROUPS - 1) / (slots * MAX_GROUPS);
-  const int blocks = static_cast<int>(min(static_cast<long long>(groups), static_cast<long long>(slots) * rounds));
-  const int per_block = (groups + blocks - 1) / blocks;
-  const size_t smem = kWarps * SLOTS * R * B * 512 + static_cast<size_t>(per_block) * kWarps * R * NT * 4 * 32 * sizeof(float);
+template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int SLOTS, int WARPS, int TW, int MIN_BLOCKS, int RGF, bool XS>
+int launch_one(const SmallParams& p, int rows, cudaStream_t s) {
+  auto kernel = int4_small_kernel<BF16, ZEROS, MODE, NT, R, B, SPAN, SLOTS, WARPS, TW, MIN_BLOCKS, RGF, XS>;
+  const long long groups = (p.w.row_tiles() + R - 1) / R;
+  const size_t smem = WARPS * (SLOTS * R * B * 512 + (TW == 1 ? 0 : RGF * R * NT * 4 * 128)) + (XS ? static_cast<size_t>(rows) * (p.w.k_tiles() * 128 + 16) : 0);
+  if (smem > kSmallSmem) return VQG_ERR_UNSUPPORTED;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return VQG_ERR_LAUNCH;
-  kernel<<<dim3(blocks, blocks_y), kWarps * 32, smem, s>>>(p);
+  // as many blocks as run at once, or one per row group where there are fewer of those
+  const long long slots = static_cast<long long>(sm_count()) * MIN_BLOCKS;
+  const int blocks = static_cast<int>(min(slots, groups * p.chunks));
+  kernel<<<blocks, WARPS * 32, smem, s>>>(p);
   count_launch();
   return cuda_status(cudaGetLastError());
 }
 
+// rows: of a chunk, at most; p.chunks: how many chunks there are, at most
 template <int MODE>
-int launch_rows(const SmallParams& p, int rows, int blocks_y, bool bf16, cudaStream_t s) {
-  auto go = [&](auto type, auto zeros) {
-    constexpr bool B = decltype(type)::value, Z = decltype(zeros)::value;
-    const bool pairs = p.w.group % 128 == 0;
-    if (rows <= 8) {
-      if (p.w.K < 64 * 4 * kWarps) return launch_one<B, Z, MODE, 1, 1, 2, 1, 4, 3, 8>(p, blocks_y, s);
-      return pairs ? launch_one<B, Z, MODE, 1, 1, 4, 2, 3, 3, 8>(p, blocks_y, s) : launch_one<B, Z, MODE, 1, 1, 4, 1, 3, 3, 8>(p, blocks_y, s);
+int launch_rows(const SmallParams& p, int rows, bool bf16, cudaStream_t s) {
+  auto go = [&](auto type, auto zeros) -> int {
+    constexpr bool F = decltype(type)::value, Z = decltype(zeros)::value;
+    const size_t x = static_cast<size_t>(rows) * (p.w.k_tiles() * 128 + 16);
+    if constexpr (MODE == kDense) {
+      if (rows <= 8) {
+        const bool pairs = p.w.group % 128 == 0;
+        // one block of 24 warps per SM: X once per SM
+        if (p.w.K >= 64 * 4 * 8 && x + 24 * (2 * 2048 + 1024) <= kSmallSmem)
+          return pairs ? launch_one<F, Z, MODE, 1, 1, 4, 2, 2, 24, 8, 1, 2, true>(p, rows, s)
+                       : launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 24, 8, 1, 2, true>(p, rows, s);
+        if (x <= 32 * 1024) return launch_one<F, Z, MODE, 1, 1, 2, 1, 3, 8, 8, 3, 2, true>(p, rows, s);
+        return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 8, 3, 2, false>(p, rows, s);
+      }
+      if (rows <= 16) {
+        if (x + 16 * (2 * 2048 + 2048) <= kSmallSmem) return launch_one<F, Z, MODE, 2, 2, 2, 1, 2, 16, 8, 1, 1, true>(p, rows, s);
+        return launch_one<F, Z, MODE, 2, 2, 2, 1, 3, 8, 8, 2, 1, false>(p, rows, s);
+      }
+      return launch_one<F, Z, MODE, 4, 2, 2, 1, 2, 8, 8, 2, 1, false>(p, rows, s);
+    } else {
+      // Experts: short rows (a warp alone takes them whole) and many row groups, unless there are few slots.
+      if (!p.rows.chunks) {
+        if (x <= 32 * 1024) return launch_one<F, Z, MODE, 1, 1, 2, 1, 3, 8, 4, 3, 2, true>(p, rows, s);
+        return launch_one<F, Z, MODE, 1, 1, 2, 1, 3, 8, 4, 3, 2, false>(p, rows, s);
+      }
+      if (rows <= 8) {
+        if (x <= 40 * 1024) return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 2, 3, 2, true>(p, rows, s);
+        return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 2, 3, 2, false>(p, rows, s);
+      }
+      if (rows <= 16) {
+        if (x <= 70 * 1024) return launch_one<F, Z, MODE, 2, 1, 4, 1, 2, 8, 2, 2, 1, true>(p, rows, s);
+        return launch_one<F, Z, MODE, 2, 1, 4, 1, 2, 8, 2, 2, 1, false>(p, rows, s);
+      }
+      return launch_one<F, Z, MODE, 4, 1, 4, 1, 2, 8, 2, 2, 1, false>(p, rows, s);
     }
-    if (rows <= 16) return launch_one<B, Z, MODE, 2, 2, 2, 1, 3, 2, 4>(p, blocks_y, s);
-    return launch_one<B, Z, MODE, 4, 2, 2, 1, 3, 2, 2>(p, blocks_y, s);
   };
   if (p.w.zeros) return bf16 ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
   return bf16 ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});
@@ -411,24 +476,25 @@ int launch_rows(const SmallParams& p, int rows, int blocks_y, bool bf16, cudaStr
 int launch_int4_small(const Int4Weight& w, const void* x, void* y, int M, bool bf16, cudaStream_t s) {
   SmallParams p{};
   p.w = w; p.x = x; p.y = y; p.M = M;
-  const int rows = M < kInt4SmallRows ? M : kInt4SmallRows, chunks = (M + rows - 1) / rows;
-  if (chunks > 65535) return VQG_ERR_UNSUPPORTED;
-  return launch_rows<kDense>(p, rows, chunks, bf16, s);
+  const int rows = M <= 8 ? 8 : M <= 16 ? 16 : kInt4SmallRows;
+  p.chunks = (M + rows - 1) / rows;
+  return launch_rows<kDense>(p, M < rows ? M : rows, bf16, s);
 }
 
 int launch_int4_small_gated(const Int4Weight& w, const void* x, void* h, const ExpertRows& rows, int chunk_rows, int max_chunks,
                             bool bf16, cudaStream_t s) {
   SmallParams p{};
   p.w = w; p.x = x; p.y = h; p.rows = rows;
-  if (!rows.chunks) return launch_rows<kGated>(p, 1, rows.slots, bf16, s);
-  return launch_rows<kGated>(p, chunk_rows, max_chunks, bf16, s);
+  p.chunks = rows.chunks ? max_chunks : rows.slots;
+  return launch_rows<kGated>(p, rows.chunks ? chunk_rows : 1, bf16, s);
 }
 
 int launch_int4_small_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int chunk_rows, int max_chunks,
                            bool bf16, cudaStream_t s) {
   SmallParams p{};
   p.w = w; p.x = h; p.y = part; p.rows = rows;
-  return launch_rows<kDown>(p, chunk_rows, max_chunks, bf16, s);
+  p.chunks = max_chunks;
+  return launch_rows<kDown>(p, chunk_rows, bf16, s);
 }
 
 int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, const ExpertRows& rows, int tokens, bool bf16,
