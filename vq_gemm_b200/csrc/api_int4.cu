@@ -1,7 +1,23 @@
 // extern "C" entry points of the 4-bit products, their quantiser and the experts' layer: argument checks, routes, scratch.
+#include <atomic>
+
 #include "int4.cuh"
 
 using namespace vqg;
+
+namespace vqg {
+int sm_count_cached() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+}  // namespace vqg
 
 namespace {
 

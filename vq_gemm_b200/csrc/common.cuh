@@ -58,6 +58,7 @@ int* device_status_ptr();          // device address of the status word of the c
 cudaError_t ensure_status_word();  // looks its address up on first use (per device); allocates nothing
 
 void count_launch(int n = 1);
+int sm_count_cached();             // multiprocessors of the current device, asked once per device
 
 // Weights written by this library on a stream (the quantiser, the index packer): the small-batch kernels read
 // indices and codebooks BEFORE they wait for the kernel ahead of them when launched with programmatic stream

@@ -201,17 +201,11 @@ int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed,
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms > 0 ? sms : 148;
-}
-
 }  // namespace
 
 int launch_int4_dequant(const Int4Weight& w, void* out, int experts, bool bf16, cudaStream_t s) {
   const long long tiles = static_cast<long long>(w.row_tiles()) * w.k_tiles();
-  const long long want = (tiles + kThreads / 32 - 1) / (kThreads / 32), most = 8LL * sm_count();
+  const long long want = (tiles + kThreads / 32 - 1) / (kThreads / 32), most = 8LL * sm_count_cached();
   const dim3 grid(static_cast<unsigned>(want < most ? want : most), experts);
   const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0;   // rows are multiples of 64 bytes
   if (bf16) int4_dequant_kernel<true><<<grid, kThreads, 0, s>>>(w, out, wide);

@@ -17,6 +17,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace vqg {
@@ -85,6 +87,22 @@ int launch_expert_combine(const float* part, const ExpertRows& rows, void* y, in
 // K up to which 16-column runs are divided by groups with one multiplication: n / d = n * ceil(2^32 / d) >> 32 is exact while
 // n * d < 2^32, n and d at most K / 16.
 constexpr int kInt4MaxK = 1 << 19;
+
+// Opt-in to large dynamic shared memory, once per kernel and device (a static one per launcher instance): the call to the runtime
+// costs a good part of a small launch.
+struct SmemOptIn {
+  std::atomic<unsigned long long> done{0};
+  template <typename Kernel>
+  bool ask(Kernel kernel) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return false;
+    const unsigned long long bit = dev < 64 ? 1ULL << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+  }
+};
 
 #ifdef __CUDACC__
 // group of columns k ... k + 15 (k a multiple of 16)

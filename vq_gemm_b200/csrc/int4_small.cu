@@ -406,23 +406,16 @@ int4_small_down_direct_kernel(const SmallParams p) {
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms > 0 ? sms : 148;
-}
-
 template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int SLOTS, int WARPS, int TW, int MIN_BLOCKS, int RGF, bool XS>
 int launch_one(const SmallParams& p, int rows, cudaStream_t s) {
   auto kernel = int4_small_kernel<BF16, ZEROS, MODE, NT, R, B, SPAN, SLOTS, WARPS, TW, MIN_BLOCKS, RGF, XS>;
   const long long groups = (p.w.row_tiles() + R - 1) / R;
   const size_t smem = WARPS * (SLOTS * R * B * 512 + (TW == 1 ? 0 : RGF * R * NT * 4 * 128)) + (XS ? static_cast<size_t>(rows) * (p.w.k_tiles() * 128 + 16) : 0);
   if (smem > kSmallSmem) return VQG_ERR_UNSUPPORTED;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
-    return VQG_ERR_LAUNCH;
+  static SmemOptIn opt_in;
+  if (smem > 48 * 1024 && !opt_in.ask(kernel)) return VQG_ERR_LAUNCH;
   // as many blocks as run at once, or one per row group where there are fewer of those
-  const long long slots = static_cast<long long>(sm_count()) * MIN_BLOCKS;
+  const long long slots = static_cast<long long>(sm_count_cached()) * MIN_BLOCKS;
   const int blocks = static_cast<int>(min(slots, groups * p.chunks));
   kernel<<<blocks, WARPS * 32, smem, s>>>(p);
   count_launch();

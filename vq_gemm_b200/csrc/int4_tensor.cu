@@ -673,20 +673,17 @@ bool make_x_map(CUtensorMap* map, const void* ptr, int rows, int cols, int box_r
             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-int sm_pairs() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms > 1 ? sms / 2 : 74;
-}
+int sm_pairs() { return max(1, sm_count_cached() / 2); }
 constexpr size_t kPairPartialBytes = 2 * 2 * static_cast<size_t>(BM) * BNH * sizeof(float);
 
-template <typename Kernel>
-int launch(Kernel kernel, int pairs, const void* x, int rows, bool bf16, const TensorParams& p, cudaStream_t s) {
-  constexpr int smem = kSmem + 1024;
+template <bool BF16, int MODE>
+int launch(int pairs, const void* x, int rows, const TensorParams& p, cudaStream_t s) {
+  static SmemOptIn opt_in;
+  auto kernel = int4_tensor_kernel<BF16, MODE>;
   CUtensorMap map, map32;
-  if (!make_x_map(&map, x, rows, p.w.K, 128, bf16) || !make_x_map(&map32, x, rows, p.w.K, 32, bf16)) return VQG_ERR_LAUNCH;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return VQG_ERR_LAUNCH;
-  kernel<<<2 * pairs, kThreads, smem, s>>>(map, map32, p);
+  if (!make_x_map(&map, x, rows, p.w.K, 128, BF16) || !make_x_map(&map32, x, rows, p.w.K, 32, BF16) || !opt_in.ask(kernel))
+    return VQG_ERR_LAUNCH;
+  kernel<<<2 * pairs, kThreads, kSmem + 1024, s>>>(map, map32, p);
   count_launch();
   return cuda_status(cudaGetLastError());
 }
@@ -716,8 +713,7 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   p.q = static_cast<int>(units / pairs);
   p.r = static_cast<int>(units % pairs);
   p.ws_partial = split ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes) : nullptr;
-  const int st = bf16 ? launch(int4_tensor_kernel<true, kDense>, pairs, x, M, true, p, s)
-                      : launch(int4_tensor_kernel<false, kDense>, pairs, x, M, false, p, s);
+  const int st = bf16 ? launch<true, kDense>(pairs, x, M, p, s) : launch<false, kDense>(pairs, x, M, p, s);
   if (st != VQG_OK || !split || pairs == 1) return st;
   // enqueued so that it can take its place on the SMs as the first kernel leaves them; it waits for that one to complete
   cudaLaunchConfig_t cfg{};
@@ -744,8 +740,8 @@ int launch_experts(const Int4Weight& w, const void* x, void* y, const ExpertRows
   const long long most = static_cast<long long>(max_chunks) * p.n_tiles;
   if (most > 0x7fffffffLL) return VQG_ERR_UNSUPPORTED;
   const int pairs = most < sm_pairs() ? static_cast<int>(most) : sm_pairs();
-  if (gated) return bf16 ? launch(int4_tensor_kernel<true, kGated>, pairs, x, rows.slots, true, p, s) : launch(int4_tensor_kernel<false, kGated>, pairs, x, rows.slots, false, p, s);
-  return bf16 ? launch(int4_tensor_kernel<true, kDown>, pairs, x, rows.slots, true, p, s) : launch(int4_tensor_kernel<false, kDown>, pairs, x, rows.slots, false, p, s);
+  if (gated) return bf16 ? launch<true, kGated>(pairs, x, rows.slots, p, s) : launch<false, kGated>(pairs, x, rows.slots, p, s);
+  return bf16 ? launch<true, kDown>(pairs, x, rows.slots, p, s) : launch<false, kDown>(pairs, x, rows.slots, p, s);
 }
 }  // namespace
 

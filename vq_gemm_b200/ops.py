@@ -71,14 +71,6 @@ def _stream_ptr(dev) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _launch(dev: torch.device, fn, *args) -> int:
-    """fn(*args, stream) with ``dev`` current; entering a device that is current already costs microseconds."""
-    if torch._C._cuda_getDevice() == dev.index:
-        return fn(*args, _stream_ptr(dev))
-    with torch.cuda.device(dev):
-        return fn(*args, _stream_ptr(dev))
-
-
 def auto_path(M: int, N: int, K: int, v: int, C: int, index_bits: int = 8, rows_per_codebook: int = 0, layout: str = "bl") -> str:
     """Name of the kernel route the library picks by itself for a problem (``vqg_auto_path``)."""
     ib = {8: 1, 16: 2, 12: _lib.IDX_PACKED12}[index_bits]
@@ -345,53 +337,41 @@ def _int4_weight(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[tor
     return N, group
 
 
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+_host_module = None
+_INT4_FEW_ROWS = 32          # rows up to which vqg_int4_gemm needs no scratch (vqg_int4_workspace_bytes is 0)
+
+
+def _host(tensor: torch.Tensor):
+    """The native host layer (csrc/host.cpp), which checks, allocates and launches; for tensors on a GPU."""
+    if not tensor.is_cuda:
+        raise RuntimeError("vq_gemm_b200 has no CPU path: all tensors must be CUDA tensors")
+    global _host_module
+    if _host_module is None:
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise RuntimeError("vq_gemm_b200/_host.so is missing or does not load: build it with "
+                               f"`python compile_kernels.py build_ext --inplace`. There is no fallback path. ({e})") from None
+        _host_module = module
+    return _host_module
 
 
 def int4_gemm(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Y[M, N] = X[M, K] @ W^T for a 4-bit weight with group scales (``quantize.int4_quantize``), fp32 accumulation.
     x, scales and Y are of one type, float16 or bfloat16; group = K // scales.shape[0]."""
-    lib = _lib.load()
-    dev = _require_cuda(x, packed, scales, *(() if zeros is None else (zeros,)))
-    if x.dim() != 2 or x.dtype != scales.dtype:
-        raise RuntimeError("x must be [M, K] and of the type of scales")
-    M, K = x.shape
-    N, group = _int4_weight(packed, scales, zeros, K, False)
-    if out is None:
-        out = x.new_empty((M, N))
-    elif tuple(out.shape) != (M, N) or out.dtype != x.dtype or not out.is_contiguous() or out.device != dev:
-        raise RuntimeError("out must be a contiguous [M, N] tensor of x's type on the inputs' device")
-    ws = _ws(dev, lib.vqg_int4_workspace_bytes(M, N, K))
-    st = _launch(dev, lib.vqg_int4_gemm, x.data_ptr(), packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), M, N, K,
-                 group, _INT4_TYPES[x.dtype], _ptr(ws), 0 if ws is None else ws.numel())
-    _lib.check(st, "int4_gemm")
-    return out
+    host = _host(x)
+    ws = None
+    if x.dim() == 2 and x.shape[0] > _INT4_FEW_ROWS:
+        ws = _ws(x.device, _lib.load().vqg_int4_workspace_bytes(x.shape[0], scales.shape[-1], x.shape[1]))
+    return host.int4_gemm(x, packed, scales, zeros, out, ws)
 
 
 def int4_dequant(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
                  in_features: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The dense [N, K] (or [E, N, K]) weights that the 4-bit products multiply, bit for bit.  ``in_features`` is K
     where it is not a multiple of 64."""
-    lib = _lib.load()
-    dev = _require_cuda(packed, scales, *(() if zeros is None else (zeros,)))
-    experts = packed.dim() == 4
-    K = packed.shape[-2] * 64 if in_features is None else int(in_features)
-    N, group = _int4_weight(packed, scales, zeros, K, experts)
-    E = packed.shape[0] if experts else 1
-    shape = (E, N, K) if experts else (N, K)
-    if out is None:
-        out = torch.empty(shape, dtype=scales.dtype, device=dev)
-    elif tuple(out.shape) != shape or out.dtype != scales.dtype or out.device != dev or not out.is_contiguous():
-        raise RuntimeError(f"out must be a contiguous tensor of shape {shape} and of the type of scales on {dev}")
-    st = _launch(dev, lib.vqg_int4_dequant, packed.data_ptr(), scales.data_ptr(), _ptr(zeros), out.data_ptr(), E, N, K, group,
-                 _INT4_TYPES[scales.dtype])
-    _lib.check(st, "int4_dequant")
-    return out
-
-
-_LOGIT_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+    return _host(packed).int4_dequant(packed, scales, zeros, -1 if in_features is None else in_features, out)
 
 
 def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,
@@ -404,24 +384,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     ``group_score="max"`` its largest); weights are p of the chosen, divided by their sum with ``renormalize``, times
     ``scale``.  In falling order of choice, equal ones to the lower index.  Experts with a logit of -inf or NaN are
     never chosen; a slot for which none is left has expert -1 and weight 0."""
-    lib = _lib.load()
-    dev = _require_cuda(logits, *(() if bias is None else (bias,)))
-    if logits.dim() != 2 or logits.dtype not in _LOGIT_TYPES:
-        raise RuntimeError("logits must be [T, E], float16, bfloat16 or float32")
-    T, E = logits.shape
-    if scoring not in ("softmax", "sigmoid") or group_score not in ("top2", "max"):
-        raise RuntimeError("scoring must be softmax or sigmoid, group_score top2 or max")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
-        raise RuntimeError("bias must be a float32 [E] tensor")
-    top_groups = groups if top_groups is None else top_groups
-    if E < 1 or not 1 <= top_k <= E or groups < 1 or E % groups or not 1 <= top_groups <= groups:
-        raise RuntimeError(f"cannot choose {top_k} of {E} experts in {top_groups} of {groups} groups")
-    weights = logits.new_empty((T, top_k), dtype=torch.float32)
-    experts = logits.new_empty((T, top_k), dtype=torch.int32)
-    st = _launch(dev, lib.vqg_route_experts, logits.data_ptr(), _ptr(bias), weights.data_ptr(), experts.data_ptr(), T, E, top_k,
-                 scoring == "sigmoid", groups, top_groups, group_score == "max", renormalize, scale, _LOGIT_TYPES[logits.dtype])
-    _lib.check(st, "route_experts")
-    return weights, experts
+    return _host(logits).route_experts(logits, top_k, scoring, bias, groups, top_groups, group_score, renormalize, scale)
 
 
 def int4_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, gate_up: Sequence[Optional[torch.Tensor]],
@@ -431,34 +394,7 @@ def int4_experts(x: torch.Tensor, experts: torch.Tensor, weights: torch.Tensor, 
     ``gate_up`` and ``down`` are (packed, scales, zeros or None) of 4-bit weights [E, 2 * inner, hidden] (row pairs as
     :func:`interleave_gate_up` makes them) and [E, hidden, inner]; ``experts`` [T, top_k] int32 and ``weights`` [T, top_k]
     float32 as :func:`route_experts` gives them.  Slots with an expert outside 0 ... E-1 add nothing."""
-    lib = _lib.load()
-    up_p, up_s, up_z = gate_up
-    dn_p, dn_s, dn_z = down
-    dev = _require_cuda(x, experts, weights, *(t for t in (up_p, up_s, up_z, dn_p, dn_s, dn_z) if t is not None))
-    if x.dim() != 2 or x.dtype != up_s.dtype or x.dtype != dn_s.dtype:
-        raise RuntimeError("x must be [T, hidden] and of the type of both weights' scales")
-    T, hidden = x.shape
-    if experts.dim() != 2 or experts.shape[0] != T or experts.dtype != torch.int32 or experts.shape[1] < 1:
-        raise RuntimeError("experts must be an int32 [T, top_k] tensor")
-    if weights.shape != experts.shape or weights.dtype != torch.float32:
-        raise RuntimeError("weights must be a float32 tensor of the shape of experts")
-    rows, up_group = _int4_weight(up_p, up_s, up_z, hidden, True)
-    if rows % 2 or rows < 2:
-        raise RuntimeError("gate_up needs an even number of rows (gate, up pairs)")
-    inner, E, top_k = rows // 2, up_p.shape[0], experts.shape[1]
-    dn_rows, down_group = _int4_weight(dn_p, dn_s, dn_z, inner, True)
-    if dn_rows != hidden or dn_p.shape[0] != E:
-        raise RuntimeError(f"down must be [{E}, {hidden}, {inner}] to follow gate_up")
-    if out is None:
-        out = x.new_empty((T, hidden))
-    elif tuple(out.shape) != (T, hidden) or out.dtype != x.dtype or not out.is_contiguous() or out.device != dev:
-        raise RuntimeError("out must be a contiguous [T, hidden] tensor of x's type on the inputs' device")
-    ws = torch.empty(lib.vqg_int4_experts_workspace_bytes(T, top_k, E, hidden, inner), dtype=torch.uint8, device=dev)
-    st = _launch(dev, lib.vqg_int4_experts, x.data_ptr(), experts.data_ptr(), weights.data_ptr(), up_p.data_ptr(),
-                 up_s.data_ptr(), _ptr(up_z), dn_p.data_ptr(), dn_s.data_ptr(), _ptr(dn_z), out.data_ptr(), T, top_k, E, hidden,
-                 inner, up_group, down_group, _INT4_TYPES[x.dtype], ws.data_ptr(), ws.numel())
-    _lib.check(st, "int4_experts")
-    return out
+    return _host(x).int4_experts(x, experts, weights, *gate_up, *down, out)
 
 
 def device_status() -> int:

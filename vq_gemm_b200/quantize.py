@@ -21,7 +21,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .ops import _idx_bytes, _launch, _ptr, _require_cuda, _stream_ptr
+from .ops import _host, _idx_bytes, _require_cuda, _stream_ptr
 
 
 def _shape(weight: torch.Tensor, codebook: torch.Tensor, rows_per_codebook: int):
@@ -165,22 +165,7 @@ def int4_quantize(weight: torch.Tensor, *, group: int = 128, symmetric: bool = T
 
     ``group`` consecutive columns share a scale: 32, a multiple of 64, or 0 for the whole row.  Symmetric: scale =
     max|w| / 7, no zero points (``zeros`` is None); else scale = range / 15 and a zero point per group."""
-    lib = _lib.load()
-    dev = _require_cuda(weight)
-    if weight.dim() not in (2, 3) or weight.dtype not in (torch.float16, torch.bfloat16):
-        raise RuntimeError("weight must be a float16 or bfloat16 [N, K] or [E, N, K] tensor")
-    lead = tuple(weight.shape[:-2])
-    N, K = weight.shape[-2:]
-    group = K if group == 0 else group
-    if N < 1 or K < 1 or K % 32 or group < 1 or K % group or not (group == 32 or group % 64 == 0 or group == K):
-        raise RuntimeError(f"K={K} in groups of {group}: K must be a multiple of 32 and a group 32, a multiple of 64, or K")
-    packed = torch.empty(lead + (-(-N // 16), -(-K // 64), 512), dtype=torch.uint8, device=dev)
-    scales = torch.empty(lead + (K // group, N), dtype=weight.dtype, device=dev)
-    zeros = None if symmetric else torch.empty(lead + (K // group, N), dtype=torch.uint8, device=dev)
-    st = _launch(dev, lib.vqg_int4_quantize, weight.data_ptr(), packed.data_ptr(), scales.data_ptr(), _ptr(zeros),
-                 lead[0] if lead else 1, N, K, group, weight.dtype == torch.bfloat16)
-    _lib.check(st, "quantize.int4_quantize")
-    return packed, scales, zeros
+    return _host(weight).int4_quantize(weight, group, symmetric)
 
 
 def int4_pack(codes: torch.Tensor) -> torch.Tensor:
