@@ -56,6 +56,8 @@ int4_dequant_kernel(const Int4Weight w, void* __restrict__ out, bool wide) {
   using I = Int4Type<BF16>;
   const int lane = threadIdx.x & 31, g = lane & 7, t = lane >> 3;
   const long long tiles = static_cast<long long>(w.row_tiles()) * w.k_tiles();
+  grid_release();
+  grid_wait();
   const int e = blockIdx.y;
   const uint8_t* packed = w.packed + e * w.expert_bytes();
   const uint8_t* zeros = w.zeros ? w.zeros + e * w.expert_scales() : nullptr;
@@ -106,6 +108,8 @@ int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed,
   const int row_tiles = (N + 15) / 16, k_tiles = (K + 63) / 64, spans = (k_tiles + span - 1) / span;
   const long long unit = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   if (unit >= static_cast<long long>(row_tiles) * spans) return;
+  grid_release();
+  grid_wait();
   const int tr = static_cast<int>(unit / spans), kt0 = static_cast<int>(unit % spans) * span;
   const int kt1 = min(kt0 + span, k_tiles);
   const int e = blockIdx.y;
@@ -208,10 +212,8 @@ int launch_int4_dequant(const Int4Weight& w, void* out, int experts, bool bf16, 
   const long long want = (tiles + kThreads / 32 - 1) / (kThreads / 32), most = 8LL * sm_count_cached();
   const dim3 grid(static_cast<unsigned>(want < most ? want : most), experts);
   const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0;   // rows are multiples of 64 bytes
-  if (bf16) int4_dequant_kernel<true><<<grid, kThreads, 0, s>>>(w, out, wide);
-  else int4_dequant_kernel<false><<<grid, kThreads, 0, s>>>(w, out, wide);
-  count_launch();
-  return cuda_status(cudaGetLastError());
+  return cuda_status(bf16 ? launch_ahead(int4_dequant_kernel<true>, grid, kThreads, 0, s, false, w, out, wide)
+                          : launch_ahead(int4_dequant_kernel<false>, grid, kThreads, 0, s, false, w, out, wide));
 }
 
 int launch_int4_quantize(const void* w, uint8_t* packed, void* scales, uint8_t* zeros, int experts, int N, int K, int group,
@@ -223,9 +225,7 @@ int launch_int4_quantize(const void* w, uint8_t* packed, void* scales, uint8_t* 
   const dim3 grid(static_cast<unsigned>(blocks), experts);
   const bool wide = reinterpret_cast<uintptr_t>(w) % 32 == 0;
   auto go = [&](auto kernel) {
-    kernel<<<grid, kThreads, 0, s>>>(w, packed, scales, zeros, N, K, group, span, wide);
-    count_launch();
-    return cuda_status(cudaGetLastError());
+    return cuda_status(launch_ahead(kernel, grid, kThreads, 0, s, false, w, packed, scales, zeros, N, K, group, span, wide));
   };
   auto with = [&](auto n) {
     constexpr int S = decltype(n)::value;

@@ -105,6 +105,27 @@ struct SmemOptIn {
 };
 
 #ifdef __CUDACC__
+// Launch with programmatic stream serialisation: the kernel's first instructions may run while the kernel before it on the stream
+// finishes.  Every kernel launched this way executes grid_wait() before it reads what an earlier kernel may have written or
+// writes anything; only weights, which are constant, are read before it.  `plain`: the weights may have just been written.
+template <typename... Params, typename... Args>
+cudaError_t launch_ahead(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t s, bool plain, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = plain ? 0 : 1;
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // group of columns k ... k + 15 (k a multiple of 16)
 __device__ __forceinline__ int int4_group_of(const Int4Weight& w, int k) {
   return static_cast<int>(__umulhi(static_cast<uint32_t>(k) >> 4, w.group_magic));

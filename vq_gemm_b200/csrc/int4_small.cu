@@ -15,7 +15,7 @@
 namespace vqg {
 namespace {
 
-constexpr int kWarps = 8;                    // of a block of the direct down product
+constexpr int kWarps = 16;                   // of a block of the direct down product
 constexpr size_t kSmallSmem = 227 * 1024;    // shared memory of a block, at most
 
 struct SmallParams {
@@ -151,6 +151,8 @@ int4_small_kernel(const SmallParams p) {
   const int groups = (w.row_tiles() + R - 1) / R, k_tiles = w.k_tiles(), pitch = k_tiles * 128 + 16;
   const bool works = warp * B < k_tiles;                    // the warp has a block of a row group
 
+  grid_release();
+  if constexpr (MODE != kDense) grid_wait();               // (the dense product's weights are read before it)
   const int chunks = MODE == kDense ? p.chunks : p.rows.chunks ? *p.rows.n_chunks : p.rows.slots;
   const int per = max(1, static_cast<int>(gridDim.x) / max(1, chunks));    // blocks per chunk
   const int part = blockIdx.x % per, stride = gridDim.x / per;
@@ -215,6 +217,7 @@ int4_small_kernel(const SmallParams p) {
     }
     Scales<ZEROS, R, B, SPAN> ahead;
     if (works && rg0 < rg1) load_scales<ZEROS, R, B, SPAN>(ahead, w, v, rg0 * R, warp * B, g, t);
+    if constexpr (MODE == kDense) grid_wait();
     if constexpr (XS) {   // columns that fill up the last step are zero
       for (int c = threadIdx.x / 32; c < rows_here; c += WARPS) {
         const uint4* src = reinterpret_cast<const uint4*>(x_row(c));
@@ -325,11 +328,11 @@ int4_small_kernel(const SmallParams p) {
 // y[token] = sum_j weight_j * H[token * top_k + j] W_{e_j}^T: the K loops of all choices of a token, dealt out to the warps
 // one after the other, and the weighted sum in the same reduction.
 template <bool BF16, bool ZEROS>
-__global__ void __launch_bounds__(kWarps * 32, 3)
+__global__ void __launch_bounds__(kWarps * 32, 1)
 int4_small_down_direct_kernel(const SmallParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
-  constexpr int B = 2, SLOTS = 4;
+  constexpr int B = 2, SLOTS = 2;
   __shared__ __align__(128) unsigned char rings[kWarps][SLOTS][B * 512];
   __shared__ float red[kWarps][2][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -337,63 +340,77 @@ int4_small_down_direct_kernel(const SmallParams p) {
   const Int4Weight& w = p.w;
   const int token = blockIdx.y, tile_row = blockIdx.x;
   const int kts = w.k_tiles(), blocks = (kts + B - 1) / B, units = blocks * p.rows.top_k;
+  grid_release();
+  grid_wait();
   // the warp's share of the blocks of all choices; blocks of dropped choices are passed over
-  int u = static_cast<int>(static_cast<long long>(units) * warp / kWarps), ahead = u;
   const int end = static_cast<int>(static_cast<long long>(units) * (warp + 1) / kWarps);
   const int* ids = p.rows.ids + token * p.rows.top_k;
-  auto dropped = [&](int unit) {
-    const int e = ids[unit / blocks];
-    return e < 0 || e >= p.rows.E;
+  auto skip = [&](int unit) {   // the first unit from this one on whose choice was not dropped
+    while (unit < end) {
+      const int e = ids[unit / blocks];
+      if (e >= 0 && e < p.rows.E) break;
+      unit = (unit / blocks + 1) * blocks;
+    }
+    return unit;
   };
   unsigned char* ring = &rings[warp][0][0];
   const uint32_t put = place(lane & 7, lane >> 3), get = place(g, t);
+  int copy = skip(static_cast<int>(static_cast<long long>(units) * warp / kWarps)), u = copy;
   auto fill = [&](unsigned char* to) {
-    const uint32_t slot = smem_u32(to);
-    while (ahead < end && dropped(ahead)) ++ahead;
-    if (ahead < end) {
-      const int kt = (ahead % blocks) * B;
-      const uint8_t* src = w.packed + ids[ahead / blocks] * w.expert_bytes() + (static_cast<size_t>(tile_row) * kts + kt) * 512 + lane * 16;
+    if (copy < end) {
+      const int kt = (copy % blocks) * B;
+      const uint8_t* src = w.packed + ids[copy / blocks] * w.expert_bytes() + (static_cast<size_t>(tile_row) * kts + kt) * 512 + lane * 16;
 #pragma unroll
       for (int b = 0; b < B; ++b)
-        if (kt + b < kts) copy16(slot + put + b * 512, src + b * 512);
-      ++ahead;
+        if (kt + b < kts) copy16(smem_u32(to) + put + b * 512, src + b * 512);
+      copy = skip(copy + 1);
     }
     copy_commit();
   };
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) fill(ring + i * (B * 512));
-  float lo = 0.f, hi = 0.f;
-  unsigned char* at = ring;
-  for (; u < end; ++u) {
-    if (dropped(u)) continue;
-    const int j = u / blocks, slot = token * p.rows.top_k + j, expert = ids[j], kt = (u % blocks) * B;
+  struct Ahead {
+    Scales<ZEROS, 1, B, 1> sc;
+    uint4 x[B][1][2];
+    float weight;
+  };
+  auto fetch = [&](Ahead& a, int unit) {
+    const int slot = token * p.rows.top_k + unit / blocks, expert = ids[unit / blocks], kt = (unit % blocks) * B;
     const View v{w.packed, static_cast<const unsigned short*>(w.scales) + expert * w.expert_scales(),
                  ZEROS ? w.zeros + expert * w.expert_scales() : nullptr};
+    load_scales<ZEROS, 1, B, 1>(a.sc, w, v, tile_row, kt, g, t);
     const T* h = static_cast<const T*>(p.x) + static_cast<long long>(slot) * w.K + t * 16;
-    float acc[1][1][2][4] = {};
-    Scales<ZEROS, 1, B, 1> sc;
-    load_scales<ZEROS, 1, B, 1>(sc, w, v, tile_row, kt, g, t);
-    uint4 x[B][1][2];
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      x[b][0][0] = x[b][0][1] = make_uint4(0, 0, 0, 0);
+      a.x[b][0][0] = a.x[b][0][1] = make_uint4(0, 0, 0, 0);
       if ((kt + b) * 64 + t * 16 < w.K) {
-        x[b][0][0] = __ldg(reinterpret_cast<const uint4*>(h + (kt + b) * 64));
-        x[b][0][1] = __ldg(reinterpret_cast<const uint4*>(h + (kt + b) * 64) + 1);
+        a.x[b][0][0] = __ldg(reinterpret_cast<const uint4*>(h + (kt + b) * 64));
+        a.x[b][0][1] = __ldg(reinterpret_cast<const uint4*>(h + (kt + b) * 64) + 1);
       }
     }
+    a.weight = p.rows.weights[slot];
+  };
+  Ahead now, next;
+  if (u < end) fetch(next, u);
+  float lo = 0.f, hi = 0.f;
+  unsigned char* at = ring;
+  while (u < end) {
+    now = next;
+    const int kt = (u % blocks) * B;
+    u = skip(u + 1);
+    if (u < end) fetch(next, u);
+    float acc[1][1][2][4] = {};
     copy_wait<SLOTS - 1>();
     __syncwarp();
 #pragma unroll
     for (int b = 0; b < B; ++b)
       if (kt + b < kts)
-        multiply<BF16, ZEROS, 1, 1, B, 1, 2>(sc, b, (kt + b) * 64 + t * 16 < w.K, at + get + b * 512, x[b], acc);
+        multiply<BF16, ZEROS, 1, 1, B, 1, 2>(now.sc, b, (kt + b) * 64 + t * 16 < w.K, at + get + b * 512, now.x[b], acc);
     __syncwarp();
     fill(at);
     at = at == ring + (SLOTS - 1) * (B * 512) ? ring : at + B * 512;
-    const float weight = p.rows.weights[slot];
-    lo += weight * (acc[0][0][0][0] + acc[0][0][1][0]);
-    hi += weight * (acc[0][0][0][2] + acc[0][0][1][2]);
+    lo += now.weight * (acc[0][0][0][0] + acc[0][0][1][0]);
+    hi += now.weight * (acc[0][0][0][2] + acc[0][0][1][2]);
   }
   if (t == 0) { red[warp][0][g] = lo; red[warp][1][g] = hi; }
   __syncthreads();
@@ -417,9 +434,7 @@ int launch_one(const SmallParams& p, int rows, cudaStream_t s) {
   // as many blocks as run at once, or one per row group where there are fewer of those
   const long long slots = static_cast<long long>(sm_count_cached()) * MIN_BLOCKS;
   const int blocks = static_cast<int>(min(slots, groups * p.chunks));
-  kernel<<<blocks, WARPS * 32, smem, s>>>(p);
-  count_launch();
-  return cuda_status(cudaGetLastError());
+  return cuda_status(launch_ahead(kernel, dim3(blocks), WARPS * 32, smem, s, take_weights_written(s), p));
 }
 
 // rows: of a chunk, at most; p.chunks: how many chunks there are, at most
@@ -495,11 +510,10 @@ int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, c
   SmallParams p{};
   p.w = w; p.x = h; p.y = y; p.rows = rows;
   const dim3 grid(w.row_tiles(), tokens);
-  auto go = [&](auto kernel) { kernel<<<grid, kWarps * 32, 0, s>>>(p); };
-  if (w.zeros) bf16 ? go(int4_small_down_direct_kernel<true, true>) : go(int4_small_down_direct_kernel<false, true>);
-  else bf16 ? go(int4_small_down_direct_kernel<true, false>) : go(int4_small_down_direct_kernel<false, false>);
-  count_launch();
-  return cuda_status(cudaGetLastError());
+  const bool plain = take_weights_written(s);
+  auto go = [&](auto kernel) { return cuda_status(launch_ahead(kernel, grid, kWarps * 32, 0, s, plain, p)); };
+  if (w.zeros) return bf16 ? go(int4_small_down_direct_kernel<true, true>) : go(int4_small_down_direct_kernel<false, true>);
+  return bf16 ? go(int4_small_down_direct_kernel<true, false>) : go(int4_small_down_direct_kernel<false, false>);
 }
 
 }  // namespace vqg

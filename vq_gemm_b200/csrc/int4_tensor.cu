@@ -220,7 +220,8 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_release();
+  grid_wait();
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -609,7 +610,8 @@ __global__ void __launch_bounds__(256)
 int4_tensor_sum_kernel(const TensorParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_release();
+  grid_wait();
   const int end = pair_begin(blockIdx.y + 1, p.q, p.r);
   if (end % p.units_per_tile == 0) return;
   const int tile = end / p.units_per_tile, t0u = tile * p.units_per_tile;
@@ -641,6 +643,8 @@ int4_tensor_sum_kernel(const TensorParams p) {
 // Rows of X in the order of the plan (one block per row).
 __global__ void __launch_bounds__(128)
 gather_rows_kernel(const uint4* __restrict__ x, const ExpertRows rows, uint4* __restrict__ out, int vecs) {
+  grid_release();
+  grid_wait();
   for (int r = blockIdx.x; r < rows.n_chunks[1]; r += gridDim.x) {
     const uint4* src = x + static_cast<long long>(rows.row_slot[r] / rows.top_k) * vecs;
     for (int i = threadIdx.x; i < vecs; i += blockDim.x) out[static_cast<long long>(r) * vecs + i] = __ldg(src + i);
@@ -683,9 +687,7 @@ int launch(int pairs, const void* x, int rows, const TensorParams& p, cudaStream
   CUtensorMap map, map32;
   if (!make_x_map(&map, x, rows, p.w.K, 128, BF16) || !make_x_map(&map32, x, rows, p.w.K, 32, BF16) || !opt_in.ask(kernel))
     return VQG_ERR_LAUNCH;
-  kernel<<<2 * pairs, kThreads, kSmem + 1024, s>>>(map, map32, p);
-  count_launch();
-  return cuda_status(cudaGetLastError());
+  return cuda_status(launch_ahead(kernel, dim3(2 * pairs), kThreads, kSmem + 1024, s, false, map, map32, p));
 }
 
 }  // namespace
@@ -715,19 +717,9 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   p.ws_partial = split ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes) : nullptr;
   const int st = bf16 ? launch<true, kDense>(pairs, x, M, p, s) : launch<false, kDense>(pairs, x, M, p, s);
   if (st != VQG_OK || !split || pairs == 1) return st;
-  // enqueued so that it can take its place on the SMs as the first kernel leaves them; it waits for that one to complete
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(((M < BM ? M : BM) * 64 + 255) / 256, pairs - 1);
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, int4_tensor_sum_kernel<true>, p) : cudaLaunchKernelEx(&cfg, int4_tensor_sum_kernel<false>, p);
-  count_launch();
-  return cuda_status(e);
+  const dim3 grid(((M < BM ? M : BM) * 64 + 255) / 256, pairs - 1);
+  return cuda_status(bf16 ? launch_ahead(int4_tensor_sum_kernel<true>, grid, 256, 0, s, false, p)
+                          : launch_ahead(int4_tensor_sum_kernel<false>, grid, 256, 0, s, false, p));
 }
 
 namespace {
@@ -756,9 +748,8 @@ int launch_int4_tensor_down(const Int4Weight& w, const void* h, float* part, con
 
 int launch_gather_rows(const void* x, const ExpertRows& rows, void* out, int cols, cudaStream_t s) {
   const int blocks = rows.slots < 148 * 16 ? rows.slots : 148 * 16;
-  gather_rows_kernel<<<blocks, 128, 0, s>>>(static_cast<const uint4*>(x), rows, static_cast<uint4*>(out), cols / 8);
-  count_launch();
-  return cuda_status(cudaGetLastError());
+  return cuda_status(launch_ahead(gather_rows_kernel, dim3(blocks), 128, 0, s, false, static_cast<const uint4*>(x), rows,
+                                  static_cast<uint4*>(out), cols / 8));
 }
 
 }  // namespace vqg

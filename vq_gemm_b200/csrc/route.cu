@@ -149,13 +149,16 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
 // Selection: at least top_k + 1 choices are as large as the (top_k + 1)-th largest of the 32 lanes' maxima, and few more are
 // (about ten in all for 8 of 256).  Those go to a list in shared memory and are ranked by comparing each with all of them.
 // The kernel is bound by issue, not by its bytes.
-template <int EPL, int TYPE>
+// FULL: there are exactly 32 * EPL experts
+template <int EPL, int TYPE, bool FULL>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_kernel(const RouteParams p) {
   __shared__ double s_all[kRouteWarps][EPL * 32 + EPL * 16 + 50];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * kRouteWarps + warp;
   if (token >= p.T) return;
+  grid_release();
+  grid_wait();
   double* scratch = s_all[warp];
   const bool plain = !p.bias && p.groups == 1;
   float choice[EPL], prob[EPL];   // prob: exp(logit - top) or the sigmoid
@@ -164,7 +167,7 @@ route_kernel(const RouteParams p) {
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     float l = -INFINITY;
-    if (lane + 32 * i < p.E) l = fmaxf(load_logit(p.logits, TYPE, row + 32 * i), -INFINITY);   // NaN: -inf
+    if (FULL || lane + 32 * i < p.E) l = fmaxf(load_logit(p.logits, TYPE, row + 32 * i), -INFINITY);   // NaN: -inf
     choice[i] = l;
     top = fmaxf(top, l);
   }
@@ -203,7 +206,7 @@ route_kernel(const RouteParams p) {
     float* s = reinterpret_cast<float*>(scratch);
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
-      if (lane + 32 * i < p.E) s[lane + 32 * i] = choice[i];
+      if (FULL || lane + 32 * i < p.E) s[lane + 32 * i] = choice[i];
     __syncwarp();
     // 32 / 2^n lanes per group, 2^n >= groups; each starts at another place, so that the groups' reads spread over the banks
     const int shift = 32 - __clz(p.groups - 1), per = 32 >> shift;   // lanes per group
@@ -245,20 +248,17 @@ route_kernel(const RouteParams p) {
     }
     __syncwarp();
   }
-  // the (top_k + 1)-th largest of the lanes' maxima: a bitonic sort, largest first
+  // the (top_k + 1)-th largest of the lanes' maxima
   float bound = -INFINITY;
   if (p.top_k < 32) {
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) m = fmaxf(m, choice[i]);
-#pragma unroll
-    for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll
-      for (int d = k >> 1; d; d >>= 1) {
-        const float o = __shfl_xor_sync(kAll, m, d);
-        m = ((lane & d) == 0) == ((lane & k) == 0) ? fmaxf(m, o) : fminf(m, o);
-      }
-    bound = __shfl_sync(kAll, m, p.top_k);
+    // (lanes whose maxima are equal leave together: the bound is then lower, never higher)
+    for (int j = 0; j <= p.top_k; ++j) {
+      bound = warp_max(m);
+      if (m == bound) m = -INFINITY;
+    }
   }
   // the list: choice and expert, and p, of each candidate; behind it the first top_k + 1 in order
   float2* list = reinterpret_cast<float2*>(scratch);
@@ -335,6 +335,8 @@ expert_plan_kernel(const int* __restrict__ ids, int slots, int E, int chunk_rows
                    int4* __restrict__ chunks, int* __restrict__ n_chunks) {
   __shared__ int count[512], place[512], scan[2][16];
   const int blocks = gridDim.x, me = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grid_release();
+  grid_wait();
   if (tid < 512) count[tid] = 0;
   __syncthreads();
   const int begin = static_cast<int>(static_cast<long long>(slots) * me / blocks), end = static_cast<int>(static_cast<long long>(slots) * (me + 1) / blocks);
@@ -385,6 +387,8 @@ __global__ void __launch_bounds__(256)
 expert_combine_kernel(const float* __restrict__ part, const ExpertRows rows, void* __restrict__ y, int cols) {
   using I = Int4Type<BF16>;
   const int token = blockIdx.x;
+  grid_release();
+  grid_wait();
   for (int c = threadIdx.x * 4; c < cols; c += 256 * 4) {   // cols is a multiple of 4
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j = 0; j < rows.top_k; ++j) {
@@ -410,17 +414,15 @@ int launch_route_experts(const void* logits, int logits_type, const float* bias,
   p.size_magic = size > 1 ? static_cast<unsigned>(((1ULL << 32) + size - 1) / size) : 0u;
   const int blocks = (T + kRouteWarps - 1) / kRouteWarps;
   auto go = [&](auto kernel) {
-    kernel<<<blocks, kRouteWarps * 32, 0, s>>>(p);
-    count_launch();
-    return cuda_status(cudaGetLastError());
+    return cuda_status(launch_ahead(kernel, dim3(blocks), kRouteWarps * 32, 0, s, false, p));
   };
   auto with = [&](auto type) {
     constexpr int Y = decltype(type)::value;
-    if (E <= 32) return go(route_kernel<1, Y>);
-    if (E <= 64) return go(route_kernel<2, Y>);
-    if (E <= 128) return go(route_kernel<4, Y>);
-    if (E <= 256) return go(route_kernel<8, Y>);
-    return go(route_kernel<16, Y>);
+    if (E <= 32) return go(route_kernel<1, Y, false>);
+    if (E <= 64) return E == 64 ? go(route_kernel<2, Y, true>) : go(route_kernel<2, Y, false>);
+    if (E <= 128) return E == 128 ? go(route_kernel<4, Y, true>) : go(route_kernel<4, Y, false>);
+    if (E <= 256) return E == 256 ? go(route_kernel<8, Y, true>) : go(route_kernel<8, Y, false>);
+    return E == 512 ? go(route_kernel<16, Y, true>) : go(route_kernel<16, Y, false>);
   };
   if (E > 512) return static_cast<int>(VQG_ERR_UNSUPPORTED);
   if (logits_type == 0) return with(std::integral_constant<int, 0>{});
@@ -436,22 +438,22 @@ int launch_expert_plan(const int* ids, int slots, int E, int chunk_rows, int* ro
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(kPlanThreads);
   cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = blocks;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, expert_plan_kernel, ids, slots, E, chunk_rows, row_slot, chunks, n_chunks);
   count_launch();
   return cuda_status(e);
 }
 
 int launch_expert_combine(const float* part, const ExpertRows& rows, void* y, int tokens, int cols, bool bf16, cudaStream_t s) {
-  if (bf16) expert_combine_kernel<true><<<tokens, 256, 0, s>>>(part, rows, y, cols);
-  else expert_combine_kernel<false><<<tokens, 256, 0, s>>>(part, rows, y, cols);
-  count_launch();
-  return cuda_status(cudaGetLastError());
+  return cuda_status(bf16 ? launch_ahead(expert_combine_kernel<true>, dim3(tokens), 256, 0, s, false, part, rows, y, cols)
+                          : launch_ahead(expert_combine_kernel<false>, dim3(tokens), 256, 0, s, false, part, rows, y, cols));
 }
 
 }  // namespace vqg
