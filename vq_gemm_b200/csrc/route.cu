@@ -47,91 +47,106 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// The definition in 64 bits, for the rows whose order 32 bits do not settle.  One warp; lane l holds experts l, l + 32, ...;
-// `s_choice` has room for E values.
-template <int EPL>
-__device__ __noinline__ void route_row_64(const RouteParams& p, int token, double* s_choice) {
+// The definition in 64 bits, for the rows that 32 bits do not settle (one in some thousands).  One warp; lane l works on experts l,
+// l + 32, ...; `scratch` has room for 2 E values: p, and the choices behind them.
+__device__ __noinline__ void choices_64(const RouteParams& p, int token, double* scratch) {
   const int lane = threadIdx.x & 31;
-  double prob[EPL], choice[EPL];
+  double* prob = scratch;
+  double* choice = scratch + p.E;
   double top = kNone;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    double x = kNone;
-    if (e < p.E) {
-      const float l = load_logit(p.logits, p.type, static_cast<long long>(token) * p.E + e);
-      if (l > -INFINITY) x = fmin(static_cast<double>(l), 1e200);      // +inf takes all of the softmax
-    }
-    prob[i] = x;
+#pragma unroll 1
+  for (int e = lane; e < p.E; e += 32) {
+    const float l = load_logit(p.logits, p.type, static_cast<long long>(token) * p.E + e);
+    const double x = l > -INFINITY ? fmin(static_cast<double>(l), 1e200) : kNone;      // +inf takes all of the softmax
+    prob[e] = x;
     top = fmax(top, x);
   }
   for (int d = 16; d; d >>= 1) top = fmax(top, __shfl_xor_sync(kAll, top, d));
-  if (p.sigmoid) {
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) prob[i] = prob[i] > kNone ? 1.0 / (1.0 + exp(-prob[i])) : -1.0;
-  } else {
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      prob[i] = prob[i] > kNone ? exp(prob[i] - top) : -1.0;
-      sum += fmax(prob[i], 0.0);
+  double sum = 0.0;
+#pragma unroll 1
+  for (int e = lane; e < p.E; e += 32) {
+    const double x = prob[e];
+    const double v = exp(p.sigmoid ? -x : x - top);      // (of kNone: not used)
+    prob[e] = x <= kNone ? -1.0 : v;
+    if (x > kNone) sum += v;
+  }
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kAll, sum, d);
+#pragma unroll 1
+  for (int e = lane; e < p.E; e += 32) {
+    double v = prob[e];
+    const bool in = v >= 0.0;
+    v = p.sigmoid ? 1.0 / (1.0 + v) : v / sum;
+    prob[e] = v;
+    choice[e] = !in ? kNone : p.bias ? v + static_cast<double>(__ldg(p.bias + e)) : v;
+  }
+  __syncwarp();
+}
+
+// The kept groups, bit n << shift for group n, from the choices.
+__device__ __noinline__ unsigned groups_64(const RouteParams& p, const double* choice, int shift_out) {
+  const int lane = threadIdx.x & 31, size = p.E / p.groups;
+  const int shift = 5 - (32 - __clz(p.groups - 1)), per = 1 << shift;   // 2^shift lanes per group
+  const int group = lane >> shift, sub = lane & (per - 1);
+  double first = kNone, second = kNone;
+  if (group < p.groups)
+#pragma unroll 1
+    for (int i = sub; i < size; i += per) {
+      const double c = choice[group * size + i];
+      second = fmax(second, fmin(first, c));
+      first = fmax(first, c);
     }
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kAll, sum, d);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) prob[i] = prob[i] >= 0.0 ? prob[i] / sum : -1.0;
+  for (int d = 1; d < per; d <<= 1) {
+    const double of = __shfl_xor_sync(kAll, first, d), os = __shfl_xor_sync(kAll, second, d);
+    second = fmax(fmin(first, of), fmax(second, os));
+    first = fmax(first, of);
   }
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    choice[i] = prob[i] < 0.0 ? kNone : p.bias ? prob[i] + static_cast<double>(__ldg(p.bias + e)) : prob[i];
+  const double score = p.group_max || second <= kNone ? first : first + second;
+  int better = 0;
+  for (int j = 0; j < p.groups; ++j) {
+    const double other = __shfl_sync(kAll, score, j << shift);
+    better += other > score || (other == score && j < group);
   }
+  const unsigned kept = __ballot_sync(kAll, group < p.groups && sub == 0 && better < p.top_groups);
+  if (shift == shift_out) return kept;
+  unsigned moved = 0;
+  for (int j = 0; j < p.groups; ++j) moved |= (kept >> (j << shift) & 1u) << (j << shift_out);
+  return moved;
+}
+
+__device__ __noinline__ void route_row_64(const RouteParams& p, int token, double* scratch) {
+  const int lane = threadIdx.x & 31;
+  double* prob = scratch;
+  double* choice = scratch + p.E;
+  choices_64(p, token, scratch);
   if (p.groups > 1) {
     const int size = p.E / p.groups;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (lane + 32 * i < p.E) s_choice[lane + 32 * i] = choice[i];
+    const unsigned kept = groups_64(p, choice, 0);
+    for (int e = lane; e < p.E; e += 32)
+      if (!(kept >> (e / size) & 1u)) choice[e] = kNone;
     __syncwarp();
-    double score = kNone;
-    if (lane < p.groups) {
-      double first = kNone, second = kNone;
-      for (int i = 0; i < size; ++i) {
-        const double c = s_choice[lane * size + i];
-        if (c > first) { second = first; first = c; }
-        else if (c > second) second = c;
-      }
-      score = p.group_max || second <= kNone ? first : first + second;
-    }
-    int better = 0;
-    for (int j = 0; j < p.groups; ++j) {
-      const double other = __shfl_sync(kAll, score, j);
-      better += other > score || (other == score && j < lane);
-    }
-    const unsigned kept = __ballot_sync(kAll, lane < p.groups && better < p.top_groups);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 32 * i;
-      if (e < p.E && !(kept >> (e / size) & 1u)) choice[i] = kNone;
-    }
   }
   double chosen = 0.0, total = 0.0;   // lane j keeps slot j's weight
   int id = -1;
+#pragma unroll 1
   for (int j = 0; j < p.top_k; ++j) {
-    double best = kNone, bp = 0.0;
+    double best = kNone;              // the lane's largest choice, the lowest index first
     int at = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (choice[i] > best) { best = choice[i]; bp = prob[i]; at = lane + 32 * i; }
-    for (int d = 16; d; d >>= 1) {
-      const double ob = __shfl_xor_sync(kAll, best, d), op = __shfl_xor_sync(kAll, bp, d);
-      const int oa = __shfl_xor_sync(kAll, at, d);
-      if (ob > best || (ob == best && oa < at)) { best = ob; bp = op; at = oa; }
-    }
-    if (best <= kNone) break;
-    if (lane == j) { chosen = bp; id = at; }
-    total += bp;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (at == lane + 32 * i) choice[i] = kNone;
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32)
+      if (choice[e] > best) { best = choice[e]; at = e; }
+    // the bits of a double, made to sort like an unsigned number: the upper halves' maximum, then the lower ones' among those
+    const long long bits = __double_as_longlong(best);
+    const unsigned long long key = static_cast<unsigned long long>(bits ^ ((bits >> 63) | (1LL << 63)));
+    const unsigned high = static_cast<unsigned>(key >> 32), low = static_cast<unsigned>(key);
+    const bool in = high == __reduce_max_sync(kAll, high);
+    const unsigned most = __reduce_max_sync(kAll, in ? low : 0u);
+    const int e = static_cast<int>(__reduce_min_sync(kAll, in && low == most ? static_cast<unsigned>(at) : 0x7fffffffu));
+    if (e == 0x7fffffff) break;       // only lanes that have nothing left
+    const double pe = prob[e];
+    if (lane == j) { chosen = pe; id = e; }
+    total += pe;
+    if (lane == (e & 31)) choice[e] = kNone;
+    __syncwarp();
   }
   if (lane < p.top_k) {
     if (p.renormalize) chosen = total > 0.0 ? chosen / total : 0.0;
@@ -141,34 +156,34 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
   }
 }
 
-// One warp per token, in 32 bits, with a proof that 64 would choose the same: choices that follow one another in the order (and
-// the last kept and first dropped group) must be further apart than the arithmetic below can be wrong; rows where they are
-// not are done again in 64 bits.  Without bias and groups the order is that of the logits themselves, which are compared
-// exactly.
-//
-// Selection: at least top_k + 1 choices are as large as the (top_k + 1)-th largest of the 32 lanes' maxima, and few more are
-// (about ten in all for 8 of 256).  Those go to a list in shared memory and are ranked by comparing each with all of them.
+// One warp per token.  Where 32 bits do not settle an order, it is not taken from them:
+//   * without a bias the order of the choices is that of the logits, which are compared exactly;
+//   * sigmoid and bias: the few candidates' choices are computed in 64 bits, one lane each;
+//   * softmax and bias, and the choice of groups: values that follow one another must be further apart than the arithmetic can
+//     be wrong, else the row is done again in 64 bits.
+// Candidates: at least top_k + 1 choices are as large as the (top_k + 1)-th largest of the 32 lanes' maxima, and few more are
+// (about ten in all for 8 of 256).  They go to a list in shared memory and are ranked by comparing each with all of them.
 // The kernel is bound by issue, not by its bytes.
 // FULL: there are exactly 32 * EPL experts
 template <int EPL, int TYPE, bool FULL>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_kernel(const RouteParams p) {
-  __shared__ double s_all[kRouteWarps][EPL * 32 + EPL * 16 + 50];
+  __shared__ double s_all[kRouteWarps][EPL * 64 > EPL * 48 + 50 ? EPL * 64 : EPL * 48 + 50];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * kRouteWarps + warp;
   if (token >= p.T) return;
   grid_release();
   grid_wait();
   double* scratch = s_all[warp];
-  const bool plain = !p.bias && p.groups == 1;
-  float choice[EPL], prob[EPL];   // prob: exp(logit - top) or the sigmoid
+  const bool fine = p.bias && p.sigmoid;   // candidates in 64 bits
+  float logit[EPL], choice[EPL], prob[EPL];  // prob: exp(logit - top), or p itself where it is needed
   float top = -INFINITY;
   const long long row = static_cast<long long>(token) * p.E + lane;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     float l = -INFINITY;
     if (FULL || lane + 32 * i < p.E) l = fmaxf(load_logit(p.logits, TYPE, row + 32 * i), -INFINITY);   // NaN: -inf
-    choice[i] = l;
+    logit[i] = choice[i] = l;
     top = fmaxf(top, l);
   }
   top = warp_max(top);
@@ -176,77 +191,102 @@ route_kernel(const RouteParams p) {
   float inverse = 1.f;            // of the softmax's sum
   if (p.sigmoid) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) prob[i] = __fdividef(1.f, 1.f + expf(-choice[i]));
+    for (int i = 0; i < EPL; ++i) prob[i] = __frcp_rn(1.f + expf(-logit[i]));
   } else {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      prob[i] = choice[i] > -INFINITY ? expf(choice[i] - top) : 0.f;
+      prob[i] = expf(logit[i] - (top > -INFINITY ? top : 0.f));     // of -inf: 0
       sum += prob[i];
     }
     sum = warp_sum(sum);
     inverse = sum > 0.f ? 1.f / sum : 0.f;
+    if (p.bias || p.groups > 1) {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) prob[i] *= inverse;
+      inverse = 1.f;
+    }
   }
-  // 32-bit errors, relative to p: the exponential 2^-22, its sum with one 2^-24, the reciprocal 2^-22; in the softmax also the
-  // exponent's difference (at most 2^-25 of it, times what is left of p) and a sum of at most 16 + 5 roundings.  Adding the bias
-  // rounds once more.  `slack` is twice what that comes to, relative to what goes in.
-  const float slack = p.sigmoid ? 1.f / (1 << 20) : 1.f / (1 << 18);
-  if (!plain) {
+  if (p.bias) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      if (choice[i] > -INFINITY) {
-        prob[i] *= inverse;
-        choice[i] = p.bias ? fmaxf(prob[i] + __ldg(p.bias + lane + 32 * i), -INFINITY) : prob[i];
-      }
+      const float v = prob[i] + (FULL || lane + 32 * i < p.E ? __ldg(p.bias + lane + 32 * i) : 0.f);
+      choice[i] = logit[i] > -INFINITY ? fmaxf(v, -INFINITY) : -INFINITY;
     }
-    inverse = 1.f;
   }
+  // How far a choice can be off.  Sigmoid: the exponential 2^-22 of itself, which moves p by p (1 - p) <= 1/4 as much, its sum with
+  // one and the reciprocal 2^-24 of p each: 1.8e-7.  Softmax: exponential, argument, a sum of at most 16 + 5 roundings and a
+  // division, below 2^-19 of p.  The bias's addition: 2^-24 of the choice.  (Kept close: a row that has to be done again costs
+  // ten microseconds of latency, most of it the fetching of instructions.)
+  const float of_p = p.sigmoid ? 1.8e-7f : 1.f / (1 << 19), of_choice = 1.f / (1 << 24);
   if (p.groups > 1) {
     const int size = p.E / p.groups;
-    float* s = reinterpret_cast<float*>(scratch);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (FULL || lane + 32 * i < p.E) s[lane + 32 * i] = choice[i];
-    __syncwarp();
-    // 32 / 2^n lanes per group, 2^n >= groups; each starts at another place, so that the groups' reads spread over the banks
-    const int shift = 32 - __clz(p.groups - 1), per = 32 >> shift;   // lanes per group
-    const int group = lane >> (5 - shift), sub = lane & (per - 1);
+    // the two largest of each group: of group n in lane n << shift
     float first = -INFINITY, second = -INFINITY;
-    if (group < p.groups) {
-      const int n = (size - sub + per - 1) >> (5 - shift);
-      int at = n > group ? group : 0;
-      for (int i = 0; i < n; ++i) {
-        const float c = s[group * size + sub + per * at];
-        if (++at == n) at = 0;
-        second = fmaxf(second, fminf(first, c));
-        first = fmaxf(first, c);
+    int shift = 0;
+    if (size == 32) {   // group i is what the lanes hold in register i
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const float c = p.bias ? choice[i] : logit[i] > -INFINITY ? prob[i] : -INFINITY;
+        const float a = warp_max(c);
+        const int at = __ffs(__ballot_sync(kAll, c == a)) - 1;
+        const float b = warp_max(lane == at ? -INFINITY : c);
+        if (lane == i) { first = a; second = b; }
       }
+    } else {
+      float* s = reinterpret_cast<float*>(scratch);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (FULL || lane + 32 * i < p.E) s[lane + 32 * i] = p.bias ? choice[i] : logit[i] > -INFINITY ? prob[i] : -INFINITY;
+      __syncwarp();
+      // 2^shift lanes per group; each group starts at another place, so that the reads spread over the banks
+      shift = 5 - (32 - __clz(p.groups - 1));
+      const int per = 1 << shift, group = lane >> shift, sub = lane & (per - 1);
+      if (group < p.groups) {
+        const int n = (size - sub + per - 1) >> shift;
+        int at = n > group ? group : 0;
+        const float* mine = s + group * size + sub;
+        for (int i = 0; i < n; ++i) {
+          const float c = mine[per * at];
+          if (++at == n) at = 0;
+          second = fmaxf(second, fminf(first, c));
+          first = fmaxf(first, c);
+        }
+      }
+      for (int d = 1; d < per; d <<= 1) {
+        const float of = __shfl_xor_sync(kAll, first, d), os = __shfl_xor_sync(kAll, second, d);
+        second = fmaxf(fminf(first, of), fmaxf(second, os));
+        first = fmaxf(first, of);
+      }
+      __syncwarp();
     }
-    for (int d = 1; d < per; d <<= 1) {
-      const float of = __shfl_xor_sync(kAll, first, d), os = __shfl_xor_sync(kAll, second, d);
-      second = fmaxf(fminf(first, of), fmaxf(second, os));
-      first = fmaxf(first, of);
-    }
-    const bool mine = group < p.groups && sub == 0;
+    const bool mine = (lane >> shift) < p.groups && (lane & ((1 << shift) - 1)) == 0;
     const float score = p.group_max || second == -INFINITY ? first : first + second;
-    const float size_of = p.bias ? 1.f + fabsf(first) + fabsf(second > -INFINITY ? second : 0.f) : first + fmaxf(second, 0.f);
-    int better = 0;
-    for (int j = 0; j < p.groups; ++j) {
-      const float other = __shfl_sync(kAll, score, j << (5 - shift));
-      better += other > score || (other == score && j < group);
+    // the best top_groups of them, one after the other, equal ones in order
+    float left = mine ? score : -INFINITY, worst = INFINITY;
+    unsigned kept = 0;                                      // bit of each kept group's first lane
+    for (int j = 0; j < p.top_groups; ++j) {
+      const float m = warp_max(left);
+      if (m == -INFINITY) break;
+      const int at = __ffs(__ballot_sync(kAll, left == m)) - 1;
+      kept |= 1u << at;
+      worst = m;
+      if (lane == at) left = -INFINITY;
     }
-    const bool keep = mine && better < p.top_groups;
-    // (p is at most 1, and without bias it is the choice)
-    const float low = keep && score > -INFINITY ? score - 2.f * slack * size_of : INFINITY;
-    const float high = mine && !keep && score > -INFINITY ? score + 2.f * slack * size_of : -INFINITY;
-    sure = sure && -warp_max(-low) > warp_max(high);
-    const unsigned kept = __ballot_sync(kAll, keep);        // bit of each kept group's first lane
+    // the last kept one must be surely better than every other: two p of at most 1 (without bias they are the score), two
+    // choices of at most |score| + 2 in all, and their sum, of either group
+    const float best = warp_max(left);
+    const float wrong = (p.sigmoid || p.bias ? 2.f : fabsf(worst)) * of_p + (2.f * fabsf(worst) + (p.bias ? 2.f : 0.f)) * of_choice;
+    if (!(best == -INFINITY || worst - best > 2.1f * wrong)) {   // (the whole warp)
+      choices_64(p, token, scratch);
+      kept = groups_64(p, scratch + p.E, shift);
+      __syncwarp();
+    }
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       const unsigned e = static_cast<unsigned>(lane + 32 * i), of = p.size_magic ? __umulhi(e, p.size_magic) : e;
-      if (!(kept >> (of << (5 - shift)) & 1u)) choice[i] = -INFINITY;
+      if (!(kept >> (of << shift) & 1u)) choice[i] = -INFINITY;
     }
-    __syncwarp();
   }
   // the (top_k + 1)-th largest of the lanes' maxima
   float bound = -INFINITY;
@@ -260,55 +300,81 @@ route_kernel(const RouteParams p) {
       if (m == bound) m = -INFINITY;
     }
   }
-  // the list: choice and expert, and p, of each candidate; behind it the first top_k + 1 in order
+  if (fine) bound -= 4.f * (of_p + fabsf(bound) * of_choice);   // whoever 64 bits may put above it comes along
+  // the list: choice and expert, and logit or p, of each candidate; behind it the first top_k + 1 in order
   float2* list = reinterpret_cast<float2*>(scratch);
   float* list_p = reinterpret_cast<float*>(scratch + EPL * 32);
   float* sorted_c = list_p + EPL * 32;
   float* sorted_p = sorted_c + 33;
   int* sorted_e = reinterpret_cast<int*>(sorted_p + 33);
   int count = 0;
+  const unsigned below = (1u << lane) - 1u;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     const bool in = choice[i] >= bound && choice[i] > -INFINITY;
     const unsigned votes = __ballot_sync(kAll, in);
     if (in) {
-      const int at = count + __popc(votes & ((1u << lane) - 1u));
+      const int at = count + __popc(votes & below);
       list[at] = make_float2(choice[i], __int_as_float(lane + 32 * i));
-      list_p[at] = prob[i];
+      list_p[at] = fine ? logit[i] : prob[i];
     }
     count += __popc(votes);
   }
   __syncwarp();
   const int wanted = min(p.top_k, count);
-  for (int c = lane; c < count; c += 32) {
-    const float2 mine = list[c];
-    const int e = __float_as_int(mine.y);
+  if (fine && count <= 32) {
+    // one candidate per lane, its choice in the list's place
+    double* exact = scratch;
+    int e = 0;
+    double pe = 0.0, mine = kNone;
+    if (lane < count) {
+      e = __float_as_int(list[lane].y);
+      pe = 1.0 / (1.0 + exp(-static_cast<double>(list_p[lane])));
+      mine = pe + static_cast<double>(__ldg(p.bias + e));
+    }
+    __syncwarp();
+    exact[lane] = mine;
+    reinterpret_cast<int*>(list_p)[lane] = e;
+    __syncwarp();
     int rank = 0;
     for (int o = 0; o < count; ++o) {
-      const float2 other = list[o];
-      rank += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
+      const double other = exact[o];
+      rank += other > mine || (other == mine && reinterpret_cast<const int*>(list_p)[o] < e);
     }
-    if (rank <= p.top_k) { sorted_c[rank] = mine.x; sorted_p[rank] = list_p[c]; sorted_e[rank] = e; }
+    if (lane < count && rank < p.top_k) { sorted_p[rank] = static_cast<float>(pe); sorted_e[rank] = e; }
+    sure = sure && bound > -1e30f && bound < 1e30f;        // (a bias so large that the margin means nothing)
+  } else {
+    for (int c = lane; c < count; c += 32) {
+      const float2 mine = list[c];
+      const int e = __float_as_int(mine.y);
+      int rank = 0;
+      for (int o = 0; o < count; ++o) {
+        const float2 other = list[o];
+        rank += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
+      }
+      if (rank <= p.top_k) { sorted_c[rank] = mine.x; sorted_p[rank] = list_p[c]; sorted_e[rank] = e; }
+    }
+    if (fine) sure = false;
   }
   __syncwarp();
-  const float chosen_p = lane < wanted ? sorted_p[lane] : 0.f;
+  const float chosen = lane < wanted ? sorted_p[lane] : 0.f;
   const int id = lane < wanted ? sorted_e[lane] : -1;
-  if (lane + 1 < min(count, p.top_k + 1)) {   // is number lane + 1 surely behind number lane?
+  if (!fine && lane + 1 < min(count, p.top_k + 1)) {   // is number lane + 1 surely behind number lane?
     const float a = sorted_c[lane], b = sorted_c[lane + 1];
-    if (plain)   // different logits have different exponentials unless they are nearly equal or far out; equal ones are equal in 64 bits too
+    if (!p.bias)   // different logits have different exponentials unless they are nearly equal or far out; equal ones are equal in 64 bits too
       sure = sure && (p.sigmoid ? b > -600.f && (a == b || (a - b > 1e-12f && a < 16.f)) : a == b || (a - b > 1e-12f && b - top > -600.f));
     else
-      sure = sure && a < INFINITY && a - b > slack * (sorted_p[lane] + sorted_p[lane + 1] + fabsf(a) + fabsf(b));
+      sure = sure && a < INFINITY && a - b > (sorted_p[lane] + sorted_p[lane + 1]) * of_p + (fabsf(a) + fabsf(b)) * of_choice;
   }
-  const float total = warp_sum(chosen_p);
+  const float total = warp_sum(chosen);
   if (wanted > 0 && total < 1e-6f) sure = false;      // weights that 32 bits may not tell from zero
   if (__ballot_sync(kAll, !sure)) {
     __syncwarp();
-    route_row_64<EPL>(p, token, scratch);
+    route_row_64(p, token, scratch);
     return;
   }
   if (lane < p.top_k) {
-    const float weight = p.renormalize ? (total > 0.f ? chosen_p / total : 0.f) : chosen_p * inverse;
+    const float weight = p.renormalize ? (total > 0.f ? chosen / total : 0.f) : chosen * inverse;
     const long long o = static_cast<long long>(token) * p.top_k + lane;
     p.weights[o] = weight * p.scale;
     p.ids[o] = id;
