@@ -50,6 +50,8 @@ __device__ __forceinline__ uint32_t code_of(float q192, float zero) {
   return __float_as_uint(fminf(fmaxf(r, 12582912.f), 12582927.f));
 }
 
+__device__ __noinline__ float quotient(float a, float b) { return __fdiv_rn(a, b); }
+
 template <bool BF16>
 __global__ void __launch_bounds__(kThreads)
 int4_dequant_kernel(const Int4Weight w, void* __restrict__ out, bool wide) {
@@ -97,7 +99,7 @@ int4_dequant_kernel(const Int4Weight w, void* __restrict__ out, bool wide) {
 // two whole numbers or at least 2^-13 from there; rounding the product to multiples of 2^-16 first (adding 192 does) turns
 // what is nearly halfway into exactly halfway, and the codes are those of the correctly rounded division.
 template <bool BF16, bool ZEROS, int SPAN>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, SPAN == 2 ? 3 : 4)
 int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed, void* __restrict__ scales,
                      uint8_t* __restrict__ zeros, int N, int K, int group, int span_all, bool wide) {
   using I = Int4Type<BF16>;
@@ -166,7 +168,7 @@ int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed,
     z[h] = ZEROS ? fminf(fmaxf(rintf(__fdiv_rn(-lo[h], d)), 0.f), 15.f) : 8.f;
     inv[h] = __fdiv_rn(1.f, d);
     dv[h] = d;
-    tiny = tiny || d < 1e-36f;
+    tiny = tiny || inv[h] > 1e38f;
     const int row = tr * 16 + h * 8 + g, k = kt0 * 64 + t * 16;
     if (row < N && k < K && (group == 32 ? (t & 1) == 0 : t == 0)) {
       const long long to = sbase + static_cast<long long>(k / group) * N + row;
@@ -177,22 +179,24 @@ int4_quantize_kernel(const void* __restrict__ src, uint8_t* __restrict__ packed,
   tiny = __any_sync(0xffffffffu, tiny);
   auto encode = [&](int kt, const uint32_t (&d)[2][8]) {
     uint32_t words[4] = {0, 0, 0, 0};
+    if (!tiny) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {   // pair i: word i / 2, q = i % 2
-        const float2 f = unpack2<BF16>(d[h][i]);
-        uint32_t c0, c1;
-        if (!tiny) {
-          c0 = code_of(__fmaf_rn(f.x, inv[h], 192.f), z[h]);
-          c1 = code_of(__fmaf_rn(f.y, inv[h], 192.f), z[h]);
-        } else {                      // 1 / s may overflow
-          c0 = code_of(__fdiv_rn(f.x, dv[h]) + 192.f, z[h]);
-          c1 = code_of(__fdiv_rn(f.y, dv[h]) + 192.f, z[h]);
+        for (int i = 0; i < 8; ++i) {   // pair i: word i / 2, q = i % 2
+          const float2 f = unpack2<BF16>(d[h][i]);
+          const uint32_t pair = __byte_perm(code_of(__fmaf_rn(f.x, inv[h], 192.f), z[h]), code_of(__fmaf_rn(f.y, inv[h], 192.f), z[h]), 0x1410);
+          words[i >> 1] |= pair << (8 * (i & 1) + 4 * h);
         }
-        const uint32_t pair = __byte_perm(c0, c1, 0x1410);
-        words[i >> 1] |= pair << (8 * (i & 1) + 4 * h);
+    } else {                            // 1 / s is not a number that 32 bits hold
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int h = i >> 3, j = i & 7;
+        const float2 f = unpack2<BF16>(d[h][j]);
+        const uint32_t pair = __byte_perm(code_of(quotient(f.x, dv[h]) + 192.f, z[h]), code_of(quotient(f.y, dv[h]) + 192.f, z[h]), 0x1410);
+        words[j >> 1] |= pair << (8 * (j & 1) + 4 * h);
       }
+    }
     reinterpret_cast<uint4*>(codes + (static_cast<long long>(tr) * k_tiles + kt) * 512)[lane] =
         make_uint4(words[0], words[1], words[2], words[3]);
   };
