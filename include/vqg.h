@@ -317,8 +317,7 @@ VQG_API int vqg_unpack12(const void* packed, void* idx_u16_out, long long values
  * Experts put a leading dimension [E] before all three.
  *
  * vqg_int4_gemm: Y[M, N] = X[M, K] * W^T, fp32 accumulation, one rounding to T.  Workspace of
- *   vqg_int4_workspace_bytes() bytes (0: none is needed), 1024-byte aligned, its first
- *   vqg_workspace_counter_bytes() zeroed once, one per stream.
+ *   vqg_int4_workspace_bytes() bytes (0: none is needed), 256-byte aligned, contents arbitrary.
  * vqg_int4_dequant: W [E, N, K] of type T, the bits that the products multiply.
  * vqg_int4_quantize: the format from dense weights [E, N, K] of type T.  Per group, every operation rounded to
  *   fp32, rint to even: symmetric (zeros_out NULL) scale = round_T(max|w| / 7), code = clamp(rint(w / scale) + 8,

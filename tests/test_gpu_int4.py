@@ -183,6 +183,27 @@ def test_on_a_side_stream_and_in_two_graphs(m):
     assert V.device_status() == 0
 
 
+def test_graphs_captured_on_one_stream_and_replayed_on_two_keep_their_scratch_apart():
+    side = torch.cuda.Stream()
+    jobs = [(acts(77, 4096, F16, seed=1), make(1024, 4096, 128, F16, seed=2)), (acts(70, 4096, F16, seed=3), make(1280, 4096, 64, F16, seed=4))]
+    want = [V.int4_gemm(x, *w) for x, w in jobs]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for x, w in jobs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            got.append([V.int4_gemm(x, *w) for _ in range(8)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, ys in zip(want, got):
+        assert all(torch.equal(y, w) for y in ys)
+
+
 def test_quantised_just_before_the_product():
     for seed in range(8):      # the product reads weights that the kernel in front of it has just written
         w = (torch.randn(512, 1024, generator=torch.Generator().manual_seed(seed)) * 0.05).half().cuda()

@@ -74,6 +74,13 @@ def test_bad_arguments_are_rejected_without_cuda(lib):
     assert ex(t=0) == _lib.OK
 
 
+def test_scratch_is_asked_for_where_pieces_are_summed(lib):
+    """Above 32 rows, and above 16 for weights of more than 2^24 places."""
+    need = lib.vqg_int4_workspace_bytes
+    assert need(16, 8192, 8192) == need(32, 4096, 4096) == need(33, 0, 64) == need(0, 4096, 4096) == 0
+    assert need(17, 4096, 4160) == need(33, 64, 64) > 0
+
+
 def test_python_layer_refuses_cpu_tensors():
     _, packed, scales, _ = _packed(16, 64, 32)
     x = torch.zeros(1, 64, dtype=torch.float16)

@@ -51,14 +51,18 @@ size_t up(size_t n) { return (n + 255) / 256 * 256; }
 // Slots up to which a batch is worked on slot by slot, without ordering it by expert.
 constexpr int kDirectSlots = 32;
 
-// Rows of X from which the dense product goes to the tensor-memory kernel.
-constexpr int kTensorRows = 33;
-// Rows per expert, on average, from which the experts' products do.
-bool experts_on_tensor(long long slots, int E) { return slots >= 16LL * E; }
+// The dense product goes to the tensor-memory kernel above 32 rows, and above 16 where the weight has more than 2^24 places:
+// 32 rows of 4096 x 4096 take 12.2 us in the few-rows kernel and 13.0 in the other, of 1024 x 1024 3.6 and 6.8, of 4096 x
+// 14336 38.8 and 23.5, of 28672 x 8192 89 and 67; 16 rows of 28672 x 8192 54 and 67 (17 rows: 84 and 67).
+bool gemm_on_tensor(int M, int N, int K) { return M > 32 || (M > 16 && static_cast<long long>(N) * K > (1 << 24)); }
+// Rows per expert, on average, from which the experts' products do: 64 experts of 2048 x 1024 take, with the few-rows kernel
+// and with the other, 110 and 125 us at 9 rows, 122 and 125 at 10, 144 and 125 at 11 to 16; 8 of 4096 x 14336 348 and 371 at
+// 10, 459 and 384 at 14.
+bool experts_on_tensor(long long slots, int E) { return slots >= 11LL * E; }
 // Rows of a chunk of an expert's rows: what most experts have, so that few read their weights twice.
 int expert_chunk_rows(long long slots, int E) {
   if (experts_on_tensor(slots, E)) return kInt4TensorRows;
-  return slots <= 5LL * E ? 8 : slots <= 11LL * E ? 16 : 32;
+  return slots <= 5LL * E ? 8 : 16;
 }
 
 struct ExpertScratch {
@@ -82,12 +86,11 @@ ExpertScratch expert_scratch(int T, int top_k, int E, int hidden, int inner) {
 extern "C" {
 
 size_t vqg_int4_workspace_bytes(int M, int N, int K) {
-  return M >= kTensorRows && N > 0 && K > 0 ? int4_tensor_workspace_bytes() : 0;
+  return N > 0 && K > 0 && gemm_on_tensor(M, N, K) ? int4_tensor_workspace_bytes() : 0;
 }
 
 int vqg_int4_gemm(const void* x, const void* packed, const void* scales, const void* zeros, void* y, int M, int N, int K,
                   int group, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-
   if (M < 0) return VQG_ERR_BAD_ARG;
   const int st = check_weight(packed, scales, zeros, 1, N, K, group, dtype);
   if (st != VQG_OK) return st;
@@ -98,8 +101,8 @@ int vqg_int4_gemm(const void* x, const void* packed, const void* scales, const v
   if (!x || !aligned(x, 16)) return VQG_ERR_BAD_ARG;
   if (ensure_status_word() != cudaSuccess) return VQG_ERR_NO_DEVICE;
   const Int4Weight w = weight(packed, scales, zeros, N, K, group);
-  if (M >= kTensorRows) {
-    if (!workspace || workspace_bytes < vqg_int4_workspace_bytes(M, N, K) || !aligned(workspace, 1024)) return VQG_ERR_WORKSPACE;
+  if (gemm_on_tensor(M, N, K)) {
+    if (!workspace || workspace_bytes < vqg_int4_workspace_bytes(M, N, K) || !aligned(workspace, 256)) return VQG_ERR_WORKSPACE;
     return launch_int4_tensor(w, x, y, M, dtype == 1, workspace, workspace_bytes, s);
   }
   return launch_int4_small(w, x, y, M, dtype == 1, s);

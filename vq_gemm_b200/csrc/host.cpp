@@ -63,8 +63,7 @@ Tensor output(const OptTensor& out, at::IntArrayRef shape, const Tensor& like, c
   return *out;
 }
 
-Tensor int4_gemm(const Tensor& x, const Tensor& packed, const Tensor& scales, const OptTensor& zeros, const OptTensor& out,
-                 const OptTensor& workspace) {
+Tensor int4_gemm(const Tensor& x, const Tensor& packed, const Tensor& scales, const OptTensor& zeros, const OptTensor& out) {
   check_cuda(x, x); check_cuda(x, packed); check_cuda(x, scales);
   if (zeros) check_cuda(x, *zeros);
   TORCH_CHECK(x.dim() == 2 && x.scalar_type() == scales.scalar_type(), "x must be [M, K] and of the type of scales");
@@ -73,13 +72,17 @@ Tensor int4_gemm(const Tensor& x, const Tensor& packed, const Tensor& scales, co
   TORCH_CHECK(M < (int64_t(1) << 31), "too many rows");
   c10::cuda::CUDAGuard guard(x.device());
   Tensor y = output(out, {M, w.N}, x, "[M, N] tensor of x's type on the inputs' device");
+  // Scratch belongs to the call: graphs captured on one stream may be replayed on two.
+  const size_t need = vqg_int4_workspace_bytes(static_cast<int>(M), w.N, static_cast<int>(K));
+  Tensor ws;
+  if (need) ws = at::empty({static_cast<int64_t>(need)}, x.options().dtype(at::kByte));
   cudaStream_t s = at::cuda::getCurrentCUDAStream();
   int st;
   {
     pybind11::gil_scoped_release nogil;
     st = vqg_int4_gemm(x.const_data_ptr(), packed.const_data_ptr(), scales.const_data_ptr(), ptr(zeros), y.mutable_data_ptr(),
-                       M, w.N, K, w.group, float_code(x), workspace ? workspace->mutable_data_ptr() : nullptr,
-                       workspace ? workspace->numel() : 0, s);
+                       M, w.N, K, w.group, float_code(x), need ? ws.mutable_data_ptr() : nullptr,
+                       need, s);
   }
   check_status(st, "int4_gemm");
   return y;

@@ -57,7 +57,7 @@ int launch_int4_small_down(const Int4Weight& w, const void* h, float* part, cons
 // y[token, N] = sum over the token's choices of weight * H[slot] W_e^T, direct form
 int launch_int4_small_down_direct(const Int4Weight& w, const void* h, void* y, const ExpertRows& rows, int tokens, bool bf16,
                                   cudaStream_t s);
-constexpr int kInt4SmallRows = 32;   // rows of a chunk of the planned form, at most (8, 16 or 32)
+constexpr int kInt4SmallRows = 32;   // rows of a chunk of the dense product, at most (8, 16 or 32); of an expert's 8 or 16
 
 // Many rows: tcgen05 kernels (int4_tensor.cu).  The dense form deals out K loops evenly if it gets a workspace.
 size_t int4_tensor_workspace_bytes();

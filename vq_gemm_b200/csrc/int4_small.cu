@@ -468,11 +468,8 @@ int launch_rows(const SmallParams& p, int rows, bool bf16, cudaStream_t s) {
         if (x <= 40 * 1024) return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 2, 3, 2, true>(p, rows, s);
         return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 2, 3, 2, false>(p, rows, s);
       }
-      if (rows <= 16) {
-        if (x <= 70 * 1024) return launch_one<F, Z, MODE, 2, 1, 4, 1, 2, 8, 2, 2, 1, true>(p, rows, s);
-        return launch_one<F, Z, MODE, 2, 1, 4, 1, 2, 8, 2, 2, 1, false>(p, rows, s);
-      }
-      return launch_one<F, Z, MODE, 4, 1, 4, 1, 2, 8, 2, 2, 1, false>(p, rows, s);
+      if (x <= 70 * 1024) return launch_one<F, Z, MODE, 2, 1, 4, 1, 2, 8, 2, 2, 1, true>(p, rows, s);
+      return launch_one<F, Z, MODE, 2, 1, 4, 1, 2, 8, 2, 2, 1, false>(p, rows, s);
     }
   };
   if (p.w.zeros) return bf16 ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});

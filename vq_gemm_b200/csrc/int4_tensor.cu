@@ -693,7 +693,7 @@ int launch(int pairs, const void* x, int rows, const TensorParams& p, cudaStream
 }  // namespace
 
 size_t int4_tensor_workspace_bytes() {
-  return kCounterBytes + static_cast<size_t>(sm_pairs()) * kPairPartialBytes;
+  return static_cast<size_t>(sm_pairs()) * kPairPartialBytes;
 }
 
 int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool bf16, void* ws, size_t ws_bytes, cudaStream_t s) {
@@ -706,7 +706,7 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
   if (tiles > 0x7fffffffLL / (stages + 1)) return VQG_ERR_UNSUPPORTED;
   const bool split = ws && reinterpret_cast<uintptr_t>(ws) % 256 == 0 &&
-                     ws_bytes >= kCounterBytes + static_cast<size_t>(max_pairs) * kPairPartialBytes && stages > 1 &&
+                     ws_bytes >= static_cast<size_t>(max_pairs) * kPairPartialBytes && stages > 1 &&
                      tiles % max_pairs != 0;
   p.unit_stages = split ? (stages >= 8 ? 2 : 1) : stages;
   p.units_per_tile = (stages + p.unit_stages - 1) / p.unit_stages;
@@ -714,7 +714,7 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   const int pairs = units < max_pairs ? static_cast<int>(units) : max_pairs;
   p.q = static_cast<int>(units / pairs);
   p.r = static_cast<int>(units % pairs);
-  p.ws_partial = split ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes) : nullptr;
+  p.ws_partial = split ? static_cast<float*>(ws) : nullptr;
   const int st = bf16 ? launch<true, kDense>(pairs, x, M, p, s) : launch<false, kDense>(pairs, x, M, p, s);
   if (st != VQG_OK || !split || pairs == 1) return st;
   const dim3 grid(((M < BM ? M : BM) * 64 + 255) / 256, pairs - 1);

@@ -338,7 +338,6 @@ def _int4_weight(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[tor
 
 
 _host_module = None
-_INT4_FEW_ROWS = 32          # rows up to which vqg_int4_gemm needs no scratch (vqg_int4_workspace_bytes is 0)
 
 
 def _host(tensor: torch.Tensor):
@@ -360,11 +359,7 @@ def int4_gemm(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Y[M, N] = X[M, K] @ W^T for a 4-bit weight with group scales (``quantize.int4_quantize``), fp32 accumulation.
     x, scales and Y are of one type, float16 or bfloat16; group = K // scales.shape[0]."""
-    host = _host(x)
-    ws = None
-    if x.dim() == 2 and x.shape[0] > _INT4_FEW_ROWS:
-        ws = _ws(x.device, _lib.load().vqg_int4_workspace_bytes(x.shape[0], scales.shape[-1], x.shape[1]))
-    return host.int4_gemm(x, packed, scales, zeros, out, ws)
+    return _host(x).int4_gemm(x, packed, scales, zeros, out)
 
 
 def int4_dequant(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None, *,
