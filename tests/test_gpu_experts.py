@@ -172,6 +172,45 @@ def test_a_dropped_slot_ignores_its_weight_and_a_far_scratch_is_not_needed_clean
         check(y, O.experts(x, ids, torch.where(ids < 0, 0.0, w), up, down))
 
 
+@pytest.mark.parametrize("t", [4, 30, 200])
+def test_graphs_captured_on_one_stream_and_replayed_on_two(t):
+    # each call's scratch is its own
+    side, jobs = torch.cuda.Stream(), []
+    for seed in (1, 2):
+        up, down = moe(8, 256, 128, 64, F16, False, seed=seed)
+        x, (ids, w) = acts(t, 256, F16, seed=seed), choices(t, 2, 8, seed=seed)
+        jobs.append((x, ids, w, up, down))
+    want = [V.int4_experts(*j) for j in jobs]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for j in jobs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            got.append([V.int4_experts(*j) for _ in range(6)])
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for y, ys in zip(want, got):
+        assert all(torch.equal(v, y) for v in ys)
+
+
+def test_rows_of_experts_past_32_bits():
+    # 2.2e9 values of all rows' second products; the last and middle tokens against 64 bits
+    t, k, e, hidden, inner = 140_000, 4, 6, 4096, 32
+    up, down = moe(e, hidden, inner, 32, F16, False)
+    x = acts(t, hidden, F16)
+    ids, w = choices(40, k, e, seed=1)
+    ids, w = ids.repeat(t // 40, 1), w.repeat(t // 40, 1)
+    y = V.int4_experts(x, ids, w, up, down)
+    for at in (0, 69_980, t - 20):
+        part = slice(at, at + 20)
+        check(y[part], O.experts(x[part], ids[part], w[part], up, down))
+    assert V.device_status() == 0
+
+
 def test_experts_refusals_and_empty_batch():
     up, down = moe(4, 64, 96, 32, F16, False)
     ids, w = choices(3, 2, 4)
@@ -236,3 +275,12 @@ def test_a_layer_over_another_model_part():
     y = layer(x.cuda())
     w, ids = check_route(layer.router(x.cuda()), 2, renormalize=True)
     check(y, O.experts(x.cuda(), ids, w, up, down))
+
+
+def test_a_layer_cast_with_its_model():
+    up, down = moe(8, 128, 64, 64, F16, False)
+    router = torch.nn.Linear(128, 8, bias=False).requires_grad_(False)
+    layer = Int4Experts(router, up, down, top_k=2, in_features=128, scoring="sigmoid", bias=torch.arange(8.0) / 16).cuda().half()
+    x = acts(5, 128, F16)
+    w, ids = check_route(layer.router(x), 2, scoring="sigmoid", bias=torch.arange(8.0).cuda() / 16, renormalize=True)
+    assert torch.equal(layer(x), V.int4_experts(x, ids, w, up, down))

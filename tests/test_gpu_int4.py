@@ -1,5 +1,7 @@
 """4-bit weights on the GPU against the 64-bit restatement: quantiser and dequantisation bit for bit, products within the
 bound that follows from their sums."""
+import threading
+
 import pytest
 import torch
 
@@ -202,6 +204,73 @@ def test_graphs_captured_on_one_stream_and_replayed_on_two_keep_their_scratch_ap
     torch.cuda.synchronize()
     for w, ys in zip(want, got):
         assert all(torch.equal(y, w) for y in ys)
+
+
+@pytest.mark.parametrize("m", [1, 7, 16, 24, 40, 300])
+def test_tensors_that_start_inside_others(m):
+    # scales 2 bytes, zero points 1 byte, everything else 16 bytes behind a wide boundary
+    n, k = 150, 320
+    packed, scales, zeros = make(n, k, 64, F16, True, seed=m)
+    x = acts(m, k, F16, seed=m)
+    shift = lambda t, by: torch.cat([t.new_zeros(by), t.reshape(-1)])[by:].view(t.shape)
+    w = (shift(packed, 16), shift(scales, 1), shift(zeros, 1))
+    out = torch.full((m * n + 16,), 9.0, dtype=F16, device="cuda")
+    y = V.int4_gemm(shift(x, 8), *w, out=out[8:8 + m * n].view(m, n))
+    assert torch.equal(y, V.int4_gemm(x, packed, scales, zeros))
+    assert bool((out[:8] == 9).all()) and bool((out[8 + m * n:] == 9).all())
+    dense = V.int4_dequant(packed, scales, zeros)
+    assert torch.equal(V.int4_dequant(*w, out=shift(torch.empty_like(dense), 8)), dense)
+    for symmetric in (True, False):
+        a, b = quantize.int4_quantize(dense, group=64, symmetric=symmetric), quantize.int4_quantize(shift(dense, 8), group=64, symmetric=symmetric)
+        assert all((u is None and v is None) or torch.equal(u, v) for u, v in zip(a, b))
+
+
+@pytest.mark.parametrize("m", [1, 20, 40])
+def test_the_longest_rows(m):
+    k = 1 << 19
+    w, x = make(16, k, 64, F16, seed=3), acts(m, k, F16) * 0.25
+    check(V.int4_gemm(x, *w), O.gemm(x, *w))
+    with pytest.raises(RuntimeError):
+        V.int4_gemm(torch.zeros(m, k + 64, dtype=F16, device="cuda"), torch.zeros(1, k // 64 + 1, 512, dtype=torch.uint8, device="cuda"),
+                    torch.zeros(k // 64 + 1, 16, dtype=F16, device="cuda"))
+
+
+def test_outputs_and_weights_past_32_bits():
+    # 2.2e9 results: the last rows are those of the same rows alone (the K loop of a tile is summed in one piece either way)
+    m, n, k = 270_000, 8192, 64
+    w, x = make(n, k, 64, F16, seed=5), acts(m, k, F16)
+    y = V.int4_gemm(x, *w)
+    check(y[-40:], O.gemm(x[-40:], *w))
+    check(y[130_000:130_040], O.gemm(x[130_000:130_040], *w))
+    del x, y
+    # 2.2e9 weights of 18 experts, quantised and read back
+    e, n, k = 18, 15_000, 8192
+    dense = torch.zeros(e, n, k, dtype=BF16, device="cuda")
+    dense[-1, -300:] = acts(300, k, BF16, seed=6) * 0.05
+    q = quantize.int4_quantize(dense, group=128)
+    back = V.int4_dequant(*q)
+    alone = V.int4_dequant(*quantize.int4_quantize(dense[-1, -300:].contiguous(), group=128))
+    assert torch.equal(back[-1, -300:], alone) and not bool(back[:-1].any()) and not bool(back[-1, :-300].any())
+
+
+def test_two_threads_on_streams_of_their_own():
+    jobs = [(acts(m, 512, F16, seed=m), make(400, 512, 128, F16, seed=m)) for m in (2, 60)]
+    want = [V.int4_gemm(x, *w) for x, w in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ys = [V.int4_gemm(jobs[i][0], *jobs[i][1]) for _ in range(200)]
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(1 for y in ys if not torch.equal(y, want[i]))
+
+    threads = [threading.Thread(target=run, args=(i % 2,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and V.device_status() == 0
 
 
 def test_quantised_just_before_the_product():

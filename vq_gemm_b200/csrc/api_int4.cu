@@ -199,7 +199,6 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
     if (st == VQG_OK) st = launch_int4_tensor_gated(gu, ws + at.rows, h, rows, most, bf16, s);
     if (st == VQG_OK) st = launch_int4_tensor_down(dn, h, part, rows, most, bf16, s);
   } else {
-    if (most > 65535) return VQG_ERR_UNSUPPORTED;
     st = launch_int4_small_gated(gu, x, h, rows, chunk, most, bf16, s);
     if (st == VQG_OK) st = launch_int4_small_down(dn, h, part, rows, chunk, most, bf16, s);
   }

@@ -359,8 +359,9 @@ class Int4Experts(nn.Module):
             raise RuntimeError(f"last dimension {x.shape[-1]} != in_features {self.in_features}")
         x2 = x.reshape(-1, self.in_features)
         logits = self.router(x2).contiguous()
+        bias = None if self.bias is None else self.bias.float()       # (``.to(dtype)`` of a model casts every buffer)
         weights, chosen = torch.ops.vq_gemm_b200.route_experts(
-            logits, self.top_k, self.scoring, self.bias, self.groups, self.top_groups, self.group_score, self.renormalize,
+            logits, self.top_k, self.scoring, bias, self.groups, self.top_groups, self.group_score, self.renormalize,
             self.scale)
         y = torch.ops.vq_gemm_b200.int4_experts(
             x2.to(self.gate_up_scales.dtype).contiguous(), chosen, weights, self.gate_up_packed, self.gate_up_scales,
