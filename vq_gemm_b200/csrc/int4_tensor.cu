@@ -9,9 +9,9 @@
 // Roles per CTA (512 threads, four warpgroups):
 //   warp 0       TMA producer of X: this CTA's half of the rows, boxes of 32 rows x 64 columns, SWIZZLE_128B
 //   warp 1       pair leader: issues the MMAs and commits; other CTA: forwards "my operands are in place"
-//   warp 2       producer of packed weights: bulk copies of whole tiles into a ring of its own
+//   warp 2       producer of packed weights: whole tiles by TMA into a ring of its own
 //   warps 4..7   epilogue
-//   warps 8..15  decoding; warps 8..11 the even, 12..15 the odd 64-column steps of a stage
+//   warps 8..15  decoding; warps 8..11 the even, 12..15 the odd stages
 //
 // Rows of a tile: 256 at most, rounded up to 32 for the instruction, so a short tile costs what it needs on the tensor pipe.
 // Tensor memory: columns [0, 256) accumulator, [256 + 64 s, +64) A stage s (two 64-column steps).
@@ -34,7 +34,8 @@ constexpr int BNH = 128, BN = 256;       // weight rows per CTA and per pair
 constexpr int BK = 64, KS = 2;           // columns per step, steps per stage
 constexpr int STAGES = 4;
 constexpr int kThreads = 512;
-constexpr int kDecodeWarps = 8;
+constexpr int kStageWarps = 4;           // decoding warps of a stage: warps 8 ... 11 of the even, 12 ... 15 of the odd ones
+static_assert(STAGES % 2 == 0, "a stage is always the same warps'");
 constexpr uint32_t kXStep = 128 * BK * 2;                 // 16 KiB: 128 rows x 64 columns
 constexpr uint32_t kXStage = KS * kXStep;
 constexpr uint32_t kPStage = (BNH / 16) * KS * 512;       // 8 KiB of packed weights
@@ -142,6 +143,18 @@ __device__ __forceinline__ void mma_pair_ts(uint32_t d, uint32_t a, uint64_t bde
       ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+// arrives at the barrier of both CTAs when the instructions so far are done
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\t"
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}"
+      ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -152,11 +165,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
@@ -173,7 +188,8 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
 
 template <bool BF16, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_x32, const TensorParams p) {
+int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_x32,
+                   const __grid_constant__ CUtensorMap tmap_w, const TensorParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
   extern __shared__ unsigned char smem_dyn[];
@@ -197,12 +213,12 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      // full: X has landed (one arrival and its bytes), eight decoding warps have written their columns; in the leader one
+      // full: X has landed (one arrival and its bytes), four decoding warps have written their columns; in the leader one
       // more arrival says the same of the other CTA
-      mbar_init(bar_full(s), 1 + kDecodeWarps + (rank == 0 ? 1 : 0));
+      mbar_init(bar_full(s), 1 + kStageWarps + (rank == 0 ? 1 : 0));
       mbar_init(bar_empty(s), 1);
       mbar_init(bar_pfull(s), 1);
-      mbar_init(bar_pempty(s), kDecodeWarps);
+      mbar_init(bar_pempty(s), kStageWarps);
     }
     mbar_init(bar_acc_full, 1);
     mbar_init(bar_acc_empty, 8);
@@ -249,72 +265,73 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         }
       }
     } else if (warp == 1) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      Walk<MODE> walk(pair_id, n_pairs, p);
+      Segment g;
+      if (rank == 0) {
+        // ------------------------------- MMA issuer -------------------------------------------
+        // The whole warp walks and one lane issues: what the instructions take is then the same in all lanes, and the compiler
+        // keeps it where they want it.
+        const uint32_t d_t = __shfl_sync(0xffffffffu, tmem_base, 0);
+        uint32_t acc_phase = 0;
+        while (ok && walk.next(g, p)) {
+          // A and B of type fp16 (0) or bf16 (1), D fp32, both K-major
+          const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) |
+                                 (static_cast<uint32_t>(mma_rows(g.rows) >> 3) << 17) | (static_cast<uint32_t>(BN >> 4) << 24);
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_acc_empty, acc_phase ^ 1, p.status, DS_ACC_EMPTY_TIMEOUT));
+          if (!ok) break;
+          tc_fence_after();
+          for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(bar_full(stage), phase, p.status, DS_TMA_FULL_TIMEOUT));
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t a_t = d_t + kAccCols + static_cast<uint32_t>(stage) * kStageCols;
+#pragma unroll
+              for (int u = 0; u < KS; ++u) {
+                const uint64_t bd = make_desc(base + stage * kXStage + u * kXStep);
+#pragma unroll
+                for (int k = 0; k < BK / 16; ++k)
+                  mma_pair_ts(d_t, a_t + u * (BK / 2) + 8 * k, bd + 2 * k, idesc, ((kt - g.kt_begin) | u | k) != 0 ? 1u : 0u);
+              }
+              tc_commit_both(bar_empty(stage));
+              if (kt + 1 == g.kt_end) tc_commit_both(bar_acc_full);
+            }
+            __syncwarp();
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+          acc_phase ^= 1;
+        }
+      } else if (lane == 0) {
+        // ------------------------------- forwarder --------------------------------------------
+        while (ok && walk.next(g, p)) {
+          for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+            if (!(ok = mbar_wait(bar_full(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
+            mbar_arrive_remote(bar_full(stage) + to_peer);
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          }
+        }
+      }
+    } else if (warp == 2) {
+      // ------------------------------- packed-weight producer -----------------------------------
+      // one copy per stage: eight row tiles x KS column tiles (eight bulk copies of a row tile each, one per lane, took 1150 cycles
+      // of issue a stage, more than anything else in it).  Row tiles behind the last one are another expert's, or zero.
       if (lane == 0) {
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
         Walk<MODE> walk(pair_id, n_pairs, p);
         Segment g;
-        if (rank == 0) {
-          // ------------------------------- MMA issuer -----------------------------------------
-          uint32_t acc_phase = 0;
-          while (ok && walk.next(g, p)) {
-            // A and B of type fp16 (0) or bf16 (1), D fp32, both K-major
-            const uint32_t idesc = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) |
-                                   (static_cast<uint32_t>(mma_rows(g.rows) >> 3) << 17) | (static_cast<uint32_t>(BN >> 4) << 24);
-            if (!(ok = mbar_wait_cluster(bar_acc_empty, acc_phase ^ 1, p.status, DS_ACC_EMPTY_TIMEOUT))) break;
-            tc_fence_after();
-            for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
-              if (!(ok = mbar_wait_cluster(bar_full(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
-              tc_fence_after();
-              const uint32_t a_t = tmem_base + kAccCols + static_cast<uint32_t>(stage) * kStageCols;
-#pragma unroll
-              for (int u = 0; u < KS; ++u) {
-                const uint64_t bd = make_desc(base + stage * kXStage + u * kXStep);
-#pragma unroll
-                for (int k = 0; k < BK / 16; ++k)
-                  mma_pair_ts(tmem_base, a_t + u * (BK / 2) + 8 * k, bd + 2 * k, idesc, ((kt - g.kt_begin) | u | k) != 0 ? 1u : 0u);
-              }
-              tc_commit_pair(bar_empty(stage));
-              tc_commit_pair(bar_empty(stage) + to_peer);
-              if (++stage == STAGES) { stage = 0; phase ^= 1; }
-            }
-            if (!ok) break;
-            tc_commit_pair(bar_acc_full);
-            tc_commit_pair(bar_acc_full + to_peer);
-            acc_phase ^= 1;
+        while (ok && walk.next(g, p)) {
+          const int tile0 = g.expert * w.row_tiles() + (g.n0 + static_cast<int>(rank) * BNH) / 16;
+          for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
+            if (!(ok = mbar_wait(bar_pempty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
+            mbar_expect_tx(bar_pfull(stage), kPStage);
+            tma_load_3d(base + kPacked + stage * kPStage, &tmap_w, 0, kt * KS, tile0, bar_pfull(stage));
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
           }
-        } else {
-          // ------------------------------- forwarder ------------------------------------------
-          while (ok && walk.next(g, p)) {
-            for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
-              if (!(ok = mbar_wait(bar_full(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
-              mbar_arrive_remote(bar_full(stage) + to_peer);
-              if (++stage == STAGES) { stage = 0; phase ^= 1; }
-            }
-          }
-        }
-      }
-    } else if (warp == 2) {
-      // ------------------------------- packed-weight producer -----------------------------------
-      // lane i copies the stage's columns of row tile i
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      Walk<MODE> walk(pair_id, n_pairs, p);
-      Segment g;
-      const int k_tiles = w.k_tiles();
-      while (ok && walk.next(g, p)) {
-        const int tile0 = (g.n0 + static_cast<int>(rank) * BNH) / 16;
-        const int tiles = max(0, min(BNH / 16, w.row_tiles() - tile0));
-        const uint8_t* src = w.packed + g.expert * w.expert_bytes() + static_cast<long long>(tile0 + lane) * k_tiles * 512;
-        for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
-          if (!(ok = mbar_wait(bar_pempty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
-          const uint32_t bytes = min(KS, k_tiles - kt * KS) * 512;
-          if (lane == 0) mbar_expect_tx(bar_pfull(stage), tiles * bytes);
-          __syncwarp();
-          if (lane < tiles) bulk_load(base + kPacked + stage * kPStage + lane * (KS * 512), src + kt * (KS * 512), bytes, bar_pfull(stage));
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
     }
@@ -512,83 +529,105 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     if constexpr (MODE == kDown) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // every copy is complete
   } else {
     // ------------------------------- decoding -----------------------------------------------------
-    const int quarter = warp & 3, sub = (warp - 8) >> 2;       // the step of a stage that this warp decodes
+    // A warp takes every other stage whole: the waits, the handing over and the scales' bookkeeping of a stage take as long as the
+    // arithmetic of one of its steps.
+    const int quarter = warp & 3, parity = (warp - 8) >> 2;
     const int r = row_of_lane(quarter, lane);                  // weight row in the CTA
-    const uint32_t src = base + kPacked + (r / 16) * (KS * 512) + sub * 512 + (r & 7) * 16;
-    const uint32_t a_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols + sub * (BK / 2);
-    int stage = 0;
-    uint32_t phase = 0;
+    const uint32_t src = base + kPacked + (r / 16) * (KS * 512) + (r & 7) * 16;
+    const uint32_t a_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols;
+    uint32_t done = 0;                                         // stages before the segment
     bool ok = true;
     Walk<MODE> walk(pair_id, n_pairs, p);
     Segment g;
     const bool halves = w.group == 32;                         // columns 0 ... 31 and 32 ... 63 of a step have scales of their own
+    const bool whole = w.group % (KS * BK) == 0;               // the steps of a stage share theirs
     while (ok && walk.next(g, p)) {
       const int n = g.n0 + static_cast<int>(rank) * BNH + r;
       const bool row_ok = n < w.N;
-      // Scales and zero points, two stages ahead and as loaded: nothing is computed from them before the stage in hand is done, or
-      // the warp would wait for memory here.  Rows and columns that do not exist read the last ones and get a scale of zero, so
-      // that no fill reaches a sum.
+      // Scales and zero points, two of the warp's stages ahead and as loaded: nothing is computed from them before the stage in hand
+      // is done, or the warp would wait for memory here.  Rows and columns that do not exist read the last ones and get a scale of
+      // zero, so that no fill reaches a sum.
       const int nc = min(n, w.N - 1);
       const unsigned short* sc = static_cast<const unsigned short*>(w.scales) + g.expert * w.expert_scales() + nc;
       const uint8_t* ze = w.zeros ? w.zeros + g.expert * w.expert_scales() + nc : nullptr;
       struct Raw {
-        unsigned short s[2];
-        uint8_t z[2];
+        unsigned short s[KS][2];
+        uint8_t z[KS][2];
       };
-      auto fetch = [&](int kt) {
-        Raw f{{0, 0}, {8, 8}};
-        const int k = (kt * KS + sub) * BK;
-        const int at = int4_group_of(w, min(k, w.K - 32)) * w.N;
-        f.s[0] = __ldg(sc + at);
-        if (ze) f.z[0] = __ldg(ze + at);
-        if (halves) {
-          const int at2 = int4_group_of(w, min(k + 32, w.K - 32)) * w.N;
-          f.s[1] = __ldg(sc + at2);
-          if (ze) f.z[1] = __ldg(ze + at2);
-        }
-        return f;
+      auto fetch = [&](Raw& f, int kt) {   // only the loads: a copy of what is on its way would wait for it
+#pragma unroll
+        for (int u = 0; u < KS; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if ((u == 0 || !whole) && (h == 0 || halves)) {
+              const int at = int4_group_of(w, min((kt * KS + u) * BK + 32 * h, w.K - 32)) * w.N;
+              f.s[u][h] = __ldg(sc + at);
+              if (ze) f.z[u][h] = __ldg(ze + at);
+            }
       };
-      Raw next = fetch(g.kt_begin), after = fetch(g.kt_begin + 1);
-      for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
-        const int k = (kt * KS + sub) * BK;
-        const Raw now = next;
-        next = after;
-        after = fetch(kt + 2);
-        uint32_t s2[2], off[2];
-        s2[0] = row_ok && k < w.K ? now.s[0] * 0x10001u : 0u;
-        s2[1] = row_ok && k + 32 < w.K ? (halves ? now.s[1] : now.s[0]) * 0x10001u : 0u;
-        const int z0 = now.z[0] & 15, z1 = halves ? now.z[1] & 15 : z0;
-        if (!(ok = mbar_wait(bar_pfull(stage), phase, p.status, DS_TMA_FULL_TIMEOUT))) break;
-        uint32_t c[16], a[32];
+      const uint32_t first = done - static_cast<uint32_t>(g.kt_begin);      // stage of column tile kt: first + kt
+      int kt = g.kt_begin + static_cast<int>((done ^ static_cast<uint32_t>(parity)) & 1u);
+      done += static_cast<uint32_t>(g.kt_end - g.kt_begin);
+      // one stage; f holds its scales and gets those of the stage after the warp's next one
+      auto decode = [&](Raw& f, int kt) -> bool {
+        const uint32_t it = first + static_cast<uint32_t>(kt), stage = it % STAGES, phase = it / STAGES & 1u;
+        uint32_t s2[KS][2], off[KS][2];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(c[4 * t]), "=r"(c[4 * t + 1]), "=r"(c[4 * t + 2]), "=r"(c[4 * t + 3])
-                       : "r"(src + stage * kPStage + t * 128));
-        if (quarter < 2) {
-          off[0] = I::offset(z0); off[1] = I::offset(z1);
+        for (int u = 0; u < KS; ++u)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            a[2 * i] = int4_pair<BF16, 0, 0>(c[i], off[i >> 3], s2[i >> 3]);
-            a[2 * i + 1] = int4_pair<BF16, 0, 1>(c[i], off[i >> 3], s2[i >> 3]);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t scale = whole ? f.s[0][0] : halves ? f.s[u][h] : f.s[u][0];
+            const int zero = !ze ? 8 : (whole ? f.z[0][0] : halves ? f.z[u][h] : f.z[u][0]) & 15;
+            s2[u][h] = row_ok && (kt * KS + u) * BK + 32 * h < w.K ? scale * 0x10001u : 0u;
+            off[u][h] = quarter < 2 ? I::offset(zero) : int4_offset_hi<BF16>(zero);
           }
-        } else {
-          off[0] = int4_offset_hi<BF16>(z0); off[1] = int4_offset_hi<BF16>(z1);
+        fetch(f, kt + 4);
+        if (!mbar_wait(bar_pfull(stage), phase, p.status, DS_TMA_FULL_TIMEOUT)) return false;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            a[2 * i] = int4_pair_hi<BF16, 0>(c[i], off[i >> 3], s2[i >> 3]);
-            a[2 * i + 1] = int4_pair_hi<BF16, 1>(c[i], off[i >> 3], s2[i >> 3]);
+        for (int u = 0; u < KS; ++u) {
+          uint32_t c[16], a[32];
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(c[4 * t]), "=r"(c[4 * t + 1]), "=r"(c[4 * t + 2]), "=r"(c[4 * t + 3])
+                         : "r"(src + stage * kPStage + u * 512 + t * 128));
+          if (quarter < 2) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              a[2 * i] = int4_pair<BF16, 0, 0>(c[i], off[u][i >> 3], s2[u][i >> 3]);
+              a[2 * i + 1] = int4_pair<BF16, 0, 1>(c[i], off[u][i >> 3], s2[u][i >> 3]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              a[2 * i] = int4_pair_hi<BF16, 0>(c[i], off[u][i >> 3], s2[u][i >> 3]);
+              a[2 * i + 1] = int4_pair_hi<BF16, 1>(c[i], off[u][i >> 3], s2[u][i >> 3]);
+            }
           }
+          if (u == 0) {
+            if (!mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT)) return false;
+            tc_fence_after();
+          }
+          __syncwarp();
+          tmem_st32(a_lane + stage * kStageCols + u * (BK / 2), a);
         }
-        __syncwarp();
         if (lane == 0) mbar_arrive(bar_pempty(stage));
-        if (!(ok = mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT))) break;
-        tc_fence_after();
-        tmem_st32(a_lane + static_cast<uint32_t>(stage) * kStageCols, a);
+        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_full(stage));
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        return true;
+      };
+      // (two sets of scales in turn, not one handed to the other: a move would wait for the load)
+      Raw even{}, odd{};
+      fetch(even, kt);
+      fetch(odd, kt + 2);
+      while (kt < g.kt_end) {
+        if (!(ok = decode(even, kt))) break;
+        kt += 2;
+        if (kt >= g.kt_end) break;
+        if (!(ok = decode(odd, kt))) break;
+        kt += 2;
       }
     }
   }
@@ -677,6 +716,17 @@ bool make_x_map(CUtensorMap* map, const void* ptr, int rows, int cols, int box_r
             strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// packed weights as [row tiles][column tiles][128 words], box of a stage of a CTA: whole tiles
+bool make_w_map(CUtensorMap* map, const Int4Weight& w, int experts) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t k = w.k_tiles();
+  const cuuint64_t dims[3] = {128, k, static_cast<cuuint64_t>(w.row_tiles()) * experts}, strides[2] = {512, k * 512};
+  const cuuint32_t box[3] = {128, KS, BNH / 16}, estr[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t*>(w.packed), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 int sm_pairs() { return max(1, sm_count_cached() / 2); }
 constexpr size_t kPairPartialBytes = 2 * 2 * static_cast<size_t>(BM) * BNH * sizeof(float);
 
@@ -684,10 +734,11 @@ template <bool BF16, int MODE>
 int launch(int pairs, const void* x, int rows, const TensorParams& p, cudaStream_t s) {
   static SmemOptIn opt_in;
   auto kernel = int4_tensor_kernel<BF16, MODE>;
-  CUtensorMap map, map32;
-  if (!make_x_map(&map, x, rows, p.w.K, 128, BF16) || !make_x_map(&map32, x, rows, p.w.K, 32, BF16) || !opt_in.ask(kernel))
+  CUtensorMap map, map32, map_w;
+  if (!make_x_map(&map, x, rows, p.w.K, 128, BF16) || !make_x_map(&map32, x, rows, p.w.K, 32, BF16) ||
+      !make_w_map(&map_w, p.w, MODE == kDense ? 1 : p.rows.E) || !opt_in.ask(kernel))
     return VQG_ERR_LAUNCH;
-  return cuda_status(launch_ahead(kernel, dim3(2 * pairs), kThreads, kSmem + 1024, s, false, map, map32, p));
+  return cuda_status(launch_ahead(kernel, dim3(2 * pairs), kThreads, kSmem + 1024, s, false, map, map32, map_w, p));
 }
 
 }  // namespace
