@@ -61,7 +61,7 @@ bool gemm_on_tensor(int M, int N, int K) { return M > 32 || (M > 16 && static_ca
 bool experts_on_tensor(long long slots, int E) { return slots >= 11LL * E; }
 // Rows of a chunk of an expert's rows: what most experts have, so that few read their weights twice.
 int expert_chunk_rows(long long slots, int E) {
-  if (experts_on_tensor(slots, E)) return kInt4TensorRows;
+  if (experts_on_tensor(slots, E)) return slots <= 96LL * E ? 128 : kInt4TensorRows;
   return slots <= 5LL * E ? 8 : 16;
 }
 
@@ -196,8 +196,8 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
   rows.row_slot = row_slot; rows.chunks = chunks; rows.n_chunks = n_chunks;
   if (tensor) {
     st = launch_gather_rows(x, rows, ws + at.rows, hidden, s);
-    if (st == VQG_OK) st = launch_int4_tensor_gated(gu, ws + at.rows, h, rows, most, bf16, s);
-    if (st == VQG_OK) st = launch_int4_tensor_down(dn, h, part, rows, most, bf16, s);
+    if (st == VQG_OK) st = launch_int4_tensor_gated(gu, ws + at.rows, h, rows, chunk, most, bf16, s);
+    if (st == VQG_OK) st = launch_int4_tensor_down(dn, h, part, rows, chunk, most, bf16, s);
   } else {
     st = launch_int4_small_gated(gu, x, h, rows, chunk, most, bf16, s);
     if (st == VQG_OK) st = launch_int4_small_down(dn, h, part, rows, chunk, most, bf16, s);

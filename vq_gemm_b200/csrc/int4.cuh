@@ -62,10 +62,10 @@ constexpr int kInt4SmallRows = 32;   // rows of a chunk of the dense product, at
 // Many rows: tcgen05 kernels (int4_tensor.cu).  The dense form deals out K loops evenly if it gets a workspace.
 size_t int4_tensor_workspace_bytes();
 int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool bf16, void* ws, size_t ws_bytes, cudaStream_t s);
-// rows of a plan with chunks of up to kInt4TensorRows; x_rows is X in the order of the plan (launch_gather_rows)
-int launch_int4_tensor_gated(const Int4Weight& w, const void* x_rows, void* h, const ExpertRows& rows, int max_chunks, bool bf16,
+// rows of a plan with chunks of up to chunk_rows, kInt4TensorRows at most; x_rows is X in the order of the plan (launch_gather_rows)
+int launch_int4_tensor_gated(const Int4Weight& w, const void* x_rows, void* h, const ExpertRows& rows, int chunk_rows, int max_chunks, bool bf16,
                              cudaStream_t s);
-int launch_int4_tensor_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int max_chunks, bool bf16,
+int launch_int4_tensor_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int chunk_rows, int max_chunks, bool bf16,
                             cudaStream_t s);
 int launch_gather_rows(const void* x, const ExpertRows& rows, void* out, int cols, cudaStream_t s);
 constexpr int kInt4TensorRows = 256;

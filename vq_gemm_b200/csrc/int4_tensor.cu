@@ -29,25 +29,35 @@ using namespace tc;
 
 namespace {
 
-constexpr int BM = 256;                  // rows of X per tile, at most
+constexpr int kRows = 256;               // rows of X per tile, at most
 constexpr int BNH = 128, BN = 256;       // weight rows per CTA and per pair
 constexpr int BK = 64, KS = 2;           // columns per step, steps per stage
-constexpr int STAGES = 4;
-constexpr int kThreads = 512;
-constexpr int kStageWarps = 4;           // decoding warps of a stage: warps 8 ... 11 of the even, 12 ... 15 of the odd ones
-static_assert(STAGES % 2 == 0, "a stage is always the same warps'");
-constexpr uint32_t kXStep = 128 * BK * 2;                 // 16 KiB: 128 rows x 64 columns
-constexpr uint32_t kXStage = KS * kXStep;
 constexpr uint32_t kPStage = (BNH / 16) * KS * 512;       // 8 KiB of packed weights
-constexpr uint32_t kTmemCols = 512, kAccCols = 256, kStageCols = KS * BK / 2;
-constexpr uint32_t kPacked = STAGES * kXStage;
-constexpr uint32_t kStaging = kPacked + STAGES * kPStage; // [256 rows][128 weight rows] of 16 bits
-constexpr uint32_t kBars = kStaging + BM * BNH * 2;
-constexpr uint32_t kNumBars = 4 * STAGES + 3;             // full, empty, packed full, packed empty; accumulator full, empty; epilogue
-constexpr uint32_t kTmemSlot = kBars + (kNumBars + 1) / 2 * 16;
-constexpr uint32_t kSmem = kTmemSlot + 16;
-static_assert(kSmem + 1024 <= 227 * 1024, "shared memory");
-static_assert(kAccCols + STAGES * kStageCols <= kTmemCols, "tensor memory");
+constexpr uint32_t kTmemCols = 512, kStageCols = KS * BK / 2;
+
+// What the kernel consists of for tiles of up to 256 rows of X, and of up to 128 (SHORT).  Decoding a stage is a chain of waits and
+// of arithmetic that a warp does one after the other, some 900 cycles, whatever the rows; the epilogue of a short tile leaves the
+// registers for twice as many warps that do it.
+template <bool SHORT>
+struct Shape {
+  static constexpr int ROWS = SHORT ? 128 : kRows;
+  static constexpr int STAGES = SHORT ? 6 : 4;
+  static constexpr int GROUPS = SHORT ? 4 : 2;              // groups of four decoding warps, which take the stages in turn
+  static constexpr int THREADS = 256 + 128 * GROUPS;
+  static constexpr int OTHER_REGS = 40, EPILOGUE_REGS = SHORT ? 120 : 208;   // decoding: as launched, 80 or 128
+  static constexpr uint32_t X_STEP = ROWS / 2 * BK * 2;     // half the rows x 64 columns
+  static constexpr uint32_t X_STAGE = KS * X_STEP;
+  static constexpr uint32_t PACKED = STAGES * X_STAGE;
+  static constexpr uint32_t STAGING = PACKED + STAGES * kPStage;             // [256 rows][128 weight rows] of 16 bits, 128 of 32
+  static constexpr uint32_t BARS = STAGING + kRows * BNH * 2;
+  static constexpr uint32_t NUM_BARS = 4 * STAGES + 3;      // full, empty, packed full, packed empty; accumulator full, empty; epilogue
+  static constexpr uint32_t TMEM_SLOT = BARS + (NUM_BARS + 1) / 2 * 16;
+  static constexpr uint32_t SMEM = TMEM_SLOT + 16;
+  static_assert(SMEM + 1024 <= 227 * 1024, "shared memory");
+  static_assert(ROWS + STAGES * kStageCols <= kTmemCols, "tensor memory");
+  static constexpr int LAUNCH_REGS = 65536 / THREADS / 8 * 8;
+  static_assert(128 * (OTHER_REGS + EPILOGUE_REGS + GROUPS * LAUNCH_REGS) <= THREADS * LAUNCH_REGS, "registers of the launch");
+};
 
 enum { kDense = 0, kGated = 1, kDown = 2 };
 
@@ -115,8 +125,8 @@ struct Walk {
       g.kt_end = min((end - t0) * p.unit_stages, stages);
       g.whole = g.start == t0 && end == t0 + p.units_per_tile;
       g.expert = 0;
-      g.row0 = (g.tile % p.m_tiles) * BM;
-      g.rows = min(BM, p.M - g.row0);
+      g.row0 = (g.tile % p.m_tiles) * kRows;
+      g.rows = min(kRows, p.M - g.row0);
       g.n0 = (g.tile / p.m_tiles) * BN;
     } else {
       g.tile = g.start = lo;
@@ -155,7 +165,14 @@ __device__ __forceinline__ void tc_commit_both(uint32_t bar) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}"
       ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
       "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -186,12 +203,15 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
   }
 }
 
-template <bool BF16, int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <bool BF16, int MODE, bool SHORT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Shape<SHORT>::THREADS, 1)
 int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_x32,
                    const __grid_constant__ CUtensorMap tmap_w, const TensorParams p) {
   using I = Int4Type<BF16>;
   using T = typename I::T;
+  using C = Shape<SHORT>;
+  constexpr int BM = C::ROWS, STAGES = C::STAGES;
+  constexpr uint32_t kXStep = C::X_STEP, kXStage = C::X_STAGE, kPacked = C::PACKED, kStaging = C::STAGING, kBars = C::BARS, kAccCols = BM;
   extern __shared__ unsigned char smem_dyn[];
   const uint32_t raw = smem_u32(smem_dyn);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -209,16 +229,16 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   const uint32_t bar_acc_empty = base + kBars + 8 * (4 * STAGES + 1);
   const uint32_t bar_epi = base + kBars + 8 * (4 * STAGES + 2);
   const uint32_t to_peer = map_to_cta(base, rank ^ 1u) - base;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + kTmemSlot);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + C::TMEM_SLOT);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       // full: X has landed (one arrival and its bytes), four decoding warps have written their columns; in the leader one
       // more arrival says the same of the other CTA
-      mbar_init(bar_full(s), 1 + kStageWarps + (rank == 0 ? 1 : 0));
+      mbar_init(bar_full(s), 1 + 4 + (rank == 0 ? 1 : 0));
       mbar_init(bar_empty(s), 1);
       mbar_init(bar_pfull(s), 1);
-      mbar_init(bar_pempty(s), kStageWarps);
+      mbar_init(bar_pempty(s), 4);
     }
     mbar_init(bar_acc_full, 1);
     mbar_init(bar_acc_empty, 8);
@@ -227,7 +247,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     fence_async_smem();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + kTmemSlot), "r"(kTmemCols)
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + C::TMEM_SLOT), "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -240,7 +260,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   grid_wait();
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
     if (warp == 0) {
       // ------------------------------- X producer ---------------------------------------------
       // the whole warp walks; lane u * boxes + b issues one box (a single lane would need longer than a stage takes)
@@ -251,9 +271,9 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       Segment g;
       while (ok && walk.next(g, p)) {
         const int half = mma_rows(g.rows) / 2;
-        const int boxes = half > 64 ? 1 : (half + 31) / 32;       // one box of 128 rows, or one or two of 32
-        const CUtensorMap* map = half > 64 ? &tmap_x : &tmap_x32;
-        const int box_rows = half > 64 ? 128 : 32;
+        const int boxes = BM > 128 && half > 64 ? 1 : (half + 31) / 32;       // one box of 128 rows, or one or two of 32
+        const CUtensorMap* map = BM > 128 && half > 64 ? &tmap_x : &tmap_x32;
+        const int box_rows = BM > 128 && half > 64 ? 128 : 32;
         const int u = lane / boxes, b = lane % boxes;
         const int row = g.row0 + static_cast<int>(rank) * half + 32 * b;
         for (int kt = g.kt_begin; kt < g.kt_end; ++kt) {
@@ -338,7 +358,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
   } else if (warp < 8) {
     // ------------------------------- epilogue -----------------------------------------------------
     // lane = weight row, column = row of X
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::EPILOGUE_REGS));
     const int quarter = warp & 3, my_row = row_of_lane(quarter, lane);
     uint32_t acc_phase = 0, epi_phase = 0;
     bool ok = true;
@@ -358,7 +378,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     };
     constexpr int OUT_COLS = MODE == kGated ? BNH / 2 : BNH;   // output columns of this CTA's half tile
     constexpr int ROW_BYTES = OUT_COLS * 2;
-    constexpr size_t kPartialFloats = static_cast<size_t>(BM) * BNH;
+    constexpr size_t kPartialFloats = static_cast<size_t>(kRows) * BNH;
     Walk<MODE> walk(pair_id, n_pairs, p);
     Segment g;
     while (ok && walk.next(g, p)) {
@@ -392,7 +412,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
           ok = epi_sync();
         };
         uint32_t late[4][32];
-        if (cols > 128) {
+        if (BM > 128 && cols > 128) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (128 + 32 * i < cols) tmem_ld32_async(t_row + 128 + 32 * i, late[i]);
@@ -405,11 +425,13 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 32; ++j) col[(c + j) * BNH] = __uint_as_float(r[j]);
         }
+        if constexpr (BM > 128) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld_wait(late[i]);
+          for (int i = 0; i < 4; ++i) tmem_ld_wait(late[i]);
+        }
         release();
         send(0);
-        if (ok && cols > 128) {
+        if (BM > 128 && ok && cols > 128) {
           sent();
           if (ok) {
 #pragma unroll
@@ -529,9 +551,10 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     if constexpr (MODE == kDown) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // every copy is complete
   } else {
     // ------------------------------- decoding -----------------------------------------------------
-    // A warp takes every other stage whole: the waits, the handing over and the scales' bookkeeping of a stage take as long as the
+    // A warp takes every second or fourth stage whole: the waits, the handing over and the scales' bookkeeping of a stage take as long as the
     // arithmetic of one of its steps.
-    const int quarter = warp & 3, parity = (warp - 8) >> 2;
+    constexpr int GROUPS = C::GROUPS;
+    const int quarter = warp & 3, group = (warp - 8) >> 2;
     const int r = row_of_lane(quarter, lane);                  // weight row in the CTA
     const uint32_t src = base + kPacked + (r / 16) * (KS * 512) + (r & 7) * 16;
     const uint32_t a_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kAccCols;
@@ -543,7 +566,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     const bool whole = w.group % (KS * BK) == 0;               // the steps of a stage share theirs
     while (ok && walk.next(g, p)) {
       const int n = g.n0 + static_cast<int>(rank) * BNH + r;
-      const bool row_ok = n < w.N;
+      const uint32_t twice = n < w.N ? 0x10001u : 0u;
       // Scales and zero points, two of the warp's stages ahead and as loaded: nothing is computed from them before the stage in hand
       // is done, or the warp would wait for memory here.  Rows and columns that do not exist read the last ones and get a scale of
       // zero, so that no fill reaches a sum.
@@ -566,50 +589,68 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             }
       };
       const uint32_t first = done - static_cast<uint32_t>(g.kt_begin);      // stage of column tile kt: first + kt
-      int kt = g.kt_begin + static_cast<int>((done ^ static_cast<uint32_t>(parity)) & 1u);
+      int kt = g.kt_begin + static_cast<int>((static_cast<uint32_t>(group) - done) % GROUPS);
       done += static_cast<uint32_t>(g.kt_end - g.kt_begin);
       // one stage; f holds its scales and gets those of the stage after the warp's next one
       auto decode = [&](Raw& f, int kt) -> bool {
-        const uint32_t it = first + static_cast<uint32_t>(kt), stage = it % STAGES, phase = it / STAGES & 1u;
+        const uint32_t it = first + static_cast<uint32_t>(kt), stage = it % STAGES, phase = (it / STAGES) & 1u;
         uint32_t s2[KS][2], off[KS][2];
+        auto offset = [&](int zero) { return quarter < 2 ? I::offset(zero) : int4_offset_hi<BF16>(zero); };
+        if (whole && (kt + 1) * (KS * BK) <= w.K) {            // (a few instructions instead of some eighty in a row)
+          const uint32_t scale = f.s[0][0] * twice, o = ze ? offset(f.z[0][0] & 15) : offset(8);
 #pragma unroll
-        for (int u = 0; u < KS; ++u)
+          for (int i = 0; i < 2 * KS; ++i) { s2[i >> 1][i & 1] = scale; off[i >> 1][i & 1] = o; }
+        } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t scale = whole ? f.s[0][0] : halves ? f.s[u][h] : f.s[u][0];
-            const int zero = !ze ? 8 : (whole ? f.z[0][0] : halves ? f.z[u][h] : f.z[u][0]) & 15;
-            s2[u][h] = row_ok && (kt * KS + u) * BK + 32 * h < w.K ? scale * 0x10001u : 0u;
-            off[u][h] = quarter < 2 ? I::offset(zero) : int4_offset_hi<BF16>(zero);
-          }
-        fetch(f, kt + 4);
+          for (int u = 0; u < KS; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t scale = whole ? f.s[0][0] : halves ? f.s[u][h] : f.s[u][0];
+              const int zero = !ze ? 8 : (whole ? f.z[0][0] : halves ? f.z[u][h] : f.z[u][0]) & 15;
+              s2[u][h] = (kt * KS + u) * BK + 32 * h < w.K ? scale * twice : 0u;
+              off[u][h] = offset(zero);
+            }
+        }
+        fetch(f, kt + 2 * GROUPS);
         if (!mbar_wait(bar_pfull(stage), phase, p.status, DS_TMA_FULL_TIMEOUT)) return false;
+        // pieces of a step: a whole one, with all codes read ahead, or half of one where there are fewer registers
+        constexpr int WORDS = SHORT ? 8 : 16, PIECES = KS * 16 / WORDS;
+        uint32_t codes[SHORT ? 1 : PIECES][WORDS];
+        auto read = [&](uint32_t (&c)[WORDS], int piece) {
 #pragma unroll
-        for (int u = 0; u < KS; ++u) {
-          uint32_t c[16], a[32];
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
+          for (int t = 0; t < WORDS / 4; ++t)
             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                          : "=r"(c[4 * t]), "=r"(c[4 * t + 1]), "=r"(c[4 * t + 2]), "=r"(c[4 * t + 3])
-                         : "r"(src + stage * kPStage + u * 512 + t * 128));
+                         : "r"(src + stage * kPStage + piece * WORDS / 16 * 512 + (piece * WORDS % 16 / 4 + t) * 128));
+        };
+        if constexpr (!SHORT)
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) read(codes[i], i);
+#pragma unroll
+        for (int piece = 0; piece < PIECES; ++piece) {
+          const int u = piece * WORDS / 16, w0 = piece * WORDS % 16;
+          uint32_t (&c)[WORDS] = codes[SHORT ? 0 : piece];
+          if constexpr (SHORT) read(c, piece);
+          uint32_t a[2 * WORDS];
           if (quarter < 2) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              a[2 * i] = int4_pair<BF16, 0, 0>(c[i], off[u][i >> 3], s2[u][i >> 3]);
-              a[2 * i + 1] = int4_pair<BF16, 0, 1>(c[i], off[u][i >> 3], s2[u][i >> 3]);
+            for (int i = 0; i < WORDS; ++i) {
+              a[2 * i] = int4_pair<BF16, 0, 0>(c[i], off[u][(w0 + i) >> 3], s2[u][(w0 + i) >> 3]);
+              a[2 * i + 1] = int4_pair<BF16, 0, 1>(c[i], off[u][(w0 + i) >> 3], s2[u][(w0 + i) >> 3]);
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              a[2 * i] = int4_pair_hi<BF16, 0>(c[i], off[u][i >> 3], s2[u][i >> 3]);
-              a[2 * i + 1] = int4_pair_hi<BF16, 1>(c[i], off[u][i >> 3], s2[u][i >> 3]);
+            for (int i = 0; i < WORDS; ++i) {
+              a[2 * i] = int4_pair_hi<BF16, 0>(c[i], off[u][(w0 + i) >> 3], s2[u][(w0 + i) >> 3]);
+              a[2 * i + 1] = int4_pair_hi<BF16, 1>(c[i], off[u][(w0 + i) >> 3], s2[u][(w0 + i) >> 3]);
             }
           }
-          if (u == 0) {
+          if (piece == 0) {
             if (!mbar_wait_cluster(bar_empty(stage), phase ^ 1, p.status, DS_STAGE_EMPTY_TIMEOUT)) return false;
             tc_fence_after();
           }
           __syncwarp();
-          tmem_st32(a_lane + stage * kStageCols + u * (BK / 2), a);
+          tmem_st(a_lane + stage * kStageCols + piece * WORDS * 2, a);
         }
         if (lane == 0) mbar_arrive(bar_pempty(stage));
         tmem_st_wait();
@@ -621,13 +662,13 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       // (two sets of scales in turn, not one handed to the other: a move would wait for the load)
       Raw even{}, odd{};
       fetch(even, kt);
-      fetch(odd, kt + 2);
+      fetch(odd, kt + GROUPS);
       while (kt < g.kt_end) {
         if (!(ok = decode(even, kt))) break;
-        kt += 2;
+        kt += GROUPS;
         if (kt >= g.kt_end) break;
         if (!(ok = decode(odd, kt))) break;
-        kt += 2;
+        kt += GROUPS;
       }
     }
   }
@@ -658,14 +699,14 @@ int4_tensor_sum_kernel(const TensorParams p) {
   if (b_first != static_cast<int>(blockIdx.y)) return;
   const int i = blockIdx.x * 256 + threadIdx.x;
   const int lane4 = (i & 31) * 4, rank = (i >> 5) & 1, m = i >> 6;
-  const int row0 = (tile % p.m_tiles) * BM, n = (tile / p.m_tiles) * BN + rank * BNH + row_of_lane(lane4 >> 5, lane4 & 31);
-  if (m >= BM || row0 + m >= p.M || n >= p.w.N) return;
+  const int row0 = (tile % p.m_tiles) * kRows, n = (tile / p.m_tiles) * BN + rank * BNH + row_of_lane(lane4 >> 5, lane4 & 31);
+  if (m >= kRows || row0 + m >= p.M || n >= p.w.N) return;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int b = b_first; b <= b_last; ++b) {
     const int piece = pair_begin(b, p.q, p.r) > t0u ? 0 : 1;
     const float4 v = __ldcg(reinterpret_cast<const float4*>(
-        p.ws_partial + ((static_cast<size_t>(b) * 2 + piece) * 2 + rank) * (static_cast<size_t>(BM) * BNH) + static_cast<size_t>(m) * BNH + lane4));
+        p.ws_partial + ((static_cast<size_t>(b) * 2 + piece) * 2 + rank) * (static_cast<size_t>(kRows) * BNH) + static_cast<size_t>(m) * BNH + lane4));
     sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
   }
   T* out = static_cast<T*>(p.y) + static_cast<long long>(row0 + m) * p.w.N + n;
@@ -728,17 +769,23 @@ bool make_w_map(CUtensorMap* map, const Int4Weight& w, int experts) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 int sm_pairs() { return max(1, sm_count_cached() / 2); }
-constexpr size_t kPairPartialBytes = 2 * 2 * static_cast<size_t>(BM) * BNH * sizeof(float);
+constexpr size_t kPairPartialBytes = 2 * 2 * static_cast<size_t>(kRows) * BNH * sizeof(float);
 
-template <bool BF16, int MODE>
-int launch(int pairs, const void* x, int rows, const TensorParams& p, cudaStream_t s) {
+template <bool BF16, int MODE, bool SHORT>
+int launch_shape(int pairs, const void* x, int rows, const TensorParams& p, cudaStream_t s) {
   static SmemOptIn opt_in;
-  auto kernel = int4_tensor_kernel<BF16, MODE>;
+  auto kernel = int4_tensor_kernel<BF16, MODE, SHORT>;
   CUtensorMap map, map32, map_w;
   if (!make_x_map(&map, x, rows, p.w.K, 128, BF16) || !make_x_map(&map32, x, rows, p.w.K, 32, BF16) ||
       !make_w_map(&map_w, p.w, MODE == kDense ? 1 : p.rows.E) || !opt_in.ask(kernel))
     return VQG_ERR_LAUNCH;
-  return cuda_status(launch_ahead(kernel, dim3(2 * pairs), kThreads, kSmem + 1024, s, false, map, map32, map_w, p));
+  return cuda_status(launch_ahead(kernel, dim3(2 * pairs), Shape<SHORT>::THREADS, Shape<SHORT>::SMEM + 1024, s, false, map, map32, map_w, p));
+}
+
+template <int MODE>
+int launch(int pairs, const void* x, int rows, bool is_short, bool bf16, const TensorParams& p, cudaStream_t s) {
+  if (is_short) return bf16 ? launch_shape<true, MODE, true>(pairs, x, rows, p, s) : launch_shape<false, MODE, true>(pairs, x, rows, p, s);
+  return bf16 ? launch_shape<true, MODE, false>(pairs, x, rows, p, s) : launch_shape<false, MODE, false>(pairs, x, rows, p, s);
 }
 
 }  // namespace
@@ -751,7 +798,7 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   TensorParams p{};
   p.w = w; p.y = y; p.M = M;
   p.status = device_status_ptr();
-  p.m_tiles = (M + BM - 1) / BM;
+  p.m_tiles = (M + kRows - 1) / kRows;
   p.n_tiles = (w.N + BN - 1) / BN;
   const int max_pairs = sm_pairs(), stages = (w.k_tiles() + KS - 1) / KS;
   const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
@@ -766,15 +813,15 @@ int launch_int4_tensor(const Int4Weight& w, const void* x, void* y, int M, bool 
   p.q = static_cast<int>(units / pairs);
   p.r = static_cast<int>(units % pairs);
   p.ws_partial = split ? static_cast<float*>(ws) : nullptr;
-  const int st = bf16 ? launch<true, kDense>(pairs, x, M, p, s) : launch<false, kDense>(pairs, x, M, p, s);
+  const int st = launch<kDense>(pairs, x, M, M <= Shape<true>::ROWS, bf16, p, s);
   if (st != VQG_OK || !split || pairs == 1) return st;
-  const dim3 grid(((M < BM ? M : BM) * 64 + 255) / 256, pairs - 1);
+  const dim3 grid(((M < kRows ? M : kRows) * 64 + 255) / 256, pairs - 1);
   return cuda_status(bf16 ? launch_ahead(int4_tensor_sum_kernel<true>, grid, 256, 0, s, false, p)
                           : launch_ahead(int4_tensor_sum_kernel<false>, grid, 256, 0, s, false, p));
 }
 
 namespace {
-int launch_experts(const Int4Weight& w, const void* x, void* y, const ExpertRows& rows, int max_chunks, bool bf16, bool gated,
+int launch_experts(const Int4Weight& w, const void* x, void* y, const ExpertRows& rows, int chunk_rows, int max_chunks, bool bf16, bool gated,
                    cudaStream_t s) {
   TensorParams p{};
   p.w = w; p.y = y; p.rows = rows;
@@ -783,18 +830,18 @@ int launch_experts(const Int4Weight& w, const void* x, void* y, const ExpertRows
   const long long most = static_cast<long long>(max_chunks) * p.n_tiles;
   if (most > 0x7fffffffLL) return VQG_ERR_UNSUPPORTED;
   const int pairs = most < sm_pairs() ? static_cast<int>(most) : sm_pairs();
-  if (gated) return bf16 ? launch<true, kGated>(pairs, x, rows.slots, p, s) : launch<false, kGated>(pairs, x, rows.slots, p, s);
-  return bf16 ? launch<true, kDown>(pairs, x, rows.slots, p, s) : launch<false, kDown>(pairs, x, rows.slots, p, s);
+  const bool is_short = chunk_rows <= Shape<true>::ROWS;
+  return gated ? launch<kGated>(pairs, x, rows.slots, is_short, bf16, p, s) : launch<kDown>(pairs, x, rows.slots, is_short, bf16, p, s);
 }
 }  // namespace
 
-int launch_int4_tensor_gated(const Int4Weight& w, const void* x_rows, void* h, const ExpertRows& rows, int max_chunks, bool bf16,
+int launch_int4_tensor_gated(const Int4Weight& w, const void* x_rows, void* h, const ExpertRows& rows, int chunk_rows, int max_chunks, bool bf16,
                              cudaStream_t s) {
-  return launch_experts(w, x_rows, h, rows, max_chunks, bf16, true, s);
+  return launch_experts(w, x_rows, h, rows, chunk_rows, max_chunks, bf16, true, s);
 }
-int launch_int4_tensor_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int max_chunks, bool bf16,
+int launch_int4_tensor_down(const Int4Weight& w, const void* h, float* part, const ExpertRows& rows, int chunk_rows, int max_chunks, bool bf16,
                             cudaStream_t s) {
-  return launch_experts(w, h, part, rows, max_chunks, bf16, false, s);
+  return launch_experts(w, h, part, rows, chunk_rows, max_chunks, bf16, false, s);
 }
 
 int launch_gather_rows(const void* x, const ExpertRows& rows, void* out, int cols, cudaStream_t s) {
