@@ -197,6 +197,14 @@ def test_graphs_captured_on_one_stream_and_replayed_on_two(t):
         assert all(torch.equal(v, y) for v in ys)
 
 
+@pytest.mark.parametrize("t", [15, 17, 40, 380, 390])
+def test_large_experts_either_side_of_the_kernels_limits(t):
+    up, down = moe(8, 2080, 2048, 32, BF16, False, seed=t)       # more than 2^25 places; 4 and 96 rows each are limits
+    x = acts(t, 2080, BF16, seed=t)
+    ids, w = choices(t, 2, 8, seed=t)
+    check(V.int4_experts(x, ids, w, up, down), O.experts(x, ids, w, up, down))
+
+
 def test_rows_of_experts_past_32_bits():
     # 2.2e9 values of all rows' second products; the last and middle tokens against 64 bits
     t, k, e, hidden, inner = 140_000, 4, 6, 4096, 32

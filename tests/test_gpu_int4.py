@@ -253,6 +253,12 @@ def test_outputs_and_weights_past_32_bits():
     assert torch.equal(back[-1, -300:], alone) and not bool(back[:-1].any()) and not bool(back[-1, :-300].any())
 
 
+@pytest.mark.parametrize("m", [8, 9, 16, 17, 32, 33, 128, 129])
+def test_either_side_of_the_kernels_limits(m):
+    w, x = make(8200, 6176, 32, BF16, True, seed=m), acts(m, 6176, BF16, seed=m)       # more than 3 * 2^24 places
+    check(V.int4_gemm(x, *w), O.gemm(x, *w))
+
+
 def test_two_threads_on_streams_of_their_own():
     jobs = [(acts(m, 512, F16, seed=m), make(400, 512, 128, F16, seed=m)) for m in (2, 60)]
     want = [V.int4_gemm(x, *w) for x, w in jobs]

@@ -75,10 +75,10 @@ def test_bad_arguments_are_rejected_without_cuda(lib):
 
 
 def test_scratch_is_asked_for_where_pieces_are_summed(lib):
-    """Above 32 rows, and above 16 for weights of more than 2^24 places."""
+    """Above 32 rows, above 16 for weights of 2^24 places or more, above 8 for more than 3 * 2^24."""
     need = lib.vqg_int4_workspace_bytes
-    assert need(16, 8192, 8192) == need(32, 4096, 4096) == need(33, 0, 64) == need(0, 4096, 4096) == 0
-    assert need(17, 4096, 4160) == need(33, 64, 64) > 0
+    assert need(8, 8192, 8192) == need(16, 4096, 4096) == need(32, 4096, 4064) == need(33, 0, 64) == need(0, 4096, 4096) == 0
+    assert need(9, 8192, 8192) == need(17, 4096, 4096) == need(33, 64, 64) > 0
 
 
 def test_python_layer_refuses_cpu_tensors():

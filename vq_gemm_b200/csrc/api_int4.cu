@@ -51,17 +51,24 @@ size_t up(size_t n) { return (n + 255) / 256 * 256; }
 // Slots up to which a batch is worked on slot by slot, without ordering it by expert.
 constexpr int kDirectSlots = 32;
 
-// The dense product goes to the tensor-memory kernel above 32 rows, and above 16 where the weight has more than 2^24 places:
-// 32 rows of 4096 x 4096 take 12.2 us in the few-rows kernel and 13.0 in the other, of 1024 x 1024 3.6 and 6.8, of 4096 x
-// 14336 38.8 and 23.5, of 28672 x 8192 89 and 67; 16 rows of 28672 x 8192 54 and 67 (17 rows: 84 and 67).
-bool gemm_on_tensor(int M, int N, int K) { return M > 32 || (M > 16 && static_cast<long long>(N) * K > (1 << 24)); }
-// Rows per expert, on average, from which the experts' products do: 64 experts of 2048 x 1024 take, with the few-rows kernel
-// and with the other, 110 and 125 us at 9 rows, 122 and 125 at 10, 144 and 125 at 11 to 16; 8 of 4096 x 14336 348 and 371 at
-// 10, 459 and 384 at 14.
-bool experts_on_tensor(long long slots, int E) { return slots >= 11LL * E; }
-// Rows of a chunk of an expert's rows: what most experts have, so that few read their weights twice.
-int expert_chunk_rows(long long slots, int E) {
-  if (experts_on_tensor(slots, E)) return slots <= 96LL * E ? 128 : kInt4TensorRows;
+// The dense product goes to the tensor-memory kernel above 32 rows, above 16 for weights of 2^24 places or more, above 8 for more
+// than 3 * 2^24.  Few-rows kernel and the other: 32 rows of 1024 x 1024 3.6 and 6.8 us, of 4096 x 4096 12.0 and 11.1, of 6144 x
+// 4096 15.3 and 12.5; 16 rows of 6144 x 4096 10.0 and 12.4, of 11008 x 4096 14.0 and 15.3, of 4096 x 14336 24.3 and 17.2, of
+// 28672 x 8192 54 and 45 (and 8 rows of it 37 and 44).
+bool gemm_on_tensor(int M, int N, int K) {
+  const long long places = static_cast<long long>(N) * K;
+  return M > 32 || (M > 16 && places >= (1 << 24)) || (M > 8 && places > 3 * (1 << 24));
+}
+// Rows per expert, on average, from which the experts' products do: 4 where the down weights have more than 2^25 places in all, else
+// 11.  Both again: 64 experts of 2048 x 1024 at 4 rows 98 and 96 us, at 6 109 and 97, at 10 121 and 98; 8 of 4096 x 14336 at 5 322
+// and 263; 8 of 1024 x 512 at 9 17.5 and 19.5, at 11 19.7 and 19.9.
+bool experts_on_tensor(long long slots, int E, int hidden, int inner) {
+  return slots >= (static_cast<long long>(E) * hidden * inner > (1 << 25) ? 4LL : 11LL) * E;
+}
+// Rows of a chunk of an expert's rows: what most experts have, so that few read their weights twice.  (128 is the tensor-memory
+// kernel's short shape: 768 tokens through 64 experts, 96 rows each, 138 us with it and 163 without.)
+int expert_chunk_rows(long long slots, int E, bool tensor) {
+  if (tensor) return slots <= 96LL * E ? 128 : kInt4TensorRows;
   return slots <= 5LL * E ? 8 : 16;
 }
 
@@ -73,10 +80,11 @@ ExpertScratch expert_scratch(int T, int top_k, int E, int hidden, int inner) {
   const size_t slots = static_cast<size_t>(T) * top_k;
   a.h = 0;
   a.rows = a.h + up(slots * inner * 2);
-  a.part = a.rows + (experts_on_tensor(slots, E) && slots > kDirectSlots ? up(slots * hidden * 2) : 0);
+  const bool tensor = experts_on_tensor(slots, E, hidden, inner);
+  a.part = a.rows + (tensor && slots > kDirectSlots ? up(slots * hidden * 2) : 0);
   a.row_slot = a.part + (slots > kDirectSlots ? up(slots * hidden * 4) : 0);
   a.chunks = a.row_slot + up(slots * 4);
-  a.n_chunks = a.chunks + up(static_cast<size_t>(expert_max_chunks(static_cast<int>(slots), E, expert_chunk_rows(slots, E))) * sizeof(int4));
+  a.n_chunks = a.chunks + up(static_cast<size_t>(expert_max_chunks(static_cast<int>(slots), E, expert_chunk_rows(slots, E, tensor))) * sizeof(int4));
   a.total = a.n_chunks + 256;
   return a;
 }
@@ -189,8 +197,8 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
   int* row_slot = reinterpret_cast<int*>(ws + at.row_slot);
   int4* chunks = reinterpret_cast<int4*>(ws + at.chunks);
   int* n_chunks = reinterpret_cast<int*>(ws + at.n_chunks);
-  const bool tensor = experts_on_tensor(rows.slots, E);
-  const int chunk = expert_chunk_rows(rows.slots, E), most = expert_max_chunks(rows.slots, E, chunk);
+  const bool tensor = experts_on_tensor(rows.slots, E, hidden, inner);
+  const int chunk = expert_chunk_rows(rows.slots, E, tensor), most = expert_max_chunks(rows.slots, E, chunk);
   st = launch_expert_plan(rows.ids, rows.slots, E, chunk, row_slot, chunks, n_chunks, s);
   if (st != VQG_OK) return st;
   rows.row_slot = row_slot; rows.chunks = chunks; rows.n_chunks = n_chunks;
