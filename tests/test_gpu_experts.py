@@ -103,6 +103,21 @@ def test_route_refusals_and_empty_batch():
         V.route_experts(x.t(), 2)
 
 
+@pytest.mark.parametrize("scoring,bias,groups,top_groups", [("sigmoid", True, 8, 4), ("sigmoid", True, 1, 1), ("softmax", False, 8, 4), ("sigmoid", False, 1, 1)])
+def test_rows_with_few_experts_left_and_with_none(scoring, bias, groups, top_groups):
+    x = logits(40, 256, seed=11)
+    g = torch.Generator(device=x.device).manual_seed(12)
+    for row in range(20):                      # 0 ... 19 experts left
+        left = torch.randperm(256, generator=g, device=x.device)[:row]
+        kept = x[row, left].clone()
+        x[row] = -INF
+        x[row, left] = kept
+    b = torch.randn(256, generator=g, device=x.device) * 0.05 if bias else None
+    check_route(x, 8, scoring=scoring, bias=b, groups=groups, top_groups=top_groups, renormalize=True)
+    w, ids = V.route_experts(x, 8, scoring=scoring, bias=b, groups=groups, top_groups=top_groups, renormalize=True)
+    assert bool((ids[0] == -1).all()) and not bool(w[0].any())
+
+
 def moe(e, hidden, inner, group, dtype, zeros, seed=0):
     return make(2 * inner, hidden, group, dtype, zeros, (e,), seed), make(hidden, inner, 32 if group > inner else group, dtype, zeros, (e,), seed + 1)
 

@@ -6,8 +6,13 @@
 // asynchronously into a ring of its own in shared memory, SLOTS blocks ahead: no warp waits for another, and no register or
 // scoreboard is tied up by a load from memory.  The copies go in memory order, lane i the i-th 16 bytes (in the order in
 // which the lanes need them a quarter warp would touch four lines instead of one, which alone cost 14 of 46 us at 1 x
-// 28672 x 8192), into places that are swizzled so that neither side has bank conflicts: see place().  The eight warps' sums
-// of a row group meet in shared memory.
+// 28672 x 8192), into places that are swizzled so that neither side has bank conflicts: see place().  The sums of a team
+// of warps (one to eight, see below) meet in shared memory.
+//
+// What bounds it: bytes by the count (half a byte per weight and nothing twice), issue and latency by measurement.  1 x 28672 x
+// 8192 bf16 takes 36.9 us, 3.3 TB/s where a copy reaches 6.5: some 106 instructions of a warp per tile of 16 x 64 weights, half of
+// them the decoding (mask, subtract, multiply: each weight is rounded to T as the format says), 64 % of the issue slots busy.
+// 1 x 4096 x 4096 takes 5.2 us, 16 x 11008 x 4096 14.0.
 #include <type_traits>
 
 #include "int4.cuh"

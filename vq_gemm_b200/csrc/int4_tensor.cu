@@ -6,12 +6,12 @@
 // pair (cta_group::2), its N dimension up to 256 rows of X, A = W from tensor memory, B = X from shared memory.  A decoding
 // thread owns one weight row = one tensor-memory lane; 64 columns of it are 32 registers and one tcgen05.st.
 //
-// Roles per CTA (512 threads, four warpgroups):
-//   warp 0       TMA producer of X: this CTA's half of the rows, boxes of 32 rows x 64 columns, SWIZZLE_128B
+// Roles per CTA (512 threads, or 768 for tiles of up to 128 rows: see Shape):
+//   warp 0       TMA producer of X: this CTA's half of the rows, boxes of 128 or 32 rows x 64 columns, SWIZZLE_128B
 //   warp 1       pair leader: issues the MMAs and commits; other CTA: forwards "my operands are in place"
 //   warp 2       producer of packed weights: whole tiles by TMA into a ring of its own
 //   warps 4..7   epilogue
-//   warps 8..15  decoding; warps 8..11 the even, 12..15 the odd stages
+//   warps 8..    decoding; groups of four warps take the stages in turn
 //
 // Rows of a tile: 256 at most, rounded up to 32 for the instruction, so a short tile costs what it needs on the tensor pipe.
 // Tensor memory: columns [0, 256) accumulator, [256 + 64 s, +64) A stage s (two 64-column steps).
@@ -19,6 +19,10 @@
 // tiles go to the workspace in fp32 and a second kernel sums them in pair order: with 16 tiles over 74 pairs (256 x 4096 x
 // 4096) a sum by the contributor that arrives last, 128 threads at two 32 KiB copies in flight, took 45 of 68 thousand
 // cycles; a kernel of its own has all SMs for it.  Experts: whole tiles, dealt out in turn.
+// What bounds it: with many rows the tensor pipe under the power limit (4096 x 14336 x 4096 fp16 345 us = 1.39 PFLOP/s with cool
+// clocks, 413 us in a long run); with few rows the decoding warps' chain of waits and arithmetic (64 x 28672 x 8192 bf16 46 us =
+// 2.6 TB/s of packed weights, where one more or less stage, four times fewer instructions on the tensor pipe or weights from L2 made
+// no difference, and twice as many decoding warps took 57 to 46).
 // Every wait is bounded; no TMA load uses cluster multicast.
 #include "int4.cuh"
 #include "tc_ptx.cuh"
@@ -336,8 +340,7 @@ int4_tensor_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
       }
     } else if (warp == 2) {
       // ------------------------------- packed-weight producer -----------------------------------
-      // one copy per stage: eight row tiles x KS column tiles (eight bulk copies of a row tile each, one per lane, took 1150 cycles
-      // of issue a stage, more than anything else in it).  Row tiles behind the last one are another expert's, or zero.
+      // one copy per stage: eight row tiles x KS column tiles.  Row tiles behind the last one are another expert's, or zero.
       if (lane == 0) {
         int stage = 0;
         uint32_t phase = 0;
