@@ -1,0 +1,58 @@
+"""The router's order where 32 bits do not show it: what it answers is the definition's order in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import vq_gemm_b200 as V
+from oracle import int4_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+def check(x, k, **kw):
+    w, i = V.route_experts(x, k, **kw)
+    want, ids = O.route(x, k, **kw)
+    wrong = (i.cpu() != ids).any(-1)
+    assert not wrong.any(), (int(wrong.sum()), len(wrong), x[wrong.to(x.device)][:2], i.cpu()[wrong][:2], ids[wrong][:2])
+    # p = exp(d) / sum, d >= -104 where p is not zero in fp32: half a step of d (2^-24 of it), the exponential 2^-22, a sum of at
+    # most 21 roundings and the divisions, below (104 + 40) 2^-24 of p in all; below the normal numbers p has fewer bits
+    assert bool(((w.cpu().double() - want).abs() <= want.abs() * 2.0 ** -16 + 1e-37).all())
+
+
+def logit_of(p):
+    return np.log(p / (1 - p))
+
+
+def groups_of_equal_sums(rows, groups, apart, seed):
+    """p [rows, groups, 2]: pairs whose sums differ by about `apart`"""
+    g = np.random.default_rng(seed)
+    total = g.uniform(0.8, 1.2, (rows, 1)) + g.normal(0, apart, (rows, groups))
+    first = g.uniform(0.25, 0.55, (rows, groups))
+    return np.stack((first, total - first), -1)
+
+
+def test_groups_whose_large_biases_cancel_one_row():
+    x = torch.tensor([[1.75845480, 0.46500289, 1.75849342, 0.46500289]]).cuda()
+    bias = torch.tensor([64.0, -64.0, 80.0, -80.0]).cuda()
+    check(x, 2, scoring="sigmoid", bias=bias, groups=2, top_groups=1)
+
+
+@pytest.mark.parametrize("scoring", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("size", [1.0, 64.0, 1000.0])
+def test_groups_whose_large_biases_cancel(scoring, size):
+    p = groups_of_equal_sums(1500, 4, 2e-6 if size < 100 else 2e-5, 7).reshape(1500, 8)
+    x = torch.from_numpy(logit_of(p) if scoring == "sigmoid" else np.log(p)).float().cuda()
+    b = torch.tensor([size, 1.125 * size, 1.25 * size, 1.5 * size])
+    bias = torch.stack((b, -b), -1).flatten().cuda()
+    check(x, 4, scoring=scoring, bias=bias, groups=4, top_groups=2)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 3)])
+def test_biases_of_every_size_and_sign(scoring, groups, top_groups):
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(200, 64, generator=g) * 1.5
+    for size in (1e-6, 1.0, 64.0, 1e6, 1e30):
+        bias = torch.randint(-2, 3, (64,), generator=g).float() * size            # many experts share one
+        bias[5], bias[40] = -float("inf"), torch.finfo(torch.float32).min
+        check(x.cuda(), 8, scoring=scoring, bias=bias.cuda(), groups=groups, top_groups=top_groups)

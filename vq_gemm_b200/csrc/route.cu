@@ -272,21 +272,24 @@ route_kernel(const RouteParams p) {
     const bool mine = (lane >> shift) < p.groups && (lane & ((1 << shift) - 1)) == 0;
     const float score = p.group_max || second == -INFINITY ? first : first + second;
     // the best top_groups of them, one after the other, equal ones in order
-    float left = mine ? score : -INFINITY, worst = INFINITY;
+    float left = mine ? score : -INFINITY;
     unsigned kept = 0;                                      // bit of each kept group's first lane
     for (int j = 0; j < p.top_groups; ++j) {
       const float m = warp_max(left);
       if (m == -INFINITY) break;
       const int at = __ffs(__ballot_sync(kAll, left == m)) - 1;
       kept |= 1u << at;
-      worst = m;
       if (lane == at) left = -INFINITY;
     }
-    // the last kept one must be surely better than every other: two p of at most 1 (without bias they are the score), two
-    // choices of at most |score| + 2 in all, and their sum, of either group
-    const float best = warp_max(left);
-    const float wrong = (p.sigmoid || p.bias ? 2.f : fabsf(worst)) * of_p + (2.f * fabsf(worst) + (p.bias ? 2.f : 0.f)) * of_choice;
-    if (!(best == -INFINITY || worst - best > 2.1f * wrong)) {   // (the whole warp)
+    // Every kept group must be surely better than every other.  How far a score can be off: two p (of at most 1; without a bias
+    // they are the score), the two choices' own roundings -- of the choices, which may be large and cancel in their sum -- and
+    // the sum's.  (A choice and its error grow together, so an expert that 32 bits do not put among a group's first two cannot
+    // raise the score by more.)  Twice that, for the rounding of the limits themselves.
+    const float sizes = fabsf(first) + (p.group_max || second == -INFINITY ? 0.f : fabsf(second)) + fabsf(score);
+    const float wrong = 2.f * ((p.sigmoid || p.bias ? 2.f : fabsf(score)) * of_p + sizes * of_choice);
+    const float lower = wrong < INFINITY ? score - wrong : -INFINITY, upper = left > -INFINITY ? left + wrong : -INFINITY;
+    const float best = warp_max(upper), worst = -warp_max(kept >> lane & 1u ? -lower : -INFINITY);
+    if (!(best == -INFINITY || worst > best)) {                  // (the whole warp)
       choices_64(p, token, scratch);
       kept = groups_64(p, scratch + p.E, shift);
       __syncwarp();
