@@ -1,0 +1,44 @@
+"""Products and experts' layers at sizes of large models: long rows of X, which the few-rows kernels read from memory instead of shared
+memory, wide hidden and inner dimensions, and either side of the choice between the kernels."""
+import pytest
+import torch
+
+import vq_gemm_b200 as V
+from oracle import int4_oracle as O
+from tests.test_gpu_experts import choices
+from tests.test_gpu_int4 import BF16, F16, acts, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype,zeros,group", [(F16, True, 64), (BF16, False, 32)])
+@pytest.mark.parametrize("m,n,k", [(8, 100, 8192), (5, 33, 20032), (9, 77, 9024), (12, 130, 7232), (16, 50, 4224), (16, 300, 8192), (24, 40, 8192)])
+def test_products_of_few_long_rows(m, n, k, dtype, zeros, group):
+    w, x = make(n, k, group, dtype, zeros, seed=m + n), acts(m, k, dtype, seed=m)
+    y = V.int4_gemm(x, *w)
+    check(y, O.gemm(x, *w))
+    assert torch.equal(V.int4_gemm(x, *w), y)
+
+
+# tokens, choices, experts, hidden, inner: over 32 slots, under 11 per expert; chunks of 8 rows up to 5 per expert, else of 16
+@pytest.mark.parametrize("dtype,zeros,group", [(F16, False, 128), (BF16, True, 32)])
+@pytest.mark.parametrize("t,k,e,hidden,inner", [(12, 4, 16, 4096, 128), (30, 4, 16, 4096, 128), (16, 8, 32, 2304, 160), (40, 4, 16, 2304, 160),
+                                                (12, 4, 16, 128, 4096), (30, 4, 16, 128, 4096)])
+def test_planned_experts_of_few_long_rows(t, k, e, hidden, inner, dtype, zeros, group):
+    group = 32 if inner % group else group
+    up, down = make(2 * inner, hidden, group, dtype, zeros, (e,), seed=t), make(hidden, inner, group, dtype, zeros, (e,), seed=t + 1)
+    x = acts(t, hidden, dtype, seed=t)
+    ids, w = choices(t, k, e, seed=t, drop=0.1)
+    y = V.int4_experts(x, ids, w, up, down)
+    check(y, O.experts(x, ids, w, up, down))
+    assert torch.equal(V.int4_experts(x, ids, w, up, down), y)
+
+
+@pytest.mark.parametrize("t", [1, 16, 17, 60])
+@pytest.mark.parametrize("hidden,inner,e", [(7168, 640, 8), (256, 14336, 4), (4096, 1536, 8)])
+def test_experts_of_large_models(t, hidden, inner, e):
+    up, down = make(2 * inner, hidden, 128, BF16, False, (e,), seed=t), make(hidden, inner, 128, BF16, False, (e,), seed=t + 1)
+    x = acts(t, hidden, BF16, seed=t)
+    ids, w = choices(t, 2, e, seed=t)
+    check(V.int4_experts(x, ids, w, up, down), O.experts(x, ids, w, up, down))
+    assert V.device_status() == 0

@@ -47,6 +47,25 @@ def test_groups_whose_large_biases_cancel(scoring, size):
     check(x, 4, scoring=scoring, bias=bias, groups=4, top_groups=2)
 
 
+def test_softmax_with_a_bias_that_takes_a_large_p_back():
+    # two experts of small p whose choices are a few steps of fp32 apart, and one whose large p its negative bias takes back: its choice
+    # is only known to some 1e-7
+    g = np.random.default_rng(5)
+    for e, k in ((4, 1), (4, 2), (40, 1), (70, 3)):
+        for _ in range(60):
+            x = np.full(e, -60.0)
+            big, small, other, middle = g.permutation(e)[:4]
+            x[big] = g.uniform(0, 3)
+            x[small], x[other] = x[big] - 11 + g.normal(0, 0.5, 2)
+            x[middle] = x[big] - g.uniform(0.1, 4)
+            x = torch.from_numpy(x).float()[None]
+            p = torch.softmax(x.double(), -1)[0]
+            bias = torch.full((e,), -2.0)
+            bias[small], bias[other] = 0.01, 0.01 + float(p[small] - p[other] + g.uniform(-1e-8, 1e-8))
+            bias[big] = float(0.01 + p[small] + g.uniform(-1e-7, 1e-7) - p[big])
+            check(x.cuda(), k, bias=bias.cuda())
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 3)])
 def test_biases_of_every_size_and_sign(scoring, groups, top_groups):

@@ -159,8 +159,10 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
 // One warp per token.  Where 32 bits do not settle an order, it is not taken from them:
 //   * without a bias the order of the choices is that of the logits, which are compared exactly;
 //   * sigmoid and bias: the few candidates' choices are computed in 64 bits, one lane each;
-//   * softmax and bias, and the choice of groups: values that follow one another must be further apart than the arithmetic can
-//     be wrong, else the row is done again in 64 bits.
+//   * softmax and bias: each chosen one must be further from every other candidate than the two can be wrong, each by its own p
+//     and choice (a large p that a negative bias takes back is wrong by far more than its choice shows), else the row is done
+//     again in 64 bits;
+//   * the choice of groups: the same with the groups' scores.
 // Candidates: at least top_k + 1 choices are as large as the (top_k + 1)-th largest of the 32 lanes' maxima, and few more are
 // (about ten in all for 8 of 256).  They go to a list in shared memory and are ranked by comparing each with all of them.
 // The kernel is bound by issue, not by its bytes: 8 of 256 for 16384 tokens takes 18 us, with eight groups and a bias in 64 bits 25 us,
@@ -169,7 +171,7 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
 template <int EPL, int TYPE, bool FULL>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_kernel(const RouteParams p) {
-  __shared__ double s_all[kRouteWarps][EPL * 64 > EPL * 48 + 50 ? EPL * 64 : EPL * 48 + 50];
+  __shared__ double s_all[kRouteWarps][EPL * 64 + 50];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * kRouteWarps + warp;
   if (token >= p.T) return;
@@ -312,11 +314,15 @@ route_kernel(const RouteParams p) {
       if (m == bound) m = -INFINITY;
     }
   }
-  if (fine) bound -= 4.f * (of_p + fabsf(bound) * of_choice);   // whoever 64 bits may put above it comes along
-  // the list: choice and expert, and logit or p, of each candidate; behind it the first top_k + 1 in order
+  // whoever 64 bits may put above it comes along (a softmax's p is wrong by at most 40 2^-24: see below)
+  if (p.bias) bound -= 4.f * ((fine ? of_p : 40.f / (1 << 24)) + fabsf(bound) * of_choice);
+  // the list: choice and expert, logit or p, and how far the choice can be off, of each candidate; behind it the first top_k + 1
+  // in order.  A softmax's p with d = top - logit is off by half a step of d, 2^-24 d of p, and by less than 40 2^-24 of p for the
+  // exponential (4), the sum (26), its inverse and the product; below the normal numbers by a step.
   float2* list = reinterpret_cast<float2*>(scratch);
   float* list_p = reinterpret_cast<float*>(scratch + EPL * 32);
-  float* sorted_c = list_p + EPL * 32;
+  float* list_off = list_p + EPL * 32;
+  float* sorted_c = list_off + EPL * 32;
   float* sorted_p = sorted_c + 33;
   int* sorted_e = reinterpret_cast<int*>(sorted_p + 33);
   int count = 0;
@@ -329,6 +335,7 @@ route_kernel(const RouteParams p) {
       const int at = count + __popc(votes & below);
       list[at] = make_float2(choice[i], __int_as_float(lane + 32 * i));
       list_p[at] = fine ? logit[i] : prob[i];
+      if (p.bias && !fine) list_off[at] = ((top - logit[i]) + 40.f) * 6e-8f * prob[i] + 6e-8f * fabsf(choice[i]) + 1e-37f;
     }
     count += __popc(votes);
   }
@@ -357,27 +364,32 @@ route_kernel(const RouteParams p) {
     sure = sure && (bound == -INFINITY || (bound > -1e30f && bound < 1e30f));   // all are here, or no bias so large that the margin
                                                                                 // means nothing
   } else {
-    for (int c = lane; c < count; c += 32) {
-      const float2 mine = list[c];
-      const int e = __float_as_int(mine.y);
-      int rank = 0;
-      for (int o = 0; o < count; ++o) {
-        const float2 other = list[o];
-        rank += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
+    auto rank_all = [&](auto with_bias) {
+      for (int c = lane; c < count; c += 32) {
+        const float2 mine = list[c];
+        const int e = __float_as_int(mine.y);
+        const float off = decltype(with_bias)::value ? list_off[c] : 0.f;
+        int rank = 0, close = 0;   // close: neighbours that 64 bits may put on the other side, itself among them
+        for (int o = 0; o < count; ++o) {
+          const float2 other = list[o];
+          rank += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
+          if constexpr (decltype(with_bias)::value) close += !(fabsf(mine.x - other.x) > off + list_off[o]);
+        }
+        if (rank <= p.top_k) { sorted_c[rank] = mine.x; sorted_p[rank] = list_p[c]; sorted_e[rank] = e; }
+        if (rank < p.top_k && close > 1) sure = false;
       }
-      if (rank <= p.top_k) { sorted_c[rank] = mine.x; sorted_p[rank] = list_p[c]; sorted_e[rank] = e; }
-    }
-    if (fine) sure = false;
+    };
+    if (p.bias) rank_all(std::true_type{});
+    else rank_all(std::false_type{});
+    if (fine || !(bound == -INFINITY || (bound > -1e30f && bound < 1e30f))) sure = false;
   }
   __syncwarp();
   const float chosen = lane < wanted ? sorted_p[lane] : 0.f;
   const int id = lane < wanted ? sorted_e[lane] : -1;
-  if (!fine && lane + 1 < min(count, p.top_k + 1)) {   // is number lane + 1 surely behind number lane?
+  if (!p.bias && lane + 1 < min(count, p.top_k + 1)) {   // is number lane + 1 surely behind number lane?
+    // different logits have different exponentials unless they are nearly equal or far out; equal ones are equal in 64 bits too
     const float a = sorted_c[lane], b = sorted_c[lane + 1];
-    if (!p.bias)   // different logits have different exponentials unless they are nearly equal or far out; equal ones are equal in 64 bits too
-      sure = sure && (p.sigmoid ? b > -600.f && (a == b || (a - b > 1e-12f && a < 16.f)) : a == b || (a - b > 1e-12f && b - top > -600.f));
-    else
-      sure = sure && a < INFINITY && a - b > (sorted_p[lane] + sorted_p[lane + 1]) * of_p + (fabsf(a) + fabsf(b)) * of_choice;
+    sure = sure && (p.sigmoid ? b > -600.f && (a == b || (a - b > 1e-12f && a < 16.f)) : a == b || (a - b > 1e-12f && b - top > -600.f));
   }
   const float total = warp_sum(chosen);
   if (wanted > 0 && total < 1e-6f) sure = false;      // weights that 32 bits may not tell from zero
