@@ -66,6 +66,23 @@ def test_softmax_with_a_bias_that_takes_a_large_p_back():
             check(x.cuda(), k, bias=bias.cuda())
 
 
+@pytest.mark.parametrize("low,high", [(40, 63), (63, 87), (87, 104)])
+@pytest.mark.parametrize("group_score", ["top2", "max"])
+def test_softmax_groups_far_below_the_largest_logit(low, high, group_score):
+    g = np.random.default_rng(int(low))
+    rows, apart = 4000, 1e-5
+    x = np.empty((rows, 3, 2))
+    x[:, 0] = 16.75, -30.0
+    depth = 16.75 - g.uniform(low, high, (rows, 1, 1))
+    if group_score == "top2":
+        x[:, 1:] = depth + np.log(groups_of_equal_sums(rows, 2, apart, low))
+    else:
+        x[:, 1:, :1] = depth + g.normal(0, apart, (rows, 2, 1))
+        x[:, 1:, 1:] = x[:, 1:, :1] - 1
+    order = torch.from_numpy(x.reshape(rows, 6)).float().cuda()
+    check(order, 4, groups=3, top_groups=2, group_score=group_score)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 3)])
 def test_biases_of_every_size_and_sign(scoring, groups, top_groups):

@@ -225,11 +225,16 @@ route_kernel(const RouteParams p) {
       choice[i] = logit[i] > -INFINITY ? fmaxf(v, -INFINITY) : -INFINITY;
     }
   }
-  // How far a choice can be off.  Sigmoid: the exponential 2^-22 of itself, which moves p by p (1 - p) <= 1/4 as much, its sum with
-  // one and the reciprocal 2^-24 of p each: 1.8e-7.  Softmax: exponential, argument, a sum of at most 16 + 5 roundings and a
-  // division, below 2^-19 of p.  The bias's addition: 2^-24 of the choice.  (Kept close: a row that has to be done again costs
-  // ten microseconds of latency, most of it the fetching of instructions.)
-  const float of_p = p.sigmoid ? 1.8e-7f : 1.f / (1 << 19), of_choice = 1.f / (1 << 24);
+  // How far 32 bits can be off, in steps of 2^-24.
+  // Sigmoid: the exponential 4 of itself, which moves p by p (1 - p) <= 1/4 as much, its sum with one and the reciprocal 1 of p each:
+  // 3, or 1.8e-7, in all.
+  // Softmax, with d = top - logit: d of p for the rounding of d, 4 for the exponential, 26 for the sum (15 + 5 roundings and the
+  // exponentials in it), its inverse 1, the product 1: (d + 32) p, taken as (d + 40) p; d is at most -ln p, and not above 104
+  // where p is not zero.  It falls as p does; all of a row's p together are off by less than 41.  Below the normal numbers p is off
+  // by steps of 2^-149.
+  // The bias's addition: 1 of the choice.
+  // (Kept close: a row that has to be done again costs ten microseconds of latency, most of it the fetching of instructions.)
+  constexpr float kStep = 1.f / (1 << 24), kSigmoidOff = 1.8e-7f;
   if (p.groups > 1) {
     const int size = p.E / p.groups;
     // the two largest of each group: of group n in lane n << shift
@@ -283,12 +288,15 @@ route_kernel(const RouteParams p) {
       kept |= 1u << at;
       if (lane == at) left = -INFINITY;
     }
-    // Every kept group must be surely better than every other.  How far a score can be off: two p (of at most 1; without a bias
-    // they are the score), the two choices' own roundings -- of the choices, which may be large and cancel in their sum -- and
-    // the sum's.  (A choice and its error grow together, so an expert that 32 bits do not put among a group's first two cannot
-    // raise the score by more.)  Twice that, for the rounding of the limits themselves.
-    const float sizes = fabsf(first) + (p.group_max || second == -INFINITY ? 0.f : fabsf(second)) + fabsf(score);
-    const float wrong = 2.f * ((p.sigmoid || p.bias ? 2.f : fabsf(score)) * of_p + sizes * of_choice);
+    // Every kept group must be surely better than every other.  How far a score can be off: its two p, the two choices' own
+    // roundings -- of the choices, which may be large and cancel in their sum -- and the sum's.  (A choice and its error grow
+    // together, so an expert that 32 bits do not put among a group's first two cannot raise the score by more.)  Twice that, for
+    // the rounding of the limits themselves.
+    const float next = p.group_max || second == -INFINITY ? 0.f : second;
+    float off = p.sigmoid ? 2.f * kSigmoidOff : 41.f * kStep;
+    if (!p.sigmoid && !p.bias)
+      off = (first * (40.f + fminf(-__logf(first), 104.f)) + next * (40.f + fminf(-__logf(next), 104.f))) * kStep + 1e-37f;
+    const float wrong = 2.f * (off + (fabsf(first) + fabsf(next) + fabsf(score)) * kStep);
     const float lower = wrong < INFINITY ? score - wrong : -INFINITY, upper = left > -INFINITY ? left + wrong : -INFINITY;
     const float best = warp_max(upper), worst = -warp_max(kept >> lane & 1u ? -lower : -INFINITY);
     if (!(best == -INFINITY || worst > best)) {                  // (the whole warp)
@@ -314,11 +322,10 @@ route_kernel(const RouteParams p) {
       if (m == bound) m = -INFINITY;
     }
   }
-  // whoever 64 bits may put above it comes along (a softmax's p is wrong by at most 40 2^-24: see below)
-  if (p.bias) bound -= 4.f * ((fine ? of_p : 40.f / (1 << 24)) + fabsf(bound) * of_choice);
+  // whoever 64 bits may put above it comes along
+  if (p.bias) bound -= 4.f * ((fine ? kSigmoidOff : 40.f * kStep) + fabsf(bound) * kStep);
   // the list: choice and expert, logit or p, and how far the choice can be off, of each candidate; behind it the first top_k + 1
-  // in order.  A softmax's p with d = top - logit is off by half a step of d, 2^-24 d of p, and by less than 40 2^-24 of p for the
-  // exponential (4), the sum (26), its inverse and the product; below the normal numbers by a step.
+  // in order
   float2* list = reinterpret_cast<float2*>(scratch);
   float* list_p = reinterpret_cast<float*>(scratch + EPL * 32);
   float* list_off = list_p + EPL * 32;
@@ -335,7 +342,7 @@ route_kernel(const RouteParams p) {
       const int at = count + __popc(votes & below);
       list[at] = make_float2(choice[i], __int_as_float(lane + 32 * i));
       list_p[at] = fine ? logit[i] : prob[i];
-      if (p.bias && !fine) list_off[at] = ((top - logit[i]) + 40.f) * 6e-8f * prob[i] + 6e-8f * fabsf(choice[i]) + 1e-37f;
+      if (p.bias && !fine) list_off[at] = 1.01f * kStep * ((top - logit[i] + 40.f) * prob[i] + fabsf(choice[i])) + 1e-37f;
     }
     count += __popc(votes);
   }
