@@ -83,6 +83,21 @@ def test_softmax_groups_far_below_the_largest_logit(low, high, group_score):
     check(order, 4, groups=3, top_groups=2, group_score=group_score)
 
 
+def test_ties_of_64_bits_between_logits_that_differ():
+    x = torch.full((4, 64), -1.0)
+    x[0, 5], x[0, 6], x[0, 0] = 40.0, 40.0, 39.875          # sigmoid: p = 1 in 64 bits
+    x[1, 9:] = 40.0
+    x[1, 3] = 38.0
+    x[2] = 0.0                                              # softmax: exp(-1e-20) = 1
+    x[2, 40:50] = 1e-20
+    x[3, 60] = 800.0                                        # softmax: the others' p is zero
+    x[3, 20:30] = -0.5
+    for k in (1, 2, 12):
+        for scoring in ("softmax", "sigmoid"):
+            check(x.cuda(), k, scoring=scoring)
+            check(x[:, :8].contiguous().cuda(), min(k, 8), scoring=scoring)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 3)])
 def test_biases_of_every_size_and_sign(scoring, groups, top_groups):

@@ -157,7 +157,8 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
 }
 
 // One warp per token.  Where 32 bits do not settle an order, it is not taken from them:
-//   * without a bias the order of the choices is that of the logits, which are compared exactly;
+//   * without a bias the order of the choices is that of the logits, which are compared exactly -- where different logits have
+//     different p in 64 bits, else (a sigmoid of 16 and more, logits that nothing tells apart) the row is done again there;
 //   * sigmoid and bias: the few candidates' choices are computed in 64 bits, one lane each;
 //   * softmax and bias: each chosen one must be further from every other candidate than the two can be wrong, each by its own p
 //     and choice (a large p that a negative bias takes back is wrong by far more than its choice shows), else the row is done
@@ -171,7 +172,7 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
 template <int EPL, int TYPE, bool FULL>
 __global__ void __launch_bounds__(kRouteWarps * 32)
 route_kernel(const RouteParams p) {
-  __shared__ double s_all[kRouteWarps][EPL * 64 + 50];
+  __shared__ double s_all[kRouteWarps][EPL * 64 + 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * kRouteWarps + warp;
   if (token >= p.T) return;
@@ -323,15 +324,14 @@ route_kernel(const RouteParams p) {
     }
   }
   // whoever 64 bits may put above it comes along
-  if (p.bias) bound -= 4.f * ((fine ? kSigmoidOff : 40.f * kStep) + fabsf(bound) * kStep);
-  // the list: choice and expert, logit or p, and how far the choice can be off, of each candidate; behind it the first top_k + 1
-  // in order
+  bound -= p.bias ? 4.f * ((fine ? kSigmoidOff : 40.f * kStep) + fabsf(bound) * kStep) : 1e-12f;
+  // the list: choice and expert, logit or p, and how far the choice can be off, of each candidate; behind it the first top_k in
+  // order
   float2* list = reinterpret_cast<float2*>(scratch);
   float* list_p = reinterpret_cast<float*>(scratch + EPL * 32);
   float* list_off = list_p + EPL * 32;
-  float* sorted_c = list_off + EPL * 32;
-  float* sorted_p = sorted_c + 33;
-  int* sorted_e = reinterpret_cast<int*>(sorted_p + 33);
+  float* sorted_p = list_off + EPL * 32;
+  int* sorted_e = reinterpret_cast<int*>(sorted_p + 32);
   int count = 0;
   const unsigned below = (1u << lane) - 1u;
 #pragma unroll
@@ -371,33 +371,58 @@ route_kernel(const RouteParams p) {
     sure = sure && (bound == -INFINITY || (bound > -1e30f && bound < 1e30f));   // all are here, or no bias so large that the margin
                                                                                 // means nothing
   } else {
+    // Without a bias.  Logits that differ have different p in 64 bits if they are more than 1e-12 apart, the larger one's p is a normal
+    // number there and, of a sigmoid's, the smaller one is below 16.  `plain`: whatever differs from this one does so by more
+    // (fp32 steps of 3.6e-12 at least), and it is not far out.  What is not in the list is 1e-12 below the lanes' maxima.
+    const float none = p.sigmoid ? 0.f : top, most = p.sigmoid ? 16.f : INFINITY;
+    bool plain = true;
     auto rank_all = [&](auto with_bias) {
       for (int c = lane; c < count; c += 32) {
         const float2 mine = list[c];
         const int e = __float_as_int(mine.y);
         const float off = decltype(with_bias)::value ? list_off[c] : 0.f;
-        int rank = 0, close = 0;   // close: neighbours that 64 bits may put on the other side, itself among them
+        int rank = 0, close = 0;   // close: those that 64 bits may put on its other side, itself among them
         for (int o = 0; o < count; ++o) {
           const float2 other = list[o];
           rank += other.x > mine.x || (other.x == mine.x && __float_as_int(other.y) < e);
           if constexpr (decltype(with_bias)::value) close += !(fabsf(mine.x - other.x) > off + list_off[o]);
         }
-        if (rank <= p.top_k) { sorted_c[rank] = mine.x; sorted_p[rank] = list_p[c]; sorted_e[rank] = e; }
-        if (rank < p.top_k && close > 1) sure = false;
+        if (rank < p.top_k) {
+          sorted_p[rank] = list_p[c];
+          sorted_e[rank] = e;
+          if (close > 1) sure = false;
+        }
+        if constexpr (!decltype(with_bias)::value) plain = plain && fabsf(mine.x) > 6.2e-5f && mine.x - none > -600.f && mine.x < most;
       }
     };
-    if (p.bias) rank_all(std::true_type{});
-    else rank_all(std::false_type{});
-    if (fine || !(bound == -INFINITY || (bound > -1e30f && bound < 1e30f))) sure = false;
+    if (p.bias) {
+      rank_all(std::true_type{});
+    } else {
+      rank_all(std::false_type{});
+      if (__any_sync(kAll, !plain)) {
+        float last = INFINITY;       // place top_k; equal logits have equal p, so their ranks are the definition's
+        for (int c = lane; c < count; c += 32) {
+          const float mine = list[c].x;
+          int before = 0;
+          for (int o = 0; o < count; ++o) before += list[o].x > mine;
+          if (before < p.top_k) last = fminf(last, mine);
+        }
+        last = -warp_max(-last);
+        for (int c = lane; c < count; c += 32) {
+          const float a = list[c].x;
+          for (int o = 0; o < count; ++o) {
+            const float b = list[o].x;
+            if (a >= last && b < a) sure = sure && a - b > 1e-12f && a - none > -600.f && b < most;
+          }
+        }
+        sure = sure && (bound == -INFINITY || (last - none > -600.f && bound < most));
+      }
+    }
+    if (fine || (p.bias && !(bound == -INFINITY || (bound > -1e30f && bound < 1e30f)))) sure = false;
   }
   __syncwarp();
   const float chosen = lane < wanted ? sorted_p[lane] : 0.f;
   const int id = lane < wanted ? sorted_e[lane] : -1;
-  if (!p.bias && lane + 1 < min(count, p.top_k + 1)) {   // is number lane + 1 surely behind number lane?
-    // different logits have different exponentials unless they are nearly equal or far out; equal ones are equal in 64 bits too
-    const float a = sorted_c[lane], b = sorted_c[lane + 1];
-    sure = sure && (p.sigmoid ? b > -600.f && (a == b || (a - b > 1e-12f && a < 16.f)) : a == b || (a - b > 1e-12f && b - top > -600.f));
-  }
   const float total = warp_sum(chosen);
   if (wanted > 0 && total < 1e-6f) sure = false;      // weights that 32 bits may not tell from zero
   if (__ballot_sync(kAll, !sure)) {
