@@ -4,6 +4,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "written.h"
 
 namespace vqg {
 
@@ -19,27 +20,34 @@ __device__ int g_status_word[64];
 void count_launch(int n) { g_launches.fetch_add(static_cast<unsigned long long>(n), std::memory_order_relaxed); }
 
 namespace {
-std::mutex g_dirty_mu;
-cudaStream_t g_dirty[16];
-int g_ndirty = 0;
+WrittenMarks g_written;
+
+// The default streams have one handle on every device, cudaStreamPerThread one in every thread.
+const void* stream_identity(cudaStream_t s) {
+  static thread_local char per_thread;
+  return s == cudaStreamPerThread ? static_cast<const void*>(&per_thread) : s == cudaStreamLegacy ? nullptr : s;
+}
+int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : -1;
+}
+unsigned long long capture_id(cudaStream_t s) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(s, &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
 }  // namespace
 
-void note_weights_written(cudaStream_t s) {
-  std::lock_guard<std::mutex> lk(g_dirty_mu);
-  for (int i = 0; i < g_ndirty; ++i)
-    if (g_dirty[i] == s) return;
-  if (g_ndirty < 16) g_dirty[g_ndirty++] = s;
-  else g_dirty[0] = s;   // table full: streams may then be reported late; the documented contract still holds
-}
+void note_weights_written(cudaStream_t s) { g_written.note({current_device(), stream_identity(s), capture_id(s)}); }
 
 bool take_weights_written(cudaStream_t s) {
-  std::lock_guard<std::mutex> lk(g_dirty_mu);
-  for (int i = 0; i < g_ndirty; ++i)
-    if (g_dirty[i] == s) {
-      g_dirty[i] = g_dirty[--g_ndirty];
-      return true;
-    }
-  return false;
+  const int dev = current_device();
+  const void* id = stream_identity(s);
+  return g_written.maybe(dev, id) && g_written.take({dev, id, capture_id(s)});
 }
 
 cudaError_t ensure_status_word() {
