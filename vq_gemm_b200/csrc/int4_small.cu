@@ -127,8 +127,6 @@ __device__ __forceinline__ void multiply(const Scales<ZEROS, R, B, SPAN>& h, int
     }
 }
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
-
 // The work is chunks of rows of X (one for the dense product; the plan's or one per slot for experts) times the weight's row
 // groups (R row tiles each).  The grid is what runs at once; gridDim.x / chunks blocks share a chunk, and there are teams of TW
 // warps in a block, team n of the chunk's taking row groups [groups * n / teams, groups * (n + 1) / teams).  The warps of a
