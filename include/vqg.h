@@ -309,7 +309,7 @@ VQG_API int vqg_unpack12(const void* packed, void* idx_u16_out, long long values
  * of activations, scales and results:
  *     W[n, k] = round_T((code[n, k] - zero[k / group, n]) * scale[k / group, n]),      code, zero in 0 ... 15,
  * zero = 8 everywhere where no zero points are given.  `group` consecutive columns share a scale: 32, a
- * multiple of 64, or K; K is a multiple of 32 and of `group`, N is any number.
+ * multiple of 64, or K; K is a multiple of 32 and of `group`, at most 2^19; N and M are any numbers up to 2^31 - 512.
  *   packed  [ceil(N/16)][ceil(K/64)][512] bytes, 16-byte aligned: tiles of 16 rows x 64 columns; the byte at
  *           (((t*8 + g)*4 + s)*2 + e)*2 + q of a tile holds column 16t + 4s + 2q + e of row g (low four bits) and
  *           of row g + 8 (high four bits).  What fills up the last tiles is not used.
@@ -340,7 +340,7 @@ VQG_API int vqg_int4_quantize(const void* w, void* packed_out, void* scales_out,
  *   [T, top_k] int32 in falling order and weights_out [T, top_k] fp32 = p, divided by their sum if renormalize,
  *   times scale.  Equal choices and equal scores go to the lower index; they are compared in 64 bits, so the
  *   answer is that of exact arithmetic.  An expert whose logit is -inf or NaN is never chosen and takes no part in
- *   the softmax; a slot for which nothing is left gets expert -1 and weight 0.  E <= 512, top_k <= 32, groups <= 32.
+ *   the softmax; a slot for which nothing is left gets expert -1 and weight 0.  E <= 512, top_k <= 32, groups <= 32, T <= 2^31 - 512.
  * vqg_int4_experts: y[t] = sum over j of weights[t, j] * down_e(SiLU(gate_e(x_t)) * up_e(x_t)), e = experts[t, j].
  *   up_* [E, 2 * inner, hidden]: (gate, up) row pairs as in vqg_gemm_swiglu; down_* [E, hidden, inner]; both in the
  *   4-bit format.  A slot whose expert is outside 0 ... E-1 adds nothing (a token with no expert gets zeros); the

@@ -26,10 +26,13 @@ bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % 
 // A group is 32 columns, a multiple of 64, or the whole row; a row is a whole number of groups.
 bool group_ok(int K, int group) { return K % 32 == 0 && group > 0 && K % group == 0 && (group == 32 || group % 64 == 0 || group == K); }
 
+// Rows of X or of a weight, at most: row numbers are 32 bits and are rounded up to whole tiles of up to 256.
+constexpr int kMaxRows = 0x7fffffff - 511;
+
 int check_weight(const void* packed, const void* scales, const void* zeros, int experts, int N, int K, int group, int dtype) {
   if (experts < 0 || N < 0 || K < 0 || (dtype != 0 && dtype != 1)) return VQG_ERR_BAD_ARG;
   if (experts == 0 || N == 0 || K == 0) return VQG_OK;
-  if (!group_ok(K, group) || K > kInt4MaxK) return VQG_ERR_UNSUPPORTED;
+  if (!group_ok(K, group) || K > kInt4MaxK || N > kMaxRows) return VQG_ERR_UNSUPPORTED;
   if (static_cast<long long>(K / group) * N > 0x7fffffffLL) return VQG_ERR_UNSUPPORTED;   // 32-bit positions of scales
   if (!packed || !scales || !aligned(packed, 16) || !aligned(scales, 2)) return VQG_ERR_BAD_ARG;
   (void)zeros;   // bytes: any address
@@ -103,6 +106,7 @@ int vqg_int4_gemm(const void* x, const void* packed, const void* scales, const v
   const int st = check_weight(packed, scales, zeros, 1, N, K, group, dtype);
   if (st != VQG_OK) return st;
   if (M == 0 || N == 0) return VQG_OK;
+  if (M > kMaxRows) return VQG_ERR_UNSUPPORTED;
   if (!y || !aligned(y, 16)) return VQG_ERR_BAD_ARG;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (K == 0) return cuda_status(cudaMemsetAsync(y, 0, static_cast<size_t>(M) * N * 2, s));
@@ -147,7 +151,7 @@ int vqg_route_experts(const void* logits, const void* bias, void* weights_out, v
   if (T < 0 || E < 1 || top_k < 1 || top_k > E) return VQG_ERR_BAD_ARG;
   if (scoring < 0 || scoring > 1 || group_score < 0 || group_score > 1 || logits_dtype < 0 || logits_dtype > 2) return VQG_ERR_BAD_ARG;
   if (groups < 1 || E % groups != 0 || top_groups < 1 || top_groups > groups) return VQG_ERR_BAD_ARG;
-  if (E > 512 || top_k > 32 || groups > 32) return VQG_ERR_UNSUPPORTED;
+  if (E > 512 || top_k > 32 || groups > 32 || T > kMaxRows) return VQG_ERR_UNSUPPORTED;
   if (T == 0) return VQG_OK;
   if (!logits || !weights_out || !experts_out || !aligned(logits, logits_dtype == 2 ? 4 : 2) || !aligned(bias, 4) ||
       !aligned(weights_out, 4) || !aligned(experts_out, 4))
