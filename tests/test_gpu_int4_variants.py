@@ -7,6 +7,7 @@ import vq_gemm_b200 as V
 from oracle import int4_oracle as O
 from tests.test_gpu_experts import choices
 from tests.test_gpu_int4 import BF16, F16, acts, check, make
+from vq_gemm_b200.linear import Int4Experts
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +43,18 @@ def test_experts_of_large_models(t, hidden, inner, e):
     ids, w = choices(t, 2, e, seed=t)
     check(V.int4_experts(x, ids, w, up, down), O.experts(x, ids, w, up, down))
     assert V.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_cast_layer_routes_with_the_balance_bias_it_was_given(dtype):
+    # biases whose order neither 16-bit type holds: logits are all equal, so the largest biases choose
+    e = 32
+    up, down = make(64, 128, 64, dtype, False, (e,)), make(128, 32, 32, dtype, False, (e,))
+    bias = 0.05 + torch.randperm(e, generator=torch.Generator().manual_seed(4)).float() * 1e-6
+    router = torch.nn.Linear(128, e, bias=False).requires_grad_(False)
+    router.weight.zero_()
+    layer = Int4Experts(router, up, down, top_k=2, in_features=128, scoring="sigmoid", bias=bias).cuda().to(dtype)
+    x = acts(5, 128, dtype)
+    w, ids = V.route_experts(layer.router(x), 2, scoring="sigmoid", bias=bias.cuda(), renormalize=True)
+    assert torch.equal(ids[0].cpu(), bias.topk(2).indices.int())
+    assert torch.equal(layer(x), V.int4_experts(x, ids, w, up, down))

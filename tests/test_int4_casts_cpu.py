@@ -1,0 +1,34 @@
+"""What a cast of a model does to the 4-bit layers' buffers, without a GPU."""
+import copy
+
+import pytest
+import torch
+
+from tests.test_int4_cpu import _packed
+from vq_gemm_b200.linear import Int4Experts
+
+TYPES = [torch.float16, torch.bfloat16, torch.float32, torch.float64]
+
+
+def experts(dtype=torch.float16, bias=True):
+    up, down = _packed(64, 96, 32, dtype, lead=(4,))[1:], _packed(96, 32, 32, dtype, True, lead=(4,), seed=1)[1:]
+    return Int4Experts(torch.nn.Linear(96, 4), up, down, top_k=2, in_features=96,
+                       bias=torch.randn(4, generator=torch.Generator().manual_seed(3)) * 0.05 if bias else None)
+
+
+@pytest.mark.parametrize("to", TYPES)
+def test_the_balance_bias_keeps_its_bits(to):
+    layer = experts()
+    was = layer.bias.clone()
+    for cast in (layer.to(to), copy.deepcopy(layer).to("cpu", to), torch.nn.Sequential(layer).to(to)[0]):
+        assert cast.bias.dtype == torch.float32 and torch.equal(cast.bias, was) and cast.router.weight.dtype == to
+    assert experts(bias=False).to(to).bias is None
+
+
+def test_the_balance_bias_follows_to_another_device():
+    layer = experts().half().to("meta")
+    assert layer.bias.device.type == "meta" and layer.bias.dtype == torch.float32
+    assert experts().to("meta", torch.bfloat16).bias.dtype == torch.float32
+    other = experts().half()
+    other.load_state_dict({k: v + 1 if k == "bias" else v for k, v in other.state_dict().items()})
+    assert other.bias.dtype == torch.float32

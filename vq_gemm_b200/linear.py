@@ -268,6 +268,21 @@ class VQGatedUp(nn.Module):
                 f"entries={self.codebook.shape[1]}, rows_per_codebook={self.rows_per_codebook}")
 
 
+class _KeptTypes(nn.Module):
+    """A module with floating buffers (``_kept``) whose bits matter: casting a model (``.half()``, ``.to(dtype)``) moves them with it and
+    leaves their type."""
+
+    _kept: Tuple[str, ...] = ()
+
+    def _apply(self, fn, recurse=True):
+        before = {name: self._buffers[name] for name in self._kept if self._buffers.get(name) is not None}
+        super()._apply(fn, recurse)
+        for name, t in before.items():
+            if self._buffers[name].dtype != t.dtype:
+                self._buffers[name] = t.to(self._buffers[name].device)
+        return self
+
+
 class Int4Linear(nn.Module):
     """``y = x @ W^T (+ bias)`` with 4-bit weights and group scales, for the layers that one or two bits do not serve.
 
@@ -315,12 +330,14 @@ class Int4Linear(nn.Module):
                 f"zeros={self.zeros is not None}, bias={self.bias is not None}")
 
 
-class Int4Experts(nn.Module):
+class Int4Experts(_KeptTypes):
     """Mixture-of-experts MLP with 4-bit experts: ``router`` (a module that gives logits [..., E], e.g. an ``Int4Linear``, a
     ``VQLinear`` or an ``nn.Linear``), then ``route_experts``, then the gated products of the chosen experts.
 
     ``gate_up`` and ``down`` are (packed, scales, zeros or None) of [E, 2 * inner, hidden] and [E, hidden, inner] weights;
-    ``in_features`` is hidden.  ``bias`` [E] float32 is the router's balance bias."""
+    ``in_features`` is hidden.  ``bias`` [E] float32 is the router's balance bias; it stays float32 when the model is cast."""
+
+    _kept = ("bias",)
 
     def __init__(self, router: nn.Module, gate_up, down, *, top_k: int, in_features: int, scoring: str = "softmax",
                  bias: Optional[torch.Tensor] = None, groups: int = 1, top_groups: Optional[int] = None,
@@ -359,7 +376,7 @@ class Int4Experts(nn.Module):
             raise RuntimeError(f"last dimension {x.shape[-1]} != in_features {self.in_features}")
         x2 = x.reshape(-1, self.in_features)
         logits = self.router(x2).contiguous()
-        bias = None if self.bias is None else self.bias.float()       # (``.to(dtype)`` of a model casts every buffer)
+        bias = None if self.bias is None else self.bias.float()       # (a checkpoint that was assigned may hold another type)
         weights, chosen = torch.ops.vq_gemm_b200.route_experts(
             logits, self.top_k, self.scoring, bias, self.groups, self.top_groups, self.group_score, self.renormalize,
             self.scale)
