@@ -7,7 +7,7 @@ import vq_gemm_b200 as V
 from oracle import int4_oracle as O
 from tests.test_gpu_experts import choices
 from tests.test_gpu_int4 import BF16, F16, acts, check, make
-from vq_gemm_b200.linear import Int4Experts
+from vq_gemm_b200.linear import Int4Experts, Int4Linear
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,22 @@ def test_a_cast_layer_routes_with_the_balance_bias_it_was_given(dtype):
     w, ids = V.route_experts(layer.router(x), 2, scoring="sigmoid", bias=bias.cuda(), renormalize=True)
     assert torch.equal(ids[0].cpu(), bias.topk(2).indices.int())
     assert torch.equal(layer(x), V.int4_experts(x, ids, w, up, down))
+
+
+@pytest.mark.parametrize("own", [F16, BF16])
+@pytest.mark.parametrize("to", [F16, BF16, torch.float32])
+def test_cast_layers_multiply_the_same_weights_and_answer_in_the_models_type(own, to):
+    packed, scales, zeros = make(40, 128, 32, own, True)
+    bias = torch.linspace(-1, 1, 40)
+    layer = Int4Linear(packed, scales, zeros, bias.cuda(), 128)
+    model = torch.nn.Sequential(layer, torch.nn.Linear(40, 8).requires_grad_(False)).cuda().to(to)
+    x = acts(6, 128, torch.float32).to(to)
+    y = layer(x)
+    assert y.dtype == to and torch.equal(y, (V.int4_gemm(x.to(own), packed, scales, zeros) + bias.to(own).cuda()).to(to))
+    assert model(x).dtype == to
+    assert torch.equal(torch.compile(layer, backend="eager", fullgraph=True)(x), y)
+    up, down = make(64, 128, 64, own, False, (8,)), make(128, 32, 32, own, False, (8,))
+    moe = Int4Experts(torch.nn.Linear(128, 8, bias=False).requires_grad_(False), up, down, top_k=2, in_features=128).cuda().to(to)
+    w, ids = V.route_experts(moe.router(x), 2, renormalize=True)
+    y = moe(x)
+    assert y.dtype == to and torch.equal(y, V.int4_experts(x.to(own), ids, w, up, down).to(to))

@@ -270,11 +270,17 @@ class VQGatedUp(nn.Module):
 
 class _KeptTypes(nn.Module):
     """A module with floating buffers (``_kept``) whose bits matter: casting a model (``.half()``, ``.to(dtype)``) moves them with it and
-    leaves their type."""
+    leaves their type; what the model is cast to becomes the type of the module's results (``result_type``, None before: the
+    module's own)."""
 
     _kept: Tuple[str, ...] = ()
+    result_type: Optional[torch.dtype] = None
 
     def _apply(self, fn, recurse=True):
+        # what fn makes of two types tells a cast from a move
+        to = {fn(torch.empty(0, dtype=t)).dtype for t in (torch.float64, torch.float32)}
+        if len(to) == 1:
+            self.result_type = to.pop()
         before = {name: self._buffers[name] for name in self._kept if self._buffers.get(name) is not None}
         super()._apply(fn, recurse)
         for name, t in before.items():
@@ -283,12 +289,15 @@ class _KeptTypes(nn.Module):
         return self
 
 
-class Int4Linear(nn.Module):
+class Int4Linear(_KeptTypes):
     """``y = x @ W^T (+ bias)`` with 4-bit weights and group scales, for the layers that one or two bits do not serve.
 
     ``packed`` [ceil(out/16), ceil(in/64), 512] uint8, ``scales`` [in/group, out] float16 or bfloat16 -- the layer's type --
     and optionally ``zeros`` [in/group, out] uint8, as ``quantize.int4_quantize`` makes them; ``in_features`` where it is
-    not a multiple of 64.  All are buffers.  Accepts inputs of any leading shape and casts them to the layer's type."""
+    not a multiple of 64.  All are buffers.  Accepts inputs of any leading shape and casts them to the layer's type.  Casting a
+    model leaves the layer's type and weights as they are and has the result in the model's type."""
+
+    _kept = ("scales", "bias")
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
                  bias: Optional[torch.Tensor] = None, in_features: Optional[int] = None):
@@ -319,7 +328,7 @@ class Int4Linear(nn.Module):
         y = torch.ops.vq_gemm_b200.int4_linear(x2.contiguous(), self.packed, self.scales, self.zeros)
         if self.bias is not None:
             y = y + self.bias
-        return y.reshape(*x.shape[:-1], self.out_features)
+        return (y if self.result_type is None else y.to(self.result_type)).reshape(*x.shape[:-1], self.out_features)
 
     def dequantized_weight(self) -> torch.Tensor:
         """The dense [out_features, in_features] weight this layer stands for, bit for bit."""
@@ -335,9 +344,11 @@ class Int4Experts(_KeptTypes):
     ``VQLinear`` or an ``nn.Linear``), then ``route_experts``, then the gated products of the chosen experts.
 
     ``gate_up`` and ``down`` are (packed, scales, zeros or None) of [E, 2 * inner, hidden] and [E, hidden, inner] weights;
-    ``in_features`` is hidden.  ``bias`` [E] float32 is the router's balance bias; it stays float32 when the model is cast."""
+    ``in_features`` is hidden.  ``bias`` [E] float32 is the router's balance bias.  Casting a
+    model casts the router (an ``nn.Linear``, say), leaves the experts' weights and the balance bias as they are and has the result
+    in the model's type."""
 
-    _kept = ("bias",)
+    _kept = ("gate_up_scales", "down_scales", "bias")
 
     def __init__(self, router: nn.Module, gate_up, down, *, top_k: int, in_features: int, scoring: str = "softmax",
                  bias: Optional[torch.Tensor] = None, groups: int = 1, top_groups: Optional[int] = None,
@@ -383,7 +394,7 @@ class Int4Experts(_KeptTypes):
         y = torch.ops.vq_gemm_b200.int4_experts(
             x2.to(self.gate_up_scales.dtype).contiguous(), chosen, weights, self.gate_up_packed, self.gate_up_scales,
             self.gate_up_zeros, self.down_packed, self.down_scales, self.down_zeros)
-        return y.reshape(x.shape)
+        return (y if self.result_type is None else y.to(self.result_type)).reshape(x.shape)
 
     def extra_repr(self) -> str:
         return (f"hidden={self.in_features}, inner={self.inner}, experts={self.experts}, top_k={self.top_k}, "
