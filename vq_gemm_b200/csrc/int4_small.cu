@@ -434,8 +434,8 @@ int launch_one(const SmallParams& p, int rows, cudaStream_t s) {
   if (smem > kSmallSmem) return VQG_ERR_UNSUPPORTED;
   static SmemOptIn opt_in;
   if (smem > 48 * 1024 && !opt_in.ask(kernel)) return VQG_ERR_LAUNCH;
-  // as many blocks as run at once, or one per row group where there are fewer of those
-  const long long slots = static_cast<long long>(sm_count_cached()) * MIN_BLOCKS;
+  // as many blocks as run at once (1 KiB of an SM's shared memory goes with each), or one per row group where there are fewer of those
+  const long long slots = static_cast<long long>(sm_count_cached()) * min(MIN_BLOCKS, static_cast<int>(228 * 1024 / (smem + 1024)));
   const int blocks = static_cast<int>(min(slots, groups * p.chunks));
   return cuda_status(launch_ahead(kernel, dim3(blocks), WARPS * 32, smem, s, take_weights_written(s), p));
 }
@@ -468,7 +468,9 @@ int launch_rows(const SmallParams& p, int rows, bool bf16, cudaStream_t s) {
         return launch_one<F, Z, MODE, 1, 1, 2, 1, 3, 8, 4, 3, 2, false>(p, rows, s);
       }
       if (rows <= 8) {
-        if (x <= 40 * 1024) return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 2, 3, 2, true>(p, rows, s);
+        // X in shared memory while three blocks fit with it (2432 columns, 8 tokens through 64 experts: two blocks 92 us, three that
+        // read X from memory 81)
+        if (x <= 35 * 1024) return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 2, 3, 2, true>(p, rows, s);
         return launch_one<F, Z, MODE, 1, 1, 4, 1, 2, 8, 2, 3, 2, false>(p, rows, s);
       }
       if (x <= 70 * 1024) return launch_one<F, Z, MODE, 2, 1, 4, 1, 2, 8, 2, 2, 1, true>(p, rows, s);
