@@ -7,7 +7,7 @@
 // scoreboard is tied up by a load from memory.  The copies go in memory order, lane i the i-th 16 bytes (in the order in
 // which the lanes need them a quarter warp would touch four lines instead of one, which alone cost 14 of 46 us at 1 x
 // 28672 x 8192), into places that are swizzled so that neither side has bank conflicts: see place().  The sums of a team
-// of warps (one to eight, see below) meet in shared memory.
+// of warps (two, four or eight, see below) meet in shared memory.
 //
 // What bounds it: bytes by the count (half a byte per weight and nothing twice), issue and latency by measurement.  1 x 28672 x
 // 8192 bf16 takes 36.9 us, 3.3 TB/s where a copy reaches 6.5: some 106 instructions of a warp per tile of 16 x 64 weights, half of
@@ -142,7 +142,8 @@ int4_small_kernel(const SmallParams p) {
   constexpr int CH = R * NT == 1 ? 2 : 1;   // chains of accumulators: a matrix instruction waits for the one before it
   constexpr int VALUES = R * NT * 4;        // sums of a lane per row group
   constexpr int BYTES = R * B * 512;
-  constexpr int RED = TW == 1 ? 0 : RGF * VALUES * 128;     // per warp
+  constexpr int RED = RGF * VALUES * 128;     // per warp
+  static_assert(TW > 1, "the sums of a team meet in shared memory");
   extern __shared__ __align__(128) unsigned char smem[];   // rings, sums [team][row group][warp][VALUES][lane], X
   const int warp = (threadIdx.x >> 5) % TW, team = threadIdx.x / (TW * 32), lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -305,24 +306,21 @@ int4_small_kernel(const SmallParams p) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const float sum = CH == 2 ? acc[a][b][0][c] + acc[a][b][CH - 1][c] : acc[a][b][0][c];
-              if constexpr (TW == 1) write(rg, (a * NT + b) * 4 + c, sum);
-              else out[((a * NT + b) * 4 + c) * 32] = sum;
+              out[((a * NT + b) * 4 + c) * 32] = sum;
 #pragma unroll
               for (int d = 0; d < CH; ++d) acc[a][b][d][c] = 0.f;
             }
       }
-      if constexpr (TW > 1) {
-        if (n_red + 1 < RGF && rg + 1 < rg1) continue;
-        asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TW * 32) : "memory");
-        const int with_work = min(TW, (k_tiles + B - 1) / B);   // warps that had a block at all
-        for (int u = warp; u < (n_red + 1) * VALUES; u += TW) {
-          const int r = u / VALUES, q = u % VALUES;
-          float sum = 0.f;
-          for (int k = 0; k < with_work; ++k) sum += red[((r * TW + k) * VALUES + q) * 32 + lane];
-          write(rg - n_red + r, q, sum);
-        }
-        asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TW * 32) : "memory");
+      if (n_red + 1 < RGF && rg + 1 < rg1) continue;
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TW * 32) : "memory");
+      const int with_work = min(TW, (k_tiles + B - 1) / B);   // warps that had a block at all
+      for (int u = warp; u < (n_red + 1) * VALUES; u += TW) {
+        const int r = u / VALUES, q = u % VALUES;
+        float sum = 0.f;
+        for (int k = 0; k < with_work; ++k) sum += red[((r * TW + k) * VALUES + q) * 32 + lane];
+        write(rg - n_red + r, q, sum);
       }
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(TW * 32) : "memory");
     }
     if constexpr (XS) __syncthreads();                          // the rows of X may be overwritten
   }
@@ -430,7 +428,7 @@ template <bool BF16, bool ZEROS, int MODE, int NT, int R, int B, int SPAN, int S
 int launch_one(const SmallParams& p, int rows, cudaStream_t s) {
   auto kernel = int4_small_kernel<BF16, ZEROS, MODE, NT, R, B, SPAN, SLOTS, WARPS, TW, MIN_BLOCKS, RGF, XS>;
   const long long groups = (p.w.row_tiles() + R - 1) / R;
-  const size_t smem = WARPS * (SLOTS * R * B * 512 + (TW == 1 ? 0 : RGF * R * NT * 4 * 128)) + (XS ? static_cast<size_t>(rows) * (p.w.k_tiles() * 128 + 16) : 0);
+  const size_t smem = WARPS * (SLOTS * R * B * 512 + RGF * R * NT * 4 * 128) + (XS ? static_cast<size_t>(rows) * (p.w.k_tiles() * 128 + 16) : 0);
   if (smem > kSmallSmem) return VQG_ERR_UNSUPPORTED;
   static SmemOptIn opt_in;
   if (smem > 48 * 1024 && !opt_in.ask(kernel)) return VQG_ERR_LAUNCH;
@@ -462,7 +460,7 @@ int launch_rows(const SmallParams& p, int rows, bool bf16, cudaStream_t s) {
       }
       return launch_one<F, Z, MODE, 4, 2, 2, 1, 2, 8, 8, 2, 1, false>(p, rows, s);
     } else {
-      // Experts: short rows (a warp alone takes them whole) and many row groups, unless there are few slots.
+      // Experts: short rows and many row groups, so teams of two warps, or of four where there are few slots.
       if (!p.rows.chunks) {
         if (x <= 32 * 1024) return launch_one<F, Z, MODE, 1, 1, 2, 1, 3, 8, 4, 3, 2, true>(p, rows, s);
         return launch_one<F, Z, MODE, 1, 1, 2, 1, 3, 8, 4, 3, 2, false>(p, rows, s);
