@@ -77,3 +77,16 @@ def test_cast_layers_multiply_the_same_weights_and_answer_in_the_models_type(own
     w, ids = V.route_experts(moe.router(x), 2, renormalize=True)
     y = moe(x)
     assert y.dtype == to and torch.equal(y, V.int4_experts(x.to(own), ids, w, up, down).to(to))
+
+
+@pytest.mark.parametrize("dtype,zeros", [(F16, True), (BF16, False)])
+@pytest.mark.parametrize("t,k,e,hidden,inner", [(3, 2, 2, 96, 64), (8, 2, 8, 1024, 512), (12, 2, 8, 1024, 512), (3, 8, 64, 512, 256), (4, 8, 64, 2048, 96),
+                                                (2, 4, 2, 64, 32), (32, 1, 1, 128, 128), (5, 6, 3, 2080, 1024), (4, 2, 2, 4096, 4256)])
+def test_few_slots_either_side_of_the_plan(t, k, e, hidden, inner, dtype, zeros):
+    up, down = make(2 * inner, hidden, 32, dtype, zeros, (e,), seed=t), make(hidden, inner, 32, dtype, zeros, (e,), seed=t + 1)
+    x = acts(t, hidden, dtype, seed=t)
+    ids = torch.randint(-1, e, (t, k), dtype=torch.int32, generator=torch.Generator().manual_seed(t)).cuda()      # repeats and dropped ones
+    w = torch.rand(t, k, generator=torch.Generator().manual_seed(k)).cuda()
+    y = V.int4_experts(x, ids, w, up, down)
+    check(y, O.experts(x, ids, w, up, down))
+    assert torch.equal(V.int4_experts(x, ids, w, up, down), y) and V.device_status() == 0

@@ -51,8 +51,20 @@ Int4Weight weight(const void* packed, const void* scales, const void* zeros, int
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-// Slots up to which a batch is worked on slot by slot, without ordering it by expert.
-constexpr int kDirectSlots = 32;
+// Whether a batch is worked on slot by slot, without ordering it by expert: two launches instead of four or five, but an expert that
+// several slots chose is read and decoded for each of them.  Worth it while what an even routing repeats costs less than the plan:
+// a slot some 1.5 million weights' time beside its own, the plan 26 million's.  Slot by slot and planned, us: 64 experts of 2048 x
+// 1024, 8 a token, 1 token 18 and 27, 2 tokens 30 and 38, 3 tokens 43 and 41, 4 tokens 56 and 51; 8 experts, 2 a token, of 1024 x 512
+// 4 tokens 10.5 and 14, 8 tokens 17 and 14.5, of 4096 x 4096 2 tokens 57 and 64, 4 tokens 99 and 73, 16 tokens 374 and 90, of 4096 x
+// 14336 1 token 88 and 103, 2 tokens 168 and 172, 16 tokens 1213 and 244.
+bool experts_direct(int T, int top_k, int E, int hidden, int inner) {
+  if (static_cast<long long>(T) * top_k > 32) return false;
+  const double share = top_k < E ? static_cast<double>(top_k) / E : 1.0;
+  double missed = 1.0;                                         // by all tokens
+  for (int t = 0; t < T; ++t) missed *= 1.0 - share;
+  const double repeats = T * top_k - E * (1.0 - missed);
+  return repeats * (3.0 * hidden * inner + 1.5e6) <= 26e6;
+}
 
 // The dense product goes to the tensor-memory kernel above 32 rows, above 16 for weights of 2^24 places or more, above 8 for more
 // than 3 * 2^24.  Few-rows kernel and the other: 32 rows of 1024 x 1024 3.6 and 6.8 us, of 4096 x 4096 12.0 and 11.1, of 6144 x
@@ -83,9 +95,9 @@ ExpertScratch expert_scratch(int T, int top_k, int E, int hidden, int inner) {
   const size_t slots = static_cast<size_t>(T) * top_k;
   a.h = 0;
   a.rows = a.h + up(slots * inner * 2);
-  const bool tensor = experts_on_tensor(slots, E, hidden, inner);
-  a.part = a.rows + (tensor && slots > kDirectSlots ? up(slots * hidden * 2) : 0);
-  a.row_slot = a.part + (slots > kDirectSlots ? up(slots * hidden * 4) : 0);
+  const bool tensor = experts_on_tensor(slots, E, hidden, inner), planned = !experts_direct(T, top_k, E, hidden, inner);
+  a.part = a.rows + (tensor && planned ? up(slots * hidden * 2) : 0);
+  a.row_slot = a.part + (planned ? up(slots * hidden * 4) : 0);
   a.chunks = a.row_slot + up(slots * 4);
   a.n_chunks = a.chunks + up(static_cast<size_t>(expert_max_chunks(static_cast<int>(slots), E, expert_chunk_rows(slots, E, tensor))) * sizeof(int4));
   a.total = a.n_chunks + 256;
@@ -192,7 +204,7 @@ int vqg_int4_experts(const void* x, const void* experts, const void* weights, co
   rows.weights = static_cast<const float*>(weights);
   rows.E = E; rows.top_k = top_k; rows.slots = T * top_k;
   void* h = ws + at.h;
-  if (rows.slots <= kDirectSlots) {
+  if (experts_direct(T, top_k, E, hidden, inner)) {
     st = launch_int4_small_gated(gu, x, h, rows, 1, 0, bf16, s);
     if (st != VQG_OK) return st;
     return launch_int4_small_down_direct(dn, h, y, rows, T, bf16, s);
