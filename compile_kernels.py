@@ -8,7 +8,8 @@ that library: the PyTorch-extension shim ``vq_gemm_cuda.so`` at the repository r
 (vq_gemm_b200/csrc/bind.cpp) and the package's native host layer ``vq_gemm_b200/_host.so``
 (vq_gemm_b200/csrc/host.cpp).  There is no Triton, no backend dispatch and no CPU fallback.  The reference's
 ``KERNELS`` environment variable is accepted and ignored: all kernels live in the one library.
-Pass ``--no-shim`` to build only the C-ABI library (seconds instead of a minute or two).
+Pass ``--no-shim`` to build only the C-ABI library (seconds instead of a minute or two): enough for C callers and for the
+Python API but its 4-bit and mixture-of-experts calls, which go through ``_host.so`` and say so where it is missing.
 """
 import os
 import subprocess

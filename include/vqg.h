@@ -338,13 +338,15 @@ VQG_API int vqg_int4_quantize(const void* w, void* packed_out, void* scales_out,
  *   the experts form `groups` equal runs; a run's score is the sum of its two largest choices (group_score 0) or
  *   its largest (1), and only the top_groups best runs take part.  The top_k largest choices give experts_out
  *   [T, top_k] int32 in falling order and weights_out [T, top_k] fp32 = p, divided by their sum if renormalize,
- *   times scale.  Equal choices and equal scores go to the lower index; they are compared in 64 bits, so the
- *   answer is that of exact arithmetic.  An expert whose logit is -inf or NaN is never chosen and takes no part in
- *   the softmax; a slot for which nothing is left gets expert -1 and weight 0.  E <= 512, top_k <= 32, groups <= 32, T <= 2^31 - 512.
+ *   times scale.  Equal choices and equal scores go to the lower index; the order is that of values
+ *   computed in 64 bits (two sigmoids that both round to 1 there are equal).  An expert whose logit is -inf or NaN is
+ *   never chosen and takes no part in the softmax; a slot for which nothing is left gets expert -1 and weight 0.
+ *   E <= 512, top_k <= 32, groups <= 32, T <= 2^31 - 512.
  * vqg_int4_experts: y[t] = sum over j of weights[t, j] * down_e(SiLU(gate_e(x_t)) * up_e(x_t)), e = experts[t, j].
  *   up_* [E, 2 * inner, hidden]: (gate, up) row pairs as in vqg_gemm_swiglu; down_* [E, hidden, inner]; both in the
  *   4-bit format.  A slot whose expert is outside 0 ... E-1 adds nothing (a token with no expert gets zeros); the
- *   same expert twice adds twice.  The gated product is rounded to T, all sums are fp32.  E <= 512.  Workspace of
+ *   same expert twice adds twice.  The gated product is rounded to T (the operand of the second matrix product;
+ *   with bf16 the result is then off by 2.3e-3 of itself instead of 1.7e-3), all sums are fp32.  E <= 512.  Workspace of
  *   vqg_int4_experts_workspace_bytes() bytes, 256-byte aligned, contents arbitrary. */
 VQG_API int vqg_route_experts(const void* logits, const void* bias, void* weights_out, void* experts_out, int T, int E,
                               int top_k, int scoring, int groups, int top_groups, int group_score, int renormalize,

@@ -155,6 +155,8 @@ struct Int4Type<true> {
   __device__ static T from_float(float v) { return __float2bfloat16_rn(v); }
 };
 
+// A code becomes a number by the usual conversion of small integers: its bits go into the low mantissa bits of a power of two whose last
+// place is one (1024 in fp16, 128 in bf16), and a subtraction of that power, here with the zero point, is exact.
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {   // (a & b) | c
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(b), "r"(c));

@@ -166,8 +166,9 @@ __device__ __noinline__ void route_row_64(const RouteParams& p, int token, doubl
 //   * the choice of groups: the same with the groups' scores.
 // Candidates: at least top_k + 1 choices are as large as the (top_k + 1)-th largest of the 32 lanes' maxima, and few more are
 // (about ten in all for 8 of 256).  They go to a list in shared memory and are ranked by comparing each with all of them.
-// The kernel is bound by issue, not by its bytes: 8 of 256 for 16384 tokens takes 18 us, with eight groups and a bias in 64 bits 25 us,
-// where the bytes alone take 2.7; some 1500 instructions of a warp per token.
+// The kernel is bound by issue, not by its bytes (72 % of the issue slots busy, one warp's dependent instructions wait for one another):
+// 8 of 256 for 16384 tokens takes 14.3 us by softmax and 15.3 by sigmoid (730 instructions of a warp per token), by sigmoid with
+// a bias 18.0, with eight groups and a bias 23.2 (1200 instructions), where the bytes alone take 2.7.
 // FULL: there are exactly 32 * EPL experts
 template <int EPL, int TYPE, bool FULL>
 __global__ void __launch_bounds__(kRouteWarps * 32)
